@@ -18,7 +18,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GAN_AMD_LIB") or os.path.join(_HERE, "libgan_amd.so")
 
 GAN_F32, GAN_BF16 = 0, 1
-ABI_VERSION = 25
+ABI_VERSION = 26
 
 _SIGNATURES = {
     "gan_amd_version": (c_int, []),
@@ -72,6 +72,10 @@ _SIGNATURES = {
     "gan_chan_lin2": (c_int, [c_void_p] * 7 + [c_int, c_int64, c_int, c_float, c_int, c_void_p]),
     "gan_layernorm2d_fwd": (c_int, [c_void_p] * 5 + [c_int64, c_int, c_float, c_float, c_int, c_void_p]),
     "gan_layernorm2d_bwd": (c_int, [c_void_p] * 7 + [c_int64, c_int, c_float, c_int, c_void_p]),
+    "gan_layernorm_workspace": (c_int64, [c_int64, c_int64, c_int, c_int, c_int]),
+    "gan_layernorm_fwd": (c_int, [c_void_p] * 5 + [c_int64, c_int64, c_float, c_int, c_void_p, c_int64, c_void_p]),
+    "gan_layernorm_bwd": (c_int, [c_void_p] * 6 + [c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "gan_layernorm_bwd2": (c_int, [c_void_p] * 10 + [c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p]),
     "gan_space_to_depth": (c_int, [c_void_p, c_void_p] + [c_int] * 7 + [c_void_p]),
     "gan_rgb_conv1x1_fwd": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int] + [c_int] * 5 + [c_float, c_void_p]),
     "gan_rgb_conv1x1_dgrad": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_void_p]),

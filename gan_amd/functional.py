@@ -2535,6 +2535,139 @@ def layer_norm2d(x: Tensor, weight: Tensor, bias: Tensor, slope: float = 1.0, ep
     return LayerNorm2dFn.apply(x, weight, bias, slope, eps)
 
 
+def _layer_norm_ws(rows: int, d: int, code: int, order: int, columns: bool, device) -> Tuple[Optional[Tensor], int]:
+    n = _lib.load().gan_layernorm_workspace(rows, d, code, order, int(columns))
+    if n < 0:
+        raise _lib.GanAmdError(f"layer_norm: {rows} rows of {d} elements are not supported")
+    return (torch.empty((n,), dtype=torch.float32, device=device) if n else None), n
+
+
+def raw_layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], d: int, eps: float):
+    """(y, stats (rows, 2)) of contiguous x, normalised over its last d elements."""
+    y = torch.empty_like(x)
+    rows, code = x.numel() // d, dtype_code(x)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        ws, n = _layer_norm_ws(rows, d, code, 0, False, x.device)
+        check(_run("layernorm", 0, _nbytes(x, y),
+                   lambda: _lib.load().gan_layernorm_fwd(ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(stats), rows, d, float(eps), code, ptr(ws), n,
+                                                         stream_of(x)), (rows, d)), "gan_layernorm_fwd")
+    return y, stats
+
+
+def raw_layer_norm_bwd(g: Tensor, x: Tensor, weight: Optional[Tensor], stats: Tensor, d: int, need_x: bool, need_cols: bool):
+    """(gx or None, (2, d) fp32 gradients of weight and bias or None)."""
+    rows, code = x.numel() // d, dtype_code(x)
+    gx = torch.empty_like(x) if need_x else None
+    if rows == 0:
+        return gx, torch.zeros((2, d), dtype=torch.float32, device=x.device) if need_cols else None
+    gwb = torch.empty((2, d), dtype=torch.float32, device=x.device) if need_cols else None
+    with torch.cuda.device(x.device):
+        ws, n = _layer_norm_ws(rows, d, code, 1, need_cols, x.device)
+        check(_run("layernorm_bwd", 0, _nbytes(g, x, gx),
+                   lambda: _lib.load().gan_layernorm_bwd(ptr(g), ptr(x), ptr(weight), ptr(stats), ptr(gx), ptr(gwb), rows, d, code, ptr(ws), n,
+                                                         stream_of(x)), (rows, d)), "gan_layernorm_bwd")
+    return gx, gwb
+
+
+def raw_layer_norm_bwd2(v: Tensor, cw: Optional[Tensor], cb: Optional[Tensor], g: Tensor, x: Tensor, weight: Optional[Tensor], stats: Tensor,
+                        d: int, need_g: bool, need_x: bool, need_w: bool):
+    """The gradients of <v, gx> + <cw, gw> + <cb, gb> (raw_layer_norm_bwd's outputs) with respect to g, x and weight."""
+    rows, code = x.numel() // d, dtype_code(x)
+    gg = torch.empty_like(x) if need_g else None
+    gxx = torch.empty_like(x) if need_x else None
+    if rows == 0:
+        return gg, gxx, torch.zeros((d,), dtype=torch.float32, device=x.device) if need_w else None
+    gww = torch.empty((d,), dtype=torch.float32, device=x.device) if need_w else None
+    with torch.cuda.device(x.device):
+        ws, n = _layer_norm_ws(rows, d, code, 2, need_w, x.device)
+        check(_run("layernorm_bwd2", 0, _nbytes(v, g, x, gg, gxx),
+                   lambda: _lib.load().gan_layernorm_bwd2(ptr(v), ptr(cw), ptr(cb), ptr(g), ptr(x), ptr(weight), ptr(stats), ptr(gg), ptr(gxx),
+                                                          ptr(gww), rows, d, code, ptr(ws), n, stream_of(x)), (rows, d)), "gan_layernorm_bwd2")
+    return gg, gxx, gww
+
+
+class LayerNormFn(Function):
+    """y = (x - mean) * rstd * weight + bias over the last d elements of contiguous x, one launch; the first and the second
+    derivative are kernels too (a gradient penalty through a normalised critic, losses.py:89-103)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, d, eps):
+        w32, b32 = _f32(weight), _f32(bias)
+        xc = x.detach()
+        y, stats = raw_layer_norm(xc, w32, b32, d, eps)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.d = d
+        ctx.meta = tuple(None if t is None else (t.shape, t.dtype) for t in (weight, bias))
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        x, weight, stats = ctx.saved_tensors
+        need = _need(ctx, 0), _need(ctx, 1), _need(ctx, 2)
+        gx, gw, gb = LayerNormBwdFn.apply(g, x, weight, stats, ctx.d, need)
+        w_like, b_like = ctx.meta
+        return gx, (gw.reshape(w_like[0]).to(w_like[1]) if need[1] else None), (gb.reshape(b_like[0]).to(b_like[1]) if need[2] else None), None, None
+
+
+class LayerNormBwdFn(Function):
+    """(g, x, weight) -> the three gradients of LayerNormFn (None where `need` says so); its own backward is one more kernel.
+    Differentiating that one again is refused."""
+
+    @staticmethod
+    def forward(ctx, g, x, weight, stats, d, need):
+        xc, w32 = x.detach(), _f32(weight)
+        gc = g.detach().to(xc.dtype).contiguous()
+        gx, gwb = raw_layer_norm_bwd(gc, xc, w32, stats, d, need[0], need[1] or need[2])
+        ctx.save_for_backward(gc, x, weight, stats)
+        ctx.d, ctx.g_dtype = d, g.dtype
+        ctx.set_materialize_grads(False)
+        return gx, (gwb[0] if need[1] else None), (gwb[1] if need[2] else None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, v, cw, cb):
+        gc, x, weight, stats = ctx.saved_tensors
+        none = (None,) * 6
+        if v is None and cw is None and cb is None:
+            return none
+        vc = torch.zeros_like(gc) if v is None else v.detach().to(gc.dtype).contiguous()
+        gg, gxx, gww = raw_layer_norm_bwd2(vc, _f32(cw), _f32(cb), gc, x.detach(), _f32(weight), stats, ctx.d, _need(ctx, 0), _need(ctx, 1),
+                                           weight is not None and _need(ctx, 2))
+        return (None if gg is None else gg.to(ctx.g_dtype)), gxx, (None if gww is None else gww.reshape(weight.shape).to(weight.dtype)), None, None, None
+
+
+def layer_norm(x: Tensor, normalized_shape, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
+    """torch.nn.functional.layer_norm on the row kernels: float32 or bfloat16 x of any number of dimensions, normalised over
+    its trailing `normalized_shape`; weight and bias (None: ones / zeros) of that shape, any floating type, their gradients
+    summed in float32.  Gradients to second order in x, its cotangent, weight and bias; nothing is kept of x but its rows'
+    mean and 1 / deviation.  A channels-last (N, C, H, W) tensor normalised over whole samples (C, H, W) is read and
+    written as it lies; any other layout is made contiguous first."""
+    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(int(s) for s in normalized_shape)
+    if not shape or any(s <= 0 for s in shape):
+        raise _lib.GanAmdError(f"layer_norm: normalized_shape must be positive sizes, got {shape}")
+    if x.dim() < len(shape) or tuple(x.shape[x.dim() - len(shape):]) != shape:
+        raise _lib.GanAmdError(f"layer_norm: the trailing sizes of {tuple(x.shape)} are not normalized_shape {shape}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and tuple(t.shape) != shape:
+            raise _lib.GanAmdError(f"layer_norm: {name} has shape {tuple(t.shape)}, normalized_shape is {shape}")
+        if t is not None and not t.is_floating_point():
+            raise _lib.GanAmdError(f"layer_norm: {name} must be floating point, got {t.dtype}")
+    if not eps >= 0.0:
+        raise _lib.GanAmdError(f"layer_norm: eps must not be negative, got {eps}")
+    dtype_code(x)
+    require_gpu(x, weight, bias)
+    if any(t is not None and t.device != x.device for t in (weight, bias)):
+        raise _lib.GanAmdError("layer_norm: x, weight and bias must be on one device")
+    d = 1
+    for s in shape:
+        d *= s
+    if x.dim() == 4 and len(shape) == 3 and not x.is_contiguous() and x.is_contiguous(memory_format=CL):
+        flat = [None if t is None else t.permute(1, 2, 0).reshape(d) for t in (weight, bias)]
+        return LayerNormFn.apply(x.permute(0, 2, 3, 1), *flat, d, float(eps)).permute(0, 3, 1, 2)
+    return LayerNormFn.apply(x.contiguous(), weight, bias, d, float(eps))
+
+
 class MbstdConcatFn(Function):
     """(x (N, C, H, W), stat (N/G,)) -> (N, C+1, H, W): the statistic of each sample's group column appended as a
     constant plane (progressive_gan.py:31-36), one launch.  Linear in both arguments; its adjoint is

@@ -101,6 +101,15 @@ class LayerNorm2d(nn.LayerNorm):
         return self.fused(x, 1.0)
 
 
+class LayerNorm(nn.LayerNorm):
+    """nn.LayerNorm over trailing dimensions on the row kernels (functional.layer_norm), in the compute dtype (the autocast
+    dtype if autocast is on).  Over whole samples, LayerNorm((C, H, W)), it is the normalisation that critics under a
+    gradient penalty take in place of batch norm: every sample keeps a gradient of its own, to second order."""
+
+    def forward(self, x: Tensor) -> Tensor:
+        return GF.layer_norm(x.to(GF.act_dtype(x)), self.normalized_shape, self.weight, self.bias, self.eps)
+
+
 def get_norm(norm: str, dim: int):
     """modelling/common.py:27-33 ("instance" is only used by models outside this build's scope)."""
     return dict(none=nn.Identity, batch=partial(nn.BatchNorm2d, track_running_stats=False), layer=LayerNorm2d)[norm](dim)

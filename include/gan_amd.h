@@ -338,6 +338,26 @@ int gan_diffaug(const void* in, int64_t sn, int64_t sc, int64_t sh, int64_t sw, 
  * H, W, C always describe the un-folded tensor. */
 int gan_space_to_depth(const void* x, void* out, int N, int H, int W, int C, int pad, int to_depth, int dtype, gan_stream_t stream);
 
+/* ---- layer norm over the rows of a dense (rows, D) matrix: forward, backward, second order ---------------------
+ * With m, r = (mean, 1 / sqrt(biased variance + eps)) of a row, t = (x - m) r and P(u) = u - mean(u) - t mean(u t):
+ * gan_layernorm_fwd : y = t * w + b; stats [rows][2] = (m, r), kept for the other two.
+ * gan_layernorm_bwd : gx = r P(g w); gwb [2][D] = (sum over rows of g t, of g).  Either may be NULL (skipped).
+ * gan_layernorm_bwd2: the gradients of <v, gx> + <cw, gwb[0]> + <cb, gwb[1]> with respect to g (gg), x (gxx) and w (gww [D]);
+ *                     any output may be NULL, cw and cb may be NULL (no such cotangent).
+ * w NULL: ones; b NULL: zeros.  w, b, cw, cb, stats, gwb, gww are fp32; x, y, g, v, gx, gg, gxx of `dtype`, aligned to their
+ * element only (any D); no output may overlap an input.  Column sums are added in an order that depends on the shape alone.
+ * 1 <= D <= 2^30.
+ * workspace: gan_layernorm_workspace floats (pass 0 forward, 1 backward, 2 second; columns: gwb / gww wanted), 16-byte
+ * aligned, may be NULL where that is 0; negative: the shape is refused. */
+int64_t gan_layernorm_workspace(int64_t rows, int64_t D, int dtype, int pass, int columns);
+int gan_layernorm_fwd(const void* x, const float* w, const float* b, void* y, float* stats, int64_t rows, int64_t D, float eps, int dtype,
+                      float* ws, int64_t ws_floats, gan_stream_t stream);
+int gan_layernorm_bwd(const void* g, const void* x, const float* w, const float* stats, void* gx, float* gwb, int64_t rows, int64_t D, int dtype,
+                      float* ws, int64_t ws_floats, gan_stream_t stream);
+int gan_layernorm_bwd2(const void* v, const float* cw, const float* cb, const void* g, const void* x, const float* w, const float* stats,
+                       void* gg, void* gxx, float* gww, int64_t rows, int64_t D, int dtype, float* ws, int64_t ws_floats,
+                       gan_stream_t stream);
+
 /* ---- AdaIN / LayerNorm2d (the StyleGAN-v1 and Progressive-GAN generators) ------------------------------------
  * replaces AdaIN.forward              modelling/common.py:13-16   F.instance_norm(x) * (style_w(w) + 1) + style_b(w)
  *          LayerNorm2d.forward        modelling/common.py:20-24   nn.LayerNorm over the channels of each pixel
