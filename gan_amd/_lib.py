@@ -5,6 +5,7 @@ ROCm device, the calls here raise -- nothing in this package computes on the CPU
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
@@ -155,3 +156,11 @@ def ptr(t: Optional[Tensor]):
 
 def stream_of(t: Tensor):
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on_device(t: Tensor):
+    """Context in which t's device is the current one (launches go to the current device's context)."""
+    return _HERE_ALREADY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)

@@ -8,8 +8,8 @@
 //             gxx = r P(g cw - r (v mean(h t) + h mean(v t))) - r^2 t (mean(v h) - mean v mean h - mean(v t) mean(h t))
 //             gww = sum_rows g r P(v)
 // All three move a few bytes per flop: HBM bounds them.  Each row is read once and kept in registers, 16 bytes a lane and
-// load, between its statistics and its results; a row belongs to TPR threads (16 ... 1024), the fewest that hold it in at
-// most four vectors each, so that short rows need no LDS and the widest still one launch.  Longer rows are cut into pieces
+// load, between its statistics and its results; a row belongs to TPR threads (16 ... 512) with one or two
+// such vectors each (four in the widest), so that short rows need no LDS and registers leave room for many waves.  Longer rows are cut into pieces
 // that first sum and then, in a second launch, join the sums and write.
 // Column sums: where a workgroup walks over many rows, its threads keep their columns' sums in registers and write one
 // partial row per workgroup (fold_cols_k adds those in a fixed order: no atomics, the same bits on every run); where there
@@ -146,7 +146,7 @@ struct RowArgs {
 
 template <int TPR>
 constexpr int block_of() {
-    return TPR <= 256 ? TPB : TPR;
+    return TPR <= TPB ? TPB : TPR;
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------
@@ -311,7 +311,7 @@ struct SecondRow {
     }
 };
 
-template <typename T, int TPR, int K, bool COLS>
+template <typename T, int TPR, int K, bool COLS, bool CC>  // CC: cotangents of the column sums are there
 __global__ void __launch_bounds__(block_of<TPR>()) ln_bwd2_k(const RowArgs a) {
     constexpr int V = VecOf<T>::V, BLK = block_of<TPR>(), G = BLK / TPR;
     __shared__ float lds[2 * NS2 * 16];
@@ -334,13 +334,15 @@ __global__ void __launch_bounds__(block_of<TPR>()) ln_bwd2_k(const RowArgs a) {
         const float2 st = a.stats[row];
         float w[K][V], cw[K][V], cb[K][V];
         load_cols<V, K, TPR>(a.w, 1.f, w, lane, D);
-        load_cols<V, K, TPR>(a.cw, 0.f, cw, lane, D);
-        load_cols<V, K, TPR>(a.cb, 0.f, cb, lane, D);
+        if (CC) {
+            load_cols<V, K, TPR>(a.cw, 0.f, cw, lane, D);
+            load_cols<V, K, TPR>(a.cb, 0.f, cb, lane, D);
+        }
         float s[NS2] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int e = 0; e < V; ++e) second_sums(x.at(k, e), g.at(k, e), v.at(k, e), w[k][e], cw[k][e], st, s);
+            for (int e = 0; e < V; ++e) second_sums(x.at(k, e), g.at(k, e), v.at(k, e), w[k][e], CC ? cw[k][e] : 0.f, st, s);
         row_sum<NS2, TPR>(s, lds, flip);
         const SecondRow sr(st, s, inv);
         if (a.vstats && lane == 0) a.vstats[row] = make_float2(sr.vm, sr.vt);
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(block_of<TPR>()) ln_bwd2_k(const RowArgs a) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 float gxx, gg, gw;
-                sr.at(x.at(k, e), g.at(k, e), v.at(k, e), w[k][e], cw[k][e], cb[k][e], gxx, gg, gw);
+                sr.at(x.at(k, e), g.at(k, e), v.at(k, e), w[k][e], CC ? cw[k][e] : 0.f, CC ? cb[k][e] : 0.f, gxx, gg, gw);
                 x.v[k].e[e] = (T)gxx;
                 v.v[k].e[e] = (T)gg;
                 if (COLS) acc[0][k][e] += gw;
@@ -616,23 +618,20 @@ Plan plan_of(int64_t rows, int64_t D, int dtype, int pass, bool cols) {
     const int64_t nv = (D + V - 1) / V;
     const int ncol = pass == 2 ? 1 : 2;
     if (nv <= 64) {
-        p.tpr = 16;
-        p.k = nv <= 16 ? 1 : nv <= 32 ? 2 : 4;
-    } else if (nv <= 256) {
-        p.tpr = 64;
-        p.k = nv <= 128 ? 2 : 4;
-    } else if (nv <= 1024) {
-        p.tpr = 256;
-        p.k = nv <= 512 ? 2 : 4;
-    } else if (nv <= 4096) {
-        p.tpr = 1024;
-        p.k = nv <= 2048 ? 2 : 4;
+        p.tpr = nv <= 16 ? 16 : 64;
+        p.k = 1;
+    } else if (nv <= 512) {
+        p.tpr = nv <= 128 ? 64 : 256;
+        p.k = nv <= 128 || nv > 256 ? 2 : 1;
+    } else if (nv <= 2048) {
+        p.tpr = 512;
+        p.k = nv <= 1024 ? 2 : 4;
     }
     if (p.tpr) {
-        const int g = p.tpr >= 256 ? 1 : TPB / p.tpr;
+        const int g = p.tpr >= TPB ? 1 : TPB / p.tpr;
         const int64_t need = ceil_div64(rows, g);
         p.blocks = (int)(need < MAXB ? need : MAXB);
-        if (cols && pass > 0 && p.tpr <= 256) {
+        if (cols && pass > 0) {
             // A partial row of ncol D floats per workgroup is written and read again, next to at least three tensor rows of D
             // elements that a row costs anyway: few enough workgroups keep that under a sixth.  Where so few are left that
             // they would not fill the chip, a kernel down the columns reads the tensors a second time instead.
@@ -665,30 +664,27 @@ Plan plan_of(int64_t rows, int64_t D, int dtype, int pass, bool cols) {
 template <typename T, int PASS, bool COLS, int TPR, int K>
 void launch_row(const Plan& p, const RowArgs& a, hipStream_t st) {
     constexpr int BLK = block_of<TPR>();
-    const size_t lds = COLS && TPR < 256 ? sizeof(float) * (PASS == 2 ? 1 : 2) * (size_t)a.D : 0;
+    const size_t lds = COLS && TPR < TPB ? sizeof(float) * (PASS == 2 ? 1 : 2) * (size_t)a.D : 0;
     if constexpr (PASS == 0)
         hipLaunchKernelGGL((ln_fwd_k<T, TPR, K>), dim3(p.blocks), dim3(BLK), 0, st, a);
     else if constexpr (PASS == 1)
         hipLaunchKernelGGL((ln_bwd_k<T, TPR, K, COLS>), dim3(p.blocks), dim3(BLK), lds, st, a);
+    else if (a.cw || a.cb)
+        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS, true>), dim3(p.blocks), dim3(BLK), lds, st, a);
     else
-        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS>), dim3(p.blocks), dim3(BLK), lds, st, a);
+        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS, false>), dim3(p.blocks), dim3(BLK), lds, st, a);
 }
 
 template <typename T, int PASS, bool COLS>
 void launch_rows(const Plan& p, const RowArgs& a, hipStream_t st) {
-    if (p.tpr == 16) {
-        if (p.k == 1) launch_row<T, PASS, COLS, 16, 1>(p, a, st);
-        else if (p.k == 2) launch_row<T, PASS, COLS, 16, 2>(p, a, st);
-        else launch_row<T, PASS, COLS, 16, 4>(p, a, st);
-    } else if (p.tpr == 64) {
-        if (p.k == 2) launch_row<T, PASS, COLS, 64, 2>(p, a, st);
-        else launch_row<T, PASS, COLS, 64, 4>(p, a, st);
-    } else if (p.tpr == 256) {
-        if (p.k == 2) launch_row<T, PASS, COLS, 256, 2>(p, a, st);
-        else launch_row<T, PASS, COLS, 256, 4>(p, a, st);
-    } else if constexpr (!COLS) {
-        if (p.k == 2) launch_row<T, PASS, COLS, 1024, 2>(p, a, st);
-        else launch_row<T, PASS, COLS, 1024, 4>(p, a, st);
+    switch (p.tpr * 8 + p.k) {
+        case 16 * 8 + 1: return launch_row<T, PASS, COLS, 16, 1>(p, a, st);
+        case 64 * 8 + 1: return launch_row<T, PASS, COLS, 64, 1>(p, a, st);
+        case 64 * 8 + 2: return launch_row<T, PASS, COLS, 64, 2>(p, a, st);
+        case 256 * 8 + 1: return launch_row<T, PASS, COLS, 256, 1>(p, a, st);
+        case 256 * 8 + 2: return launch_row<T, PASS, COLS, 256, 2>(p, a, st);
+        case 512 * 8 + 2: return launch_row<T, PASS, COLS, 512, 2>(p, a, st);
+        default: return launch_row<T, PASS, COLS, 512, 4>(p, a, st);
     }
 }
 

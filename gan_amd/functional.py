@@ -20,6 +20,8 @@ these primitives.
 from __future__ import annotations
 
 import contextlib
+import functools
+import math
 import os
 import weakref
 from typing import Dict, Optional, Tuple
@@ -30,7 +32,7 @@ from torch import Tensor
 from torch.autograd import Function as _TorchFunction
 
 from . import _lib
-from ._lib import check, dtype_code, ptr, require_gpu, stream_of
+from ._lib import check, dtype_code, on_device, ptr, require_gpu, stream_of
 
 CL = torch.channels_last
 
@@ -2535,22 +2537,24 @@ def layer_norm2d(x: Tensor, weight: Tensor, bias: Tensor, slope: float = 1.0, ep
     return LayerNorm2dFn.apply(x, weight, bias, slope, eps)
 
 
-def _layer_norm_ws(rows: int, d: int, code: int, order: int, columns: bool, device) -> Tuple[Optional[Tensor], int]:
+@functools.lru_cache(maxsize=256)
+def _layer_norm_ws(rows: int, d: int, code: int, order: int, columns: bool) -> int:
     n = _lib.load().gan_layernorm_workspace(rows, d, code, order, int(columns))
     if n < 0:
         raise _lib.GanAmdError(f"layer_norm: {rows} rows of {d} elements are not supported")
-    return (torch.empty((n,), dtype=torch.float32, device=device) if n else None), n
+    return n
 
 
 def raw_layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], d: int, eps: float):
     """(y, stats (rows, 2)) of contiguous x, normalised over its last d elements."""
     y = torch.empty_like(x)
     rows, code = x.numel() // d, dtype_code(x)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        ws, n = _layer_norm_ws(rows, d, code, 0, False, x.device)
+    n = _layer_norm_ws(rows, d, code, 0, False)
+    stats = x.new_empty((rows, 2), dtype=torch.float32)
+    ws = x.new_empty((n,), dtype=torch.float32) if n else None
+    with on_device(x):
         check(_run("layernorm", 0, _nbytes(x, y),
-                   lambda: _lib.load().gan_layernorm_fwd(ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(stats), rows, d, float(eps), code, ptr(ws), n,
+                   lambda: _lib.load().gan_layernorm_fwd(ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(stats), rows, d, eps, code, ptr(ws), n,
                                                          stream_of(x)), (rows, d)), "gan_layernorm_fwd")
     return y, stats
 
@@ -2561,9 +2565,10 @@ def raw_layer_norm_bwd(g: Tensor, x: Tensor, weight: Optional[Tensor], stats: Te
     gx = torch.empty_like(x) if need_x else None
     if rows == 0:
         return gx, torch.zeros((2, d), dtype=torch.float32, device=x.device) if need_cols else None
-    gwb = torch.empty((2, d), dtype=torch.float32, device=x.device) if need_cols else None
-    with torch.cuda.device(x.device):
-        ws, n = _layer_norm_ws(rows, d, code, 1, need_cols, x.device)
+    gwb = x.new_empty((2, d), dtype=torch.float32) if need_cols else None
+    n = _layer_norm_ws(rows, d, code, 1, need_cols)
+    ws = x.new_empty((n,), dtype=torch.float32) if n else None
+    with on_device(x):
         check(_run("layernorm_bwd", 0, _nbytes(g, x, gx),
                    lambda: _lib.load().gan_layernorm_bwd(ptr(g), ptr(x), ptr(weight), ptr(stats), ptr(gx), ptr(gwb), rows, d, code, ptr(ws), n,
                                                          stream_of(x)), (rows, d)), "gan_layernorm_bwd")
@@ -2578,9 +2583,10 @@ def raw_layer_norm_bwd2(v: Tensor, cw: Optional[Tensor], cb: Optional[Tensor], g
     gxx = torch.empty_like(x) if need_x else None
     if rows == 0:
         return gg, gxx, torch.zeros((d,), dtype=torch.float32, device=x.device) if need_w else None
-    gww = torch.empty((d,), dtype=torch.float32, device=x.device) if need_w else None
-    with torch.cuda.device(x.device):
-        ws, n = _layer_norm_ws(rows, d, code, 2, need_w, x.device)
+    gww = x.new_empty((d,), dtype=torch.float32) if need_w else None
+    n = _layer_norm_ws(rows, d, code, 2, need_w)
+    ws = x.new_empty((n,), dtype=torch.float32) if n else None
+    with on_device(x):
         check(_run("layernorm_bwd2", 0, _nbytes(v, g, x, gg, gxx),
                    lambda: _lib.load().gan_layernorm_bwd2(ptr(v), ptr(cw), ptr(cb), ptr(g), ptr(x), ptr(weight), ptr(stats), ptr(gg), ptr(gxx),
                                                           ptr(gww), rows, d, code, ptr(ws), n, stream_of(x)), (rows, d)), "gan_layernorm_bwd2")
@@ -2593,33 +2599,39 @@ class LayerNormFn(Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, d, eps):
-        w32, b32 = _f32(weight), _f32(bias)
-        xc = x.detach()
-        y, stats = raw_layer_norm(xc, w32, b32, d, eps)
-        ctx.save_for_backward(x, weight, stats)
+        w32 = _f32(weight)
+        y, stats = raw_layer_norm(x.detach(), w32, _f32(bias), d, eps)
+        ctx.save_for_backward(x, weight, w32, stats)
         ctx.d = d
-        ctx.meta = tuple(None if t is None else (t.shape, t.dtype) for t in (weight, bias))
+        ctx.bias_like = None if bias is None else (bias.shape, bias.dtype)
         return y
 
     @staticmethod
     def backward(ctx, g):
-        x, weight, stats = ctx.saved_tensors
-        need = _need(ctx, 0), _need(ctx, 1), _need(ctx, 2)
-        gx, gw, gb = LayerNormBwdFn.apply(g, x, weight, stats, ctx.d, need)
-        w_like, b_like = ctx.meta
-        return gx, (gw.reshape(w_like[0]).to(w_like[1]) if need[1] else None), (gb.reshape(b_like[0]).to(b_like[1]) if need[2] else None), None, None
+        x, weight, w32, stats = ctx.saved_tensors
+        cols = _need(ctx, 1)  # the bias's gradient comes with the weight's: one question to the engine for both
+        need = _need(ctx, 0), cols, ctx.needs_input_grad[2] if cols else _need(ctx, 2)
+        if torch.is_grad_enabled():
+            gx, gw, gb = LayerNormBwdFn.apply(g, x, weight, w32, stats, ctx.d, need)
+        else:
+            gx, gwb = raw_layer_norm_bwd(g.to(x.dtype).contiguous(), x, w32, stats, ctx.d, need[0], need[1] or need[2])
+            gw, gb = (None, None) if gwb is None else gwb.unbind(0)
+        if need[1]:
+            gw = gw.view(weight.shape).to(weight.dtype)
+        if need[2]:
+            gb = gb.view(ctx.bias_like[0]).to(ctx.bias_like[1])
+        return gx, (gw if need[1] else None), (gb if need[2] else None), None, None
 
 
 class LayerNormBwdFn(Function):
-    """(g, x, weight) -> the three gradients of LayerNormFn (None where `need` says so); its own backward is one more kernel.
-    Differentiating that one again is refused."""
+    """(g, x, weight) -> the three gradients of LayerNormFn (None where `need` says so) inside a create_graph region; its own
+    backward is one more kernel.  Differentiating that one again is refused."""
 
     @staticmethod
-    def forward(ctx, g, x, weight, stats, d, need):
-        xc, w32 = x.detach(), _f32(weight)
-        gc = g.detach().to(xc.dtype).contiguous()
-        gx, gwb = raw_layer_norm_bwd(gc, xc, w32, stats, d, need[0], need[1] or need[2])
-        ctx.save_for_backward(gc, x, weight, stats)
+    def forward(ctx, g, x, weight, w32, stats, d, need):
+        gc = g.detach().to(x.dtype).contiguous()
+        gx, gwb = raw_layer_norm_bwd(gc, x.detach(), w32, stats, d, need[0], need[1] or need[2])
+        ctx.save_for_backward(gc, x, weight, w32, stats)
         ctx.d, ctx.g_dtype = d, g.dtype
         ctx.set_materialize_grads(False)
         return gx, (gwb[0] if need[1] else None), (gwb[1] if need[2] else None)
@@ -2627,14 +2639,13 @@ class LayerNormBwdFn(Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, v, cw, cb):
-        gc, x, weight, stats = ctx.saved_tensors
-        none = (None,) * 6
+        gc, x, weight, w32, stats = ctx.saved_tensors
         if v is None and cw is None and cb is None:
-            return none
-        vc = torch.zeros_like(gc) if v is None else v.detach().to(gc.dtype).contiguous()
-        gg, gxx, gww = raw_layer_norm_bwd2(vc, _f32(cw), _f32(cb), gc, x.detach(), _f32(weight), stats, ctx.d, _need(ctx, 0), _need(ctx, 1),
+            return (None,) * 7
+        vc = torch.zeros_like(gc) if v is None else v.to(gc.dtype).contiguous()
+        gg, gxx, gww = raw_layer_norm_bwd2(vc, _f32(cw), _f32(cb), gc, x, w32, stats, ctx.d, _need(ctx, 0), _need(ctx, 1),
                                            weight is not None and _need(ctx, 2))
-        return (None if gg is None else gg.to(ctx.g_dtype)), gxx, (None if gww is None else gww.reshape(weight.shape).to(weight.dtype)), None, None, None
+        return (None if gg is None else gg.to(ctx.g_dtype)), gxx, (None if gww is None else gww.view(weight.shape).to(weight.dtype)), None, None, None, None
 
 
 def layer_norm(x: Tensor, normalized_shape, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
@@ -2643,29 +2654,31 @@ def layer_norm(x: Tensor, normalized_shape, weight: Optional[Tensor] = None, bia
     summed in float32.  Gradients to second order in x, its cotangent, weight and bias; nothing is kept of x but its rows'
     mean and 1 / deviation.  A channels-last (N, C, H, W) tensor normalised over whole samples (C, H, W) is read and
     written as it lies; any other layout is made contiguous first."""
-    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(int(s) for s in normalized_shape)
-    if not shape or any(s <= 0 for s in shape):
+    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+    d = math.prod(shape)
+    if not shape or min(shape) <= 0:
         raise _lib.GanAmdError(f"layer_norm: normalized_shape must be positive sizes, got {shape}")
-    if x.dim() < len(shape) or tuple(x.shape[x.dim() - len(shape):]) != shape:
+    if x.shape[-len(shape):] != shape:
         raise _lib.GanAmdError(f"layer_norm: the trailing sizes of {tuple(x.shape)} are not normalized_shape {shape}")
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and tuple(t.shape) != shape:
+        if t is None:
+            continue
+        if t.shape != shape:
             raise _lib.GanAmdError(f"layer_norm: {name} has shape {tuple(t.shape)}, normalized_shape is {shape}")
-        if t is not None and not t.is_floating_point():
+        if not t.is_floating_point():
             raise _lib.GanAmdError(f"layer_norm: {name} must be floating point, got {t.dtype}")
+        if t.device != x.device:
+            raise _lib.GanAmdError(f"layer_norm: x is on {x.device}, {name} on {t.device}")
     if not eps >= 0.0:
         raise _lib.GanAmdError(f"layer_norm: eps must not be negative, got {eps}")
     dtype_code(x)
-    require_gpu(x, weight, bias)
-    if any(t is not None and t.device != x.device for t in (weight, bias)):
-        raise _lib.GanAmdError("layer_norm: x, weight and bias must be on one device")
-    d = 1
-    for s in shape:
-        d *= s
-    if x.dim() == 4 and len(shape) == 3 and not x.is_contiguous() and x.is_contiguous(memory_format=CL):
+    require_gpu(x)
+    if x.is_contiguous():
+        return LayerNormFn.apply(x, weight, bias, d, eps)
+    if x.dim() == 4 and len(shape) == 3 and x.is_contiguous(memory_format=CL):
         flat = [None if t is None else t.permute(1, 2, 0).reshape(d) for t in (weight, bias)]
-        return LayerNormFn.apply(x.permute(0, 2, 3, 1), *flat, d, float(eps)).permute(0, 3, 1, 2)
-    return LayerNormFn.apply(x.contiguous(), weight, bias, d, float(eps))
+        return LayerNormFn.apply(x.permute(0, 2, 3, 1), *flat, d, eps).permute(0, 3, 1, 2)
+    return LayerNormFn.apply(x.contiguous(), weight, bias, d, eps)
 
 
 class MbstdConcatFn(Function):
