@@ -2593,6 +2593,12 @@ def raw_layer_norm_bwd2(v: Tensor, cw: Optional[Tensor], cb: Optional[Tensor], g
     return gg, gxx, gww
 
 
+def _not_a_leaf(t: Optional[Tensor]) -> Optional[Tensor]:
+    """t itself, or a view of it where it is a leaf that takes gradients.  Whether torch.autograd.grad() wants a leaf can only
+    be asked by way of an exception (_need), and raising one costs 15 us, six times what the view does."""
+    return t.view_as(t) if t is not None and t.requires_grad and t.is_leaf else t
+
+
 class LayerNormFn(Function):
     """y = (x - mean) * rstd * weight + bias over the last d elements of contiguous x, one launch; the first and the second
     derivative are kernels too (a gradient penalty through a normalised critic, losses.py:89-103)."""
@@ -2612,7 +2618,7 @@ class LayerNormFn(Function):
         cols = _need(ctx, 1)  # the bias's gradient comes with the weight's: one question to the engine for both
         need = _need(ctx, 0), cols, ctx.needs_input_grad[2] if cols else _need(ctx, 2)
         if torch.is_grad_enabled():
-            gx, gw, gb = LayerNormBwdFn.apply(g, x, weight, w32, stats, ctx.d, need)
+            gx, gw, gb = LayerNormBwdFn.apply(_not_a_leaf(g), x, weight, w32, stats, ctx.d, need)
         else:
             gx, gwb = raw_layer_norm_bwd(g.to(x.dtype).contiguous(), x, w32, stats, ctx.d, need[0], need[1] or need[2])
             gw, gb = (None, None) if gwb is None else gwb.unbind(0)
@@ -2673,6 +2679,8 @@ def layer_norm(x: Tensor, normalized_shape, weight: Optional[Tensor] = None, bia
         raise _lib.GanAmdError(f"layer_norm: eps must not be negative, got {eps}")
     dtype_code(x)
     require_gpu(x)
+    if torch.is_grad_enabled():
+        x, weight = _not_a_leaf(x), _not_a_leaf(weight)
     if x.is_contiguous():
         return LayerNormFn.apply(x, weight, bias, d, eps)
     if x.dim() == 4 and len(shape) == 3 and x.is_contiguous(memory_format=CL):
