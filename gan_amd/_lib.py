@@ -21,6 +21,12 @@ LIB_PATH = os.environ.get("GAN_AMD_LIB") or os.path.join(_HERE, "libgan_amd.so")
 GAN_F32, GAN_BF16 = 0, 1
 ABI_VERSION = 26
 
+class Matrix(ctypes.Structure):
+    """gan_matrix of include/gan_amd.h"""
+
+    _fields_ = [("g", c_void_p), ("buf", c_void_p), ("out", c_void_p), ("rows", c_int64), ("cols", c_int64), ("batch", c_int64)]
+
+
 _SIGNATURES = {
     "gan_amd_version": (c_int, []),
     "gan_amd_arch": (c_char_p, []),
@@ -95,6 +101,9 @@ _SIGNATURES = {
     "gan_conv2d_fwd_short": (c_int, [c_void_p] * 4 + [c_float, c_float, c_void_p, c_void_p, c_int, c_float] + [c_int] * 11 + [c_void_p]),
     "gan_scale_rows": (c_int, [c_void_p] * 5 + [c_int, c_int64, c_void_p]),
     "gan_scale_rows_bwd": (c_int, [c_void_p] * 5 + [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int64, c_void_p]),
+    "gan_orthogonalize_workspace": (c_int64, [c_void_p, c_int]),
+    "gan_orthogonalize": (c_int, [c_void_p, c_int, c_int] + [c_float] * 4 + [c_int, c_void_p, c_int64, c_void_p]),
+    "gan_muon_step": (c_int, [c_void_p, c_int, c_float, c_float, c_int, c_float, c_int, c_int] + [c_float] * 4 + [c_void_p, c_int64, c_void_p]),
     "gan_adam_step": (c_int, [c_void_p] * 4 + [c_int64, c_void_p, c_int] + [c_float] * 5 + [c_int, c_void_p]),
 }
 

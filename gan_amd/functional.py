@@ -20,6 +20,7 @@ these primitives.
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import functools
 import math
 import os
@@ -1007,6 +1008,52 @@ def raw_ema_lerp(ema_flat: Tensor, p_flat: Tensor, weight: float) -> None:
     assert ema_flat.dtype == torch.float32 and p_flat.dtype == torch.float32
     assert ema_flat.is_contiguous() and p_flat.is_contiguous() and ema_flat.numel() == p_flat.numel()
     check(lib.gan_ema_lerp(ptr(ema_flat), ptr(p_flat), ema_flat.numel(), float(weight), stream_of(ema_flat)), "gan_ema_lerp")
+
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def matrix_workspace(mats, device) -> Tuple[Optional[Tensor], int]:
+    """(workspace of gan_orthogonalize / gan_muon_step for an array of _lib.Matrix, its bytes)."""
+    n = _lib.load().gan_orthogonalize_workspace(ctypes.addressof(mats), len(mats))
+    if n < 0:
+        sizes = sorted({(m.rows, m.cols) for m in mats}, key=max)
+        raise _lib.GanAmdError(f"orthogonalize: matrices of 1 to 2^20 rows and columns, the smaller side at most 32768; got up to {sizes[-1]}")
+    return (torch.empty((n,), dtype=torch.uint8, device=device) if n else None), n
+
+
+def ortho_flops(rows: int, cols: int, steps: int) -> float:
+    """Operations of the products as they run: three 16-bit ones for each, the symmetric ones by half."""
+    m, n = min(rows, cols), max(rows, cols)
+    return 3.0 * steps * (3.0 * m * m * n + float(m) ** 3)
+
+
+def orthogonalize(x: Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7) -> Tensor:
+    """The nearest matrix with orthonormal rows or columns, approximately: x (..., m, n) in float32 or bfloat16 is divided by
+    max(its Frobenius norm, eps), then taken `steps` times through X <- a X + (b A + c A A) X with A = X X' (Newton-Schulz; a
+    tall x is worked on as its transpose).  With the default coefficients and five steps the singular values end between
+    0.7 and 1.2.  Each matrix of a batch is one of its own.  Products carry 22 bits of every factor and fp32 sums, for
+    bfloat16 too (whose result is rounded once); zeros stay zeros, and a matrix with a value that is not finite comes back as
+    NaN.  An update rule, not a layer: there is no derivative, x must not require one."""
+    if x.dim() < 2:
+        raise _lib.GanAmdError(f"orthogonalize: expected (..., m, n), got shape {tuple(x.shape)}")
+    a, b, c = (float(v) for v in coefficients)
+    code = dtype_code(x)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise _lib.GanAmdError("orthogonalize has no derivative: detach x or call it under torch.no_grad()")
+    require_gpu(x)
+    x = x.detach().contiguous()
+    out = torch.empty_like(x)
+    m, n = x.shape[-2:]
+    if x.numel() == 0:
+        return out
+    mats = (_lib.Matrix * 1)(_lib.Matrix(ptr(x), None, ptr(out), m, n, x.numel() // (m * n)))
+    ws, nbytes = matrix_workspace(mats, x.device)
+    with on_device(x):
+        check(_run("orthogonalize", mats[0].batch * ortho_flops(m, n, steps), _nbytes(x, out),
+                   lambda: _lib.load().gan_orthogonalize(ctypes.addressof(mats), 1, int(steps), a, b, c, float(eps), code, ptr(ws), nbytes,
+                                                         stream_of(x)), (mats[0].batch, m, n)), "gan_orthogonalize")
+    return out
 
 
 # ======================================================================================

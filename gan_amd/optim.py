@@ -9,14 +9,16 @@ for that, which costs a launch per parameter tensor for each bias-correction sca
 for the two StyleGAN2 networks)."""
 from __future__ import annotations
 
-from typing import Dict, List, Tuple
+import ctypes
+import math
+from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
-from torch import nn
+from torch import Tensor, nn
 
 from . import _lib
 from . import functional as GF
-from ._lib import check, ptr, stream_of
+from ._lib import check, ptr, require_gpu, stream_of
 from .utils import FlatArena, arena_of
 
 _FLAT_KEYS = {"betas", "eps", "weight_decay"}
@@ -127,6 +129,67 @@ class FlatAdam(torch.optim.Optimizer):
                     self.step_t[0] = float(s["step"])
                     first = False
         self._point_state()
+
+
+_SCALINGS = {None: 1, "original": 1, "match_rms_adamw": 2, "none": 0}
+
+
+def _as_matrix(shape) -> Tuple[int, int]:
+    rows = int(shape[0])
+    return rows, math.prod(shape[1:])
+
+
+@torch.no_grad()
+def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentum_buffers: Sequence[Tensor], *, lr: float, momentum: float = 0.95,
+              nesterov: bool = True, weight_decay: float = 0.0, adjust_lr_fn: Optional[str] = None, steps: int = 5,
+              coefficients=GF.NS_COEFFICIENTS, eps: float = 1e-7) -> None:
+    """One update of every parameter by its orthogonalised momentum, in place:
+        buf <- momentum * buf + (1 - momentum) * grad
+        u    = momentum * buf + (1 - momentum) * grad if nesterov else buf
+        p   <- (1 - lr * weight_decay) * p - lr * s * orthogonalize(u)
+    A parameter of two or more dimensions counts as the matrix (shape[0], everything else), a convolution as (out, in kh kw).
+    s = sqrt(max(1, rows / cols)) for adjust_lr_fn None or "original", 0.2 sqrt(max(rows, cols)) for "match_rms_adamw", 1 for
+    "none".  float32, contiguous, on one device; nothing may overlap.  All parameters share the launches; a gradient that is
+    not finite makes its own parameter NaN and no other."""
+    if not len(params) == len(grads) == len(momentum_buffers):
+        raise _lib.GanAmdError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momentum_buffers)} momentum buffers")
+    if adjust_lr_fn not in _SCALINGS:
+        raise _lib.GanAmdError(f"muon_step: adjust_lr_fn must be None, 'original', 'match_rms_adamw' or 'none', got {adjust_lr_fn!r}")
+    a, b, c = (float(v) for v in coefficients)
+    held, mats, seen = [], [], set()
+    for p, g, m in zip(params, grads, momentum_buffers):
+        if p.dim() < 2:
+            raise _lib.GanAmdError(f"muon_step: parameters of two or more dimensions, got shape {tuple(p.shape)}")
+        if p.shape != g.shape or p.shape != m.shape:
+            raise _lib.GanAmdError(f"muon_step: parameter {tuple(p.shape)}, gradient {tuple(g.shape)}, momentum {tuple(m.shape)}")
+        if not p.dtype == g.dtype == m.dtype == torch.float32:
+            raise _lib.GanAmdError(f"muon_step takes float32, got {p.dtype}, {g.dtype}, {m.dtype}")
+        if not p.device == g.device == m.device == params[0].device:
+            raise _lib.GanAmdError("muon_step: parameters, gradients and momentum buffers must be on one device")
+        if not (p.is_contiguous() and m.is_contiguous()):
+            raise _lib.GanAmdError("muon_step: parameters and momentum buffers must be contiguous")
+        if p.numel() == 0:
+            continue
+        g = g.contiguous()
+        held.append(g)
+        for t in (p, m):
+            if t.data_ptr() in seen:
+                raise _lib.GanAmdError("muon_step: a parameter or momentum buffer is given twice")
+            seen.add(t.data_ptr())
+        mats.append((g.data_ptr(), m.data_ptr(), p.data_ptr(), *_as_matrix(p.shape), 1))
+    require_gpu(*params[:1])
+    if not mats:
+        return
+    array = (_lib.Matrix * len(mats))(*mats)
+    ws, nbytes = GF.matrix_workspace(array, params[0].device)
+    flops = sum(GF.ortho_flops(t[3], t[4], steps) for t in mats)
+    with _lib.on_device(params[0]):
+        check(GF._run("muon_step", flops, 20 * sum(t[3] * t[4] for t in mats),
+                      lambda: _lib.load().gan_muon_step(ctypes.addressof(array), len(mats), float(lr), float(momentum), int(bool(nesterov)),
+                                                        float(weight_decay), _SCALINGS[adjust_lr_fn], int(steps), a, b, c, float(eps), ptr(ws),
+                                                        nbytes, stream_of(params[0]))), "gan_muon_step")
+    # written through raw pointers: cached GEMM images of the old values would still match their keys
+    GF.invalidate_packed(params)
 
 
 def make_optimizer(name: str, module: nn.Module, lr: float, kwargs: Dict, *, capturable: bool = False) -> torch.optim.Optimizer:

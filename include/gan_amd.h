@@ -439,6 +439,31 @@ int gan_ema_lerp(float* ema, const float* p, int64_t n, float weight, gan_stream
 int gan_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float* step, int advance, float lr, float beta1,
                   float beta2, float eps, float weight_decay, int decoupled, gan_stream_t stream);
 
+/* ---- orthogonalised updates: X = G / max(|G|, eps) (Frobenius norm; m x n, m <= n, a tall G as its transpose), then `steps`
+ * times X <- (a I + b A + c A A) X with A = X X' (Newton-Schulz).  A gan_matrix is `batch` (0: none) dense row-major
+ * (rows, cols) matrices one behind the other; a call takes a list of them, of any sizes.
+ * gan_orthogonalize: out = X of g, both of `dtype`; buf must be NULL.  Products carry 22 bits of every factor and are
+ *                    accumulated in fp32, whatever the dtype.  A matrix of zeros gives zeros, one with a value that is not
+ *                    finite NaN throughout; the others of the call are not touched by it.
+ * gan_muon_step    : fp32; buf = momentum buf + (1 - momentum) g;  u = nesterov ? momentum buf + (1 - momentum) g : buf;
+ *                    out = (1 - lr weight_decay) out - lr s X(u) with s = 1 (scaling 0), sqrt(max(1, rows / cols)) (1) or
+ *                    0.2 sqrt(max(rows, cols)) (2).
+ * No two of g, buf and out may overlap.  Coefficients with which a singular value can grow beyond 3.5 are refused.
+ * 1 <= rows, cols <= 2^20, the smaller at most 32768, 1 <= steps <= 100.
+ * workspace: gan_orthogonalize_workspace bytes, 256-byte aligned; negative: a size that is refused. */
+typedef struct gan_matrix {
+    const void* g;
+    float* buf;
+    void* out;
+    int64_t rows, cols, batch;
+} gan_matrix;
+int64_t gan_orthogonalize_workspace(const gan_matrix* mats, int count);
+int gan_orthogonalize(const gan_matrix* mats, int count, int steps, float a, float b, float c, float eps, int dtype, void* ws, int64_t ws_bytes,
+                      gan_stream_t stream);
+int gan_muon_step(const gan_matrix* mats, int count, float lr, float momentum, int nesterov, float weight_decay, int scaling, int steps, float a,
+                  float b, float c, float eps, void* ws, int64_t ws_bytes, gan_stream_t stream);
+
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,260 @@
+"""functional.orthogonalize, optim.muon_step and optim.FlatMuon against the definition in 64 bits.
+
+Bounds.  Products carry 22 bits of every factor (2^-22 relative to its largest entries) and fp32 sums, so a step adds an error of
+a few 2^-22 of the iterate's norm; what the first steps add is amplified with the smallest singular values, by up to a = 3.4445
+a step (485 in five).  For inputs whose singular values lie within a factor of 30 (Gaussian matrices a little off square, a few
+strong directions over a broad rest) all of them are in the flat part after five steps, and the amplification of the error
+relative to the value stays within that factor: 30 * 5 * 2^-22 = 3.6e-5 in the 2-norm, 1e-4 is asked.  A matrix of another kind
+is held to 485 * 5 * 2^-22 = 6e-4.  bfloat16 results are rounded once, 2^-8 of the value each (2^-9 and less on average)."""
+import math
+
+import pytest
+import torch
+
+from conftest import rel_err
+
+COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    return torch.device("cuda:0")
+
+
+def definition(g, steps=5, coefficients=COEFFS, eps=1e-7):
+    a, b, c = coefficients
+    x = g.detach().double().cpu()
+    x = x / torch.linalg.matrix_norm(x).clamp_min(eps)[..., None, None]
+    tall = x.shape[-2] > x.shape[-1]
+    if tall:
+        x = x.mT
+    for _ in range(steps):
+        gram = x @ x.mT.contiguous()
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.mT if tall else x
+
+
+def make(m, n, dev, seed=0, dt=torch.float32, kind="gauss"):
+    gen = torch.Generator(device="cpu").manual_seed(seed + 31 * m + n)
+    x = torch.randn(m, n, generator=gen)
+    if kind == "strong":
+        x = x + 4 * torch.randn(m, 2, generator=gen) @ torch.randn(2, n, generator=gen)
+    elif kind == "scaled":
+        x = x * torch.logspace(0, -3, m)[:, None]
+    elif kind == "lowrank":
+        k = max(1, min(m, n) // 3)
+        x = torch.randn(m, k, generator=gen) @ torch.randn(k, n, generator=gen)
+    return x.to(dt).to(dev)
+
+
+SIZES = [(1, 1), (1, 7), (9, 1), (2, 3), (16, 144), (144, 16), (63, 65), (64, 64), (65, 200), (200, 129), (128, 128), (130, 1000), (777, 300), (512, 1300), (257, 2304)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", SIZES)
+def test_against_the_definition(dev, m, n):
+    from gan_amd import functional as GF
+
+    for kind, lim in (("gauss", 1e-4), ("strong", 1e-4), ("scaled", 6e-4), ("lowrank", 6e-4)):
+        if kind == "gauss" and m == n and m > 2:
+            lim = 6e-4  # the smallest singular values of a square Gaussian matrix lie far below the others
+        g = make(m, n, dev, kind=kind)
+        got = GF.orthogonalize(g)
+        assert got.shape == g.shape and got.dtype == torch.float32
+        assert rel_err(got, definition(g)) < lim, kind
+        bf = g.bfloat16()
+        got = GF.orthogonalize(bf)
+        assert got.dtype == torch.bfloat16
+        assert rel_err(got, definition(bf)) < lim + 2.0**-8, kind
+
+
+@pytest.mark.gpu
+def test_batches_scales_layouts(dev):
+    from gan_amd import functional as GF
+
+    g = torch.stack([make(48, 100, dev, seed=k) * 10.0 ** (6 * k - 12) for k in range(5)])  # 1e-12 ... 1e12
+    got = GF.orthogonalize(g)
+    want = definition(g)
+    for k in range(5):
+        assert rel_err(got[k], want[k]) < 1e-4, k
+    assert torch.equal(GF.orthogonalize(g[3]), got[3])  # the same bits alone and in a batch
+    assert torch.equal(GF.orthogonalize(g.view(5, 1, 48, 100)), got.view(5, 1, 48, 100))
+    t = make(90, 70, dev)
+    assert torch.equal(GF.orthogonalize(t.t()), GF.orthogonalize(t.t().contiguous()))  # strided
+    off = torch.cat([torch.zeros(1, device=dev), t.flatten()])[1:].view(90, 70)  # not on a 16-byte boundary
+    assert torch.equal(GF.orthogonalize(off), GF.orthogonalize(t))
+    huge = make(20, 30, dev) * 1e25  # squares leave fp32
+    assert rel_err(GF.orthogonalize(huge), definition(huge)) < 1e-4
+    tiny = make(20, 30, dev) * 1e-9  # below eps: divided by eps
+    assert rel_err(GF.orthogonalize(tiny), definition(tiny)) < 1e-4
+    for shape in ((0, 4, 4), (3, 0, 5), (3, 5, 0)):
+        assert GF.orthogonalize(torch.empty(shape, device=dev)).shape == shape
+
+
+@pytest.mark.gpu
+def test_zeros_and_values_that_are_not_finite(dev):
+    from gan_amd import functional as GF
+
+    g = torch.stack([make(70, 90, dev, seed=k) for k in range(6)])
+    want = GF.orthogonalize(g)
+    bad = g.clone()
+    bad[1] = 0
+    bad[2, 5, 7] = float("nan")
+    bad[4, 69, 0] = float("inf")
+    got = GF.orthogonalize(bad)
+    for k in (0, 3, 5):
+        assert torch.equal(got[k], want[k])
+    assert torch.equal(got[1], torch.zeros_like(got[1]))
+    assert torch.isnan(got[2]).all() and torch.isnan(got[4]).all()
+    half = make(40, 60, dev)
+    half[10:20] = 0  # rows of zeros stay zeros
+    assert torch.equal(GF.orthogonalize(half)[10:20], torch.zeros(10, 60, device=dev))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps,coefficients", [(1, COEFFS), (2, COEFFS), (3, COEFFS), (8, COEFFS), (6, (2.0, -1.5, 0.5)), (12, (1.5, -0.5, 0.0)), (1, (1.0, 0.0, 0.0))])
+def test_steps_and_coefficients(dev, steps, coefficients):
+    """(the cubic and quintic iterations that converge to the polar factor too; (1, 0, 0) is the normalisation alone)"""
+    from gan_amd import functional as GF
+
+    for m, n in ((40, 150), (100, 60), (128, 700)):
+        g = make(m, n, dev, kind="strong")
+        want = definition(g, steps, coefficients)
+        lim = 30 * (steps + 1) * 2.0**-22
+        assert rel_err(GF.orthogonalize(g, steps=steps, coefficients=coefficients), want) < lim
+        assert rel_err(GF.orthogonalize(g.bfloat16(), steps=steps, coefficients=coefficients), definition(g.bfloat16(), steps, coefficients)) < lim + 2.0**-8
+    if steps == 12:
+        x = GF.orthogonalize(make(40, 4000, dev), steps=12, coefficients=coefficients)
+        assert rel_err(x @ x.t(), torch.eye(40)) < 1e-4  # converged
+
+
+def step_ref(p, g, buf, lr, momentum, nesterov, wd, scaling, steps=5):
+    p, g, buf = (t.detach().double().cpu() for t in (p, g, buf))
+    m, n = p.shape[0], p[0].numel()
+    buf = momentum * buf + (1 - momentum) * g
+    u = momentum * buf + (1 - momentum) * g if nesterov else buf
+    s = {None: max(1, m / n) ** 0.5, "original": max(1, m / n) ** 0.5, "match_rms_adamw": 0.2 * max(m, n) ** 0.5, "none": 1.0}[scaling]
+    return (1 - lr * wd) * p - lr * s * definition(u.reshape(m, n), steps).reshape(p.shape), buf
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nesterov,wd,scaling", [(True, 0.0, None), (False, 0.1, "original"), (True, 0.01, "match_rms_adamw"), (False, 0.0, "none")])
+def test_muon_step(dev, nesterov, wd, scaling):
+    from gan_amd.optim import muon_step
+
+    shapes = [(16, 3, 1, 1), (64, 48), (48, 64), (1, 5), (200, 10, 3, 3), (8, 8), (0, 4), (300, 1)] + [(12, 5, 3, 3)] * 40  # more than one launch holds
+    gen = torch.Generator(device="cpu").manual_seed(2)
+    p, g, buf = ([torch.randn(s, generator=gen).to(dev) for s in shapes] for _ in range(3))
+    want = [step_ref(*t, 0.02, 0.9, nesterov, wd, scaling) for t in zip(p, g, buf) if t[0].numel()]
+    before = [t.clone() for t in p if t.numel()]
+    muon_step(p, g, buf, lr=0.02, momentum=0.9, nesterov=nesterov, weight_decay=wd, adjust_lr_fn=scaling)
+    for a, b, m, (wp, wb) in zip([t for t in p if t.numel()], before, [t for t in buf if t.numel()], want):
+        assert rel_err(m, wb) < 1e-6
+        # the update alone: orthogonalize's bound, and the parameter's own rounding against it (p ~ 1, the update 0.02 and smaller)
+        upd, upd_w = a.double().cpu() - b.double().cpu(), wp - b.double().cpu()
+        assert float((upd - upd_w).norm()) <= 6e-4 * float(upd_w.norm()) + 2.0**-23 * float(b.norm())
+
+
+@pytest.mark.gpu
+def test_same_bits_other_stream_and_graph(dev):
+    from gan_amd import functional as GF
+    from gan_amd.optim import muon_step
+
+    g = make(150, 700, dev)
+    gb = torch.stack([make(33, 20, dev, seed=k, dt=torch.bfloat16) for k in range(3)])
+    p0, b0 = make(150, 700, dev, seed=3), make(150, 700, dev, seed=4)
+
+    def step():
+        p, b = p0.clone(), b0.clone()
+        muon_step([p], [g], [b], lr=0.1)
+        return [GF.orthogonalize(g), GF.orthogonalize(gb), p, b]
+
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(want, step()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    graphs, held = [], []
+    torch.cuda.synchronize()
+    for _ in range(2):  # two graphs, each with its workspace
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(step())
+    for k in range(3):
+        g.mul_(-1.5), gb.copy_(gb.flip(0))
+        eager = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for h in held:
+            assert all(torch.equal(a, b) for a, b in zip(eager, h)), k
+
+
+def test_refusals():
+    from gan_amd import _lib
+    from gan_amd import functional as GF
+    from gan_amd.optim import muon_step
+
+    x = torch.randn(4, 8)
+    for call in (
+        lambda: GF.orthogonalize(x),  # not on a ROCm device
+        lambda: GF.orthogonalize(x[0]),
+        lambda: GF.orthogonalize(x.half()),
+        lambda: GF.orthogonalize(x.requires_grad_()),
+    ):
+        with pytest.raises(_lib.GanAmdError):
+            call()
+    x = x.detach()
+    for args, kw in (
+        (([x], [x.clone()], [x.clone()]), {}),  # not on a ROCm device
+        (([x], [], [x]), {}),
+        (([x[0]], [x[0]], [x[0]]), {}),
+        (([x], [x.t()], [x]), {}),
+        (([x.double()], [x], [x]), {}),
+        (([x.t()], [x.t()], [x.t()]), {}),
+        (([x, x], [x, x], [x.clone(), x.clone()]), {}),
+        (([x], [x.clone()], [x.clone()]), dict(adjust_lr_fn="other")),
+    ):
+        with pytest.raises(_lib.GanAmdError):
+            muon_step(*args, lr=0.1, **kw)
+    # the C entries refuse before anything is launched
+    import ctypes
+
+    lib = _lib.load()
+    p = 4096  # never read
+
+    def mats(*rows):
+        return (_lib.Matrix * len(rows))(*rows)
+
+    def run(m, steps=5, coeffs=COEFFS, eps=1e-7, dtype=0, ws=p, nbytes=1 << 40):
+        return lib.gan_orthogonalize(ctypes.addressof(m), len(m), steps, *coeffs, eps, dtype, ws, nbytes, None)
+
+    ok = mats((p, None, p, 4, 8, 1))
+    need = lib.gan_orthogonalize_workspace(ctypes.addressof(ok), 1)
+    assert need > 0
+    assert run(ok, steps=0) != 0 and run(ok, steps=101) != 0
+    assert run(ok, eps=0.0) != 0 and run(ok, eps=float("nan")) != 0
+    assert run(ok, coeffs=(10.0, 0.0, 0.0)) != 0 and run(ok, coeffs=(float("nan"), 0.0, 0.0)) != 0
+    assert run(ok, dtype=2) != 0
+    assert run(ok, ws=None) != 0 and run(ok, nbytes=need - 1) != 0 and run(ok, ws=p + 16) != 0
+    assert run(mats((None, None, p, 4, 8, 1))) != 0 and run(mats((p, None, None, 4, 8, 1))) != 0
+    assert run(mats((p, p, p, 4, 8, 1))) != 0  # a momentum buffer without a step
+    for rows, cols, batch in ((0, 8, 1), (4, -1, 1), (4, 8, -1), (1 << 21, 8, 1), (40000, 40000, 1), (4, 8, 1 << 31)):
+        bad = mats((p, None, p, rows, cols, batch))
+        assert lib.gan_orthogonalize_workspace(ctypes.addressof(bad), 1) < 0 and run(bad) != 0
+    assert run(mats((p, None, p, 4, 8, 0))) == 0  # nothing to do
+    assert lib.gan_orthogonalize(None, 1, 5, *COEFFS, 1e-7, 0, p, 1 << 40, None) != 0
+    step = mats((p, p, p, 4, 8, 1))
+
+    def muon(m, lr=0.1, mu=0.9, wd=0.0, scaling=1):
+        return lib.gan_muon_step(ctypes.addressof(m), len(m), lr, mu, 1, wd, scaling, 5, *COEFFS, 1e-7, p, need - 1, None)
+
+    assert muon(step, lr=-1.0) != 0 and muon(step, mu=1.0) != 0 and muon(step, wd=-1.0) != 0 and muon(step, scaling=3) != 0
+    assert muon(ok) != 0  # no momentum buffer
+    assert muon(step) != 0 and b"workspace" in lib.gan_amd_last_error()
