@@ -50,10 +50,18 @@ struct Mats {
     float eps;
 };
 
+// How a product over k is cut when its tiles alone would leave most of the chip idle (A = X X' of a long X): slices of at least
+// 512 k, together with the tiles no more than two 64 x 64 workgroups a CU.  By the matrix's own shape, so that its bits do
+// not depend on what else is in the call.
+__host__ __device__ inline int splits_of(int64_t mp, int64_t np) {
+    const int64_t t = mp / 64, tiles = t * (t + 1) / 2, most = np / 512, s = 512 / tiles;
+    return (int)(s < most ? (s > 1 ? s : 1) : (most > 1 ? most : 1));
+}
+
 // Byte offsets in one matrix's workspace: the scale, the partial sums, two X (each [m][n] and [n][m], hi plane then lo
-// plane), A, P.
+// plane), A, P, the slices' tiles of a product that is cut.
 struct Lay {
-    int64_t mp, np, scale, part, nparts, xm[2], xt[2], a, p, bytes;
+    int64_t mp, np, scale, part, nparts, xm[2], xt[2], a, p, join, bytes;
 };
 
 __host__ __device__ inline Lay lay_of(int64_t rows, int64_t cols) {
@@ -76,6 +84,10 @@ __host__ __device__ inline Lay lay_of(int64_t rows, int64_t cols) {
     at += sq;
     l.p = at;
     at += sq;
+    l.join = at;
+    const int cut = splits_of(l.mp, l.np);
+    const int64_t t = (l.mp + 255) / 256 * 4;  // in whole tiles of the largest size
+    if (cut > 1) at += cut * t * (t + 4) / 2 * 4096 * 4;
     l.bytes = at;
     return l;
 }
@@ -198,6 +210,7 @@ struct Op {
     int rows, cols;  // of the source
     int first, tiles;  // first workgroup, workgroups per matrix
     int kind, cur;     // cur: which X holds the iterate
+    int cut, steps;    // slices of k, steps of 32 k in each but the last
 };
 
 struct Ops {
@@ -213,6 +226,78 @@ __device__ __forceinline__ float step_of(const Ops& s, int rows, int cols) {
     return s.update == 2 ? s.step * sqrtf(fmaxf(1.f, r / c)) : s.update == 3 ? s.step * 0.2f * sqrtf(fmaxf(r, c)) : s.step;
 }
 
+// Tile t of the tiles on and above the diagonal of n x n, row by row
+__device__ __forceinline__ int2 tile_of(int t, int n) {
+    int ti = 0;
+    for (int left = n; t >= left; --left, ++ti) t -= left;
+    return make_int2(ti, ti + t);
+}
+
+// Rows i ... i + 3 of column j of a product, as accumulated.  mirror: the transposed place is another tile's.
+__device__ __forceinline__ void finish(const Ops& s, const Op& q, const Lay& l, char* ws, int b, int i, int j, float (&o)[4], bool mirror, int dtype) {
+    const int mp = (int)l.mp, np = (int)l.np;
+    const int64_t sq = (int64_t)mp * mp;
+    if (q.kind == RESULT) {
+        const bool wide = q.rows <= q.cols;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int row = wide ? i + e : j, col = wide ? j : i + e;
+            if (row >= q.rows || col >= q.cols) continue;
+            const int64_t at = ((int64_t)b * q.rows + row) * q.cols + col;
+            const float val = o[e] * (1.f / (SP * SX));
+            if (s.update == 0) {
+                if (dtype == GAN_F32) ((float*)q.out)[at] = val;
+                else ((bf16*)q.out)[at] = (bf16)val;
+            } else {
+                float* p = (float*)q.out + at;
+                *p = fmaf(-step_of(s, q.rows, q.cols), val, s.decay * *p);
+            }
+        }
+        return;
+    }
+    h16 *dn, *dt;  // [i][j] and [j][i]
+    int64_t plane;
+    int ldn = mp;
+    if (q.kind == APPLY) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= 1.f / SP;
+        dn = (h16*)(ws + (q.cur ? l.xm[0] : l.xm[1]));
+        dt = (h16*)(ws + (q.cur ? l.xt[0] : l.xt[1]));
+        plane = (int64_t)mp * np;
+        ldn = np;
+        mirror = true;
+    } else {
+        if (q.kind == GRAM) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] *= SA / (SX * SX);
+        } else {
+            const h16* A = (const h16*)(ws + l.a) + (int64_t)j * mp + i;
+            const h16x4 ah = *(const h16x4*)A, al = *(const h16x4*)(A + sq);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float av = ((float)ah[e] + (float)al[e]) * (SP / SA);
+                o[e] = fmaf(s.c * (SP / (SA * SA)), o[e], s.b * av) + (i + e == j ? s.a * SP : 0.f);
+            }
+        }
+        dn = dt = (h16*)(ws + (q.kind == GRAM ? l.a : l.p));
+        plane = sq;
+    }
+    h16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        h16 p, w;
+        split(o[e], p, w);
+        hi[e] = p;
+        lo[e] = w;
+        dn[(int64_t)(i + e) * ldn + j] = p;
+        dn[plane + (int64_t)(i + e) * ldn + j] = w;
+    }
+    if (mirror) {
+        *(h16x4*)(dt + (int64_t)j * mp + i) = hi;
+        *(h16x4*)(dt + plane + (int64_t)j * mp + i) = lo;
+    }
+}
+
 // an address that is the same in every lane, in scalar registers
 __device__ __forceinline__ const char* scalar(const char* p) {
     const uint64_t v = (uint64_t)p;
@@ -223,32 +308,40 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const char* p) {
     return __builtin_amdgcn_make_buffer_rsrc((void*)scalar(p), 0, 0xffffffffu, 0x00020000);
 }
 
-// LDS-DMA of stage `step` into `base`: a wave's instruction j covers 1 KB = 16 rows of plane j / (T / 64)
-template <int T, int PER>
+// LDS-DMA of k step `step` into `base`: a wave's instruction j covers 1 KB = 16 rows of plane j / PP
+template <int WAVES, int PP, int PER>
 __device__ __forceinline__ void ortho_issue(char* base, int step, int wave, __amdgpu_buffer_rsrc_t ru, __amdgpu_buffer_rsrc_t rul,
                                             __amdgpu_buffer_rsrc_t rv, __amdgpu_buffer_rsrc_t rvl, const unsigned (&off)[PER]) {
-    constexpr int PP = T / 64;
 #pragma unroll
     for (int j = 0; j < PER; ++j)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(j / PP == 0 ? ru : j / PP == 1 ? rul : j / PP == 2 ? rv : rvl,
-                                                 (__attribute__((address_space(3))) void*)(base + (4 * j + wave) * 1024), 16, off[j], step * 64, 0,
-                                                 0);
+                                                 (__attribute__((address_space(3))) void*)(base + (WAVES * j + wave) * 1024), 16, off[j], step * 64,
+                                                 0, 0);
 }
 
-// Tile T x T of C = U V', four waves of T/2 x T/2.  U [M][K], V [N][K], each a hi plane and a lo plane; K % 32 == 0.  Stages of
-// 32 k (64 bytes a row) go to LDS by DMA, chunk c of row r at position c ^ ((r >> 2) & 3): the 16 rows that a fragment read
-// touches at a time then lie in different banks.
+template <int T>
+constexpr int gemm_threads() {
+    return T == 256 ? 512 : 256;
+}
+
+// Tile T x T of C = U V': four waves of T/2 x T/2, or eight of 128 x 64.  U [M][K], V [N][K], each a hi plane and a lo plane;
+// K % 32 == 0.  Stages of 32 k (64 bytes a row) go to LDS by DMA, chunk c of row r at position c ^ ((r >> 2) & 3): the 16 rows
+// that a fragment read touches at a time then lie in different banks.
 template <int T, int NST>
-__global__ void __launch_bounds__(256, T == 128 ? 2 : 4) ortho_gemm_k(const Ops s, int dtype) {
-    constexpr int F = T / 64;                     // 32 x 32 fragments of a wave, each way
-    constexpr int PLANE = T * 64, STAGE = 4 * PLANE;  // bytes: U hi, U lo, V hi, V lo
-    constexpr int PER = STAGE / 4096;             // DMA instructions per wave and stage
+__global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm_k(const Ops s, int dtype) {
+    constexpr int WAVES = gemm_threads<T>() / 64, WN = WAVES / 2;  // waves: 2 x WN
+    constexpr int FM = T / 64, FN = T / 32 / WN;                   // 32 x 32 fragments of a wave
+    constexpr int PLANE = T * 64, STAGE = 4 * PLANE;               // bytes: U hi, U lo, V hi, V lo
+    constexpr int PER = STAGE / 1024 / WAVES;                      // DMA instructions per wave and stage
+    constexpr int PP = PER / 4;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const Op& q = s.mat[group_of(s, blockIdx.x)];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
     // (divisions run on vector registers: say that the results are the wave's, or every use of an address loops over lanes)
-    const int b = __builtin_amdgcn_readfirstlane((int)(blockIdx.x - q.first) / q.tiles);
-    int t = (int)(blockIdx.x - q.first) - b * q.tiles;
+    const int per = q.tiles * q.cut;
+    const int b = __builtin_amdgcn_readfirstlane(((int)blockIdx.x - q.first) / per);
+    const int in_b = (int)blockIdx.x - q.first - b * per;
+    const int slice = __builtin_amdgcn_readfirstlane(in_b / q.tiles), tile = in_b - slice * q.tiles;
     const Lay l = lay_of(q.rows, q.cols);
     char* ws = q.ws + b * q.stride;
     const int mp = (int)l.mp, np = (int)l.np;
@@ -270,18 +363,14 @@ __global__ void __launch_bounds__(256, T == 128 ? 2 : 4) ortho_gemm_k(const Ops 
         N = np;
     }
     int ti, tj;
-    if (sym) {  // tiles on and above the diagonal, row by row
-        int left = (M + T - 1) / T;
-        ti = 0;
-        while (t >= left) {
-            t -= left--;
-            ++ti;
-        }
-        tj = ti + t;
+    if (sym) {
+        const int2 t = tile_of(tile, (M + T - 1) / T);
+        ti = t.x;
+        tj = t.y;
     } else {
         const int tm = (M + T - 1) / T;
-        tj = __builtin_amdgcn_readfirstlane(t / tm);
-        ti = t - tj * tm;
+        tj = __builtin_amdgcn_readfirstlane(tile / tm);
+        ti = tile - tj * tm;
     }
     const int i0 = ti * T, j0 = tj * T;
     // ---- staging: a wave's instruction j covers 1 KB of the stage = 16 rows of one plane
@@ -294,22 +383,22 @@ __global__ void __launch_bounds__(256, T == 128 ? 2 : 4) ortho_gemm_k(const Ops 
     const __amdgpu_buffer_rsrc_t rvl = rows_from(v + ((int64_t)N + j0) * kb);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const int piece = 4 * j + wave, pl = piece / (T / 16), row = piece % (T / 16) * 16 + rsub;
+        const int piece = WAVES * j + wave, pl = piece / (T / 16), row = piece % (T / 16) * 16 + rsub;
         // rows past the matrix (T = 128 over an odd number of 64s): the last row again, their results are not stored
         const int lim = pl < 2 ? M - i0 : N - j0;
         off[j] = (unsigned)(row < lim ? row : lim - 1) * kb + (unsigned)((pos ^ ((row >> 2) & 3)) * 16);
     }
-    f32x16 acc[F][F];
+    f32x16 acc[FM][FN];
 #pragma unroll
-    for (int x = 0; x < F; ++x)
+    for (int x = 0; x < FM; ++x)
 #pragma unroll
-        for (int y = 0; y < F; ++y)
+        for (int y = 0; y < FN; ++y)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
-    const int nk = K / 32;
+    const int k0 = slice * q.steps, nk = (K / 32 - k0 < q.steps ? K / 32 - k0 : q.steps);
 #pragma unroll
     for (int k = 0; k < NST - 1; ++k)
-        if (k < nk) ortho_issue<T, PER>(lds + k * STAGE, k, wave, ru, rul, rv, rvl, off);
+        if (k < nk) ortho_issue<WAVES, PP, PER>(lds + k * STAGE, k0 + k, wave, ru, rul, rv, rvl, off);
     for (int k = 0; k < nk; ++k) {
         // this wave's share of stage k has arrived and its reads of the stage before are done ...
         if (k + NST - 1 < nk + 1)
@@ -320,118 +409,121 @@ __global__ void __launch_bounds__(256, T == 128 ? 2 : 4) ortho_gemm_k(const Ops 
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         if (k + NST - 1 < nk)
-            ortho_issue<T, PER>(lds + (k + NST - 1) % NST * STAGE, k + NST - 1, wave, ru, rul, rv, rvl, off);
+            ortho_issue<WAVES, PP, PER>(lds + (k + NST - 1) % NST * STAGE, k0 + k + NST - 1, wave, ru, rul, rv, rvl, off);
         const char* base = lds + k % NST * STAGE;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            h16x8 uh[F], ul[F], vh[F], vl[F];
+            h16x8 uh[FM], ul[FM], vh[FN], vl[FN];
             const int ch = h * 2 + (lane >> 5);
 #pragma unroll
-            for (int x = 0; x < F; ++x) {
-                const int ra = wm * (T / 2) + x * 32 + (lane & 31), rb = wn * (T / 2) + x * 32 + (lane & 31);
-                const int pa = ra * 64 + ((ch ^ ((ra >> 2) & 3)) << 4), pb = rb * 64 + ((ch ^ ((rb >> 2) & 3)) << 4);
-                uh[x] = *(const h16x8*)(base + pa);
-                ul[x] = *(const h16x8*)(base + PLANE + pa);
-                vh[x] = *(const h16x8*)(base + 2 * PLANE + pb);
-                vl[x] = *(const h16x8*)(base + 3 * PLANE + pb);
+            for (int x = 0; x < FM; ++x) {
+                const int row = wm * (T / 2) + x * 32 + (lane & 31), at = row * 64 + ((ch ^ ((row >> 2) & 3)) << 4);
+                uh[x] = *(const h16x8*)(base + at);
+                ul[x] = *(const h16x8*)(base + PLANE + at);
             }
 #pragma unroll
-            for (int x = 0; x < F; ++x)
+            for (int y = 0; y < FN; ++y) {
+                const int row = wn * (T / WN) + y * 32 + (lane & 31), at = row * 64 + ((ch ^ ((row >> 2) & 3)) << 4);
+                vh[y] = *(const h16x8*)(base + 2 * PLANE + at);
+                vl[y] = *(const h16x8*)(base + 3 * PLANE + at);
+            }
 #pragma unroll
-                for (int y = 0; y < F; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh[x], vl[y], acc[x][y], 0, 0, 0);
+            for (int x = 0; x < FM; ++x)
 #pragma unroll
-            for (int x = 0; x < F; ++x)
+                for (int y = 0; y < FN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh[x], vl[y], acc[x][y], 0, 0, 0);
 #pragma unroll
-                for (int y = 0; y < F; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul[x], vh[y], acc[x][y], 0, 0, 0);
+            for (int x = 0; x < FM; ++x)
 #pragma unroll
-            for (int x = 0; x < F; ++x)
+                for (int y = 0; y < FN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul[x], vh[y], acc[x][y], 0, 0, 0);
 #pragma unroll
-                for (int y = 0; y < F; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh[x], vh[y], acc[x][y], 0, 0, 0);
+            for (int x = 0; x < FM; ++x)
+#pragma unroll
+                for (int y = 0; y < FN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh[x], vh[y], acc[x][y], 0, 0, 0);
         }
     }
-    // ---- results: lane holds column lane & 31, rows 8 (r / 4) + 4 (lane >> 5) + r % 4 of each 32 x 32 block
-    const int64_t sq = (int64_t)mp * mp, xp = (int64_t)mp * np;
+    if (q.cut > 1) {  // this slice's sums, in the order that join_k reads them
+        float4* out = (float4*)(ws + l.join) + ((int64_t)slice * q.tiles + tile) * (T * T / 4) + wave * (T * T / 4 / WAVES) + lane;
 #pragma unroll
-    for (int x = 0; x < F; ++x) {
+        for (int x = 0; x < FM; ++x)
 #pragma unroll
-        for (int y = 0; y < F; ++y) {
-            const int ib = i0 + wm * (T / 2) + x * 32, j = j0 + wn * (T / 2) + y * 32 + (lane & 31);
-            if (ib >= M || j >= N) continue;  // (both go by whole blocks of 32)
+            for (int y = 0; y < FN; ++y)
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const int i = ib + 8 * r4 + 4 * (lane >> 5);
-                float o[4];
+                for (int r = 0; r < 4; ++r)
+                    out[((x * FN + y) * 4 + r) * 64] = make_float4(acc[x][y][r * 4], acc[x][y][r * 4 + 1], acc[x][y][r * 4 + 2], acc[x][y][r * 4 + 3]);
+        return;
+    }
+    // lane holds column lane & 31, rows 8 r + 4 (lane >> 5) ... + 3 of each 32 x 32 block
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = acc[x][y][r4 * 4 + e];
-                if (q.kind == RESULT) {
-                    const bool wide = q.rows <= q.cols;
-                    const float inv = 1.f / (SP * SX);
+    for (int x = 0; x < FM; ++x) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = wide ? i + e : j, col = wide ? j : i + e;
-                        if (row >= q.rows || col >= q.cols) continue;
-                        const int64_t at = ((int64_t)b * q.rows + row) * q.cols + col;
-                        const float val = o[e] * inv;
-                        if (s.update == 0) {
-                            if (dtype == GAN_F32) ((float*)q.out)[at] = val;
-                            else ((bf16*)q.out)[at] = (bf16)val;
-                        } else {
-                            float* p = (float*)q.out + at;
-                            *p = fmaf(-step_of(s, q.rows, q.cols), val, s.decay * *p);
-                        }
-                    }
-                    continue;
-                }
-                h16 *dn, *dt;        // [i][j] and [j][i]
-                int64_t plane, ldn, ldt;
-                if (q.kind == APPLY) {
+        for (int y = 0; y < FN; ++y) {
+            const int i = i0 + wm * (T / 2) + x * 32 + 4 * (lane >> 5), j = j0 + wn * (T / WN) + y * 32 + (lane & 31);
+            if (i >= M || j >= N) continue;  // (whole blocks of 32 either way)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] *= 1.f / SP;
-                    dn = (h16*)(ws + (q.cur ? l.xm[0] : l.xm[1]));
-                    dt = (h16*)(ws + (q.cur ? l.xt[0] : l.xt[1]));
-                    plane = xp;
-                    ldn = np;
-                    ldt = mp;
-                } else {
-                    if (q.kind == GRAM) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] *= SA / (SX * SX);
-                    } else {
-                        const h16* A = (const h16*)(ws + l.a);
-                        const h16x4 ah = *(const h16x4*)(A + (int64_t)j * mp + i), al = *(const h16x4*)(A + sq + (int64_t)j * mp + i);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float av = ((float)ah[e] + (float)al[e]) * (SP / SA);
-                            o[e] = fmaf(s.c * (SP / (SA * SA)), o[e], s.b * av) + (i + e == j ? s.a * SP : 0.f);
-                        }
-                    }
-                    dn = dt = (h16*)(ws + (q.kind == GRAM ? l.a : l.p));
-                    plane = sq;
-                    ldn = ldt = mp;
-                }
-                h16x4 hi, lo;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    h16 p, w;
-                    split(o[e], p, w);
-                    hi[e] = p;
-                    lo[e] = w;
-                    dn[(int64_t)(i + e) * ldn + j] = p;
-                    dn[plane + (int64_t)(i + e) * ldn + j] = w;
-                }
-                if (!sym || ti != tj) {
-                    *(h16x4*)(dt + (int64_t)j * ldt + i) = hi;
-                    *(h16x4*)(dt + plane + (int64_t)j * ldt + i) = lo;
-                }
+            for (int r = 0; r < 4; ++r) {
+                float o[4] = {acc[x][y][r * 4], acc[x][y][r * 4 + 1], acc[x][y][r * 4 + 2], acc[x][y][r * 4 + 3]};
+                finish(s, q, l, ws, b, i + 8 * r, j, o, sym && ti != tj, dtype);
             }
         }
     }
 }
 
-// One product of every matrix, one launch.
+// The slices of a product that was cut, added in their order; one float4 (four rows of a column) a thread
+template <int T>
+__global__ void __launch_bounds__(256) ortho_join_k(const Ops s, int dtype) {
+    constexpr int WAVES = T == 256 ? 8 : 4, WN = WAVES / 2, FN = T / 32 / WN, PERT = T * T / 1024;  // workgroups of this kernel per tile
+    const Op& q = s.mat[group_of(s, blockIdx.x)];
+    const int local = (int)blockIdx.x - q.first, tile_b = local / PERT, b = tile_b / q.tiles, tile = tile_b - b * q.tiles;
+    const Lay l = lay_of(q.rows, q.cols);
+    char* ws = q.ws + b * q.stride;
+    const int at = local % PERT * 256 + threadIdx.x;
+    const float4* in = (const float4*)(ws + l.join) + (int64_t)tile * (T * T / 4) + at;
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < q.cut; ++c) {
+        const float4 v = in[(int64_t)c * q.tiles * (T * T / 4)];
+        o[0] += v.x;
+        o[1] += v.y;
+        o[2] += v.z;
+        o[3] += v.w;
+    }
+    const int lane = at & 63, r = at >> 6 & 3, frag = (at >> 8) % (T * T / WAVES / 1024), wave = at / (T * T / 4 / WAVES);
+    const int2 t = tile_of(tile, (int)(l.mp + T - 1) / T);
+    const int i = t.x * T + (wave / WN) * (T / 2) + frag / FN * 32 + 8 * r + 4 * (lane >> 5);
+    const int j = t.y * T + (wave % WN) * (T / WN) + frag % FN * 32 + (lane & 31);
+    if (i < l.mp && j < l.mp) finish(s, q, l, ws, b, i, j, o, t.x != t.y, dtype);
+}
+
+template <int T, int NST>
+int launch_gemm(unsigned blocks, const Ops& s, int dtype, hipStream_t st) {
+    constexpr int lds = NST * 4 * T * 64;
+    // more than 64 KB of dynamic LDS needs the attribute (set on every call: it is per device, and cheap)
+    if (lds > 64 * 1024 && hipFuncSetAttribute((const void*)ortho_gemm_k<T, NST>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+        gan_set_error("orthogonalize: cannot reserve %d bytes of LDS", lds);
+        return GAN_ERR_LAUNCH;
+    }
+    hipLaunchKernelGGL((ortho_gemm_k<T, NST>), dim3(blocks), dim3(gemm_threads<T>()), lds, st, s, dtype);
+    GAN_CHECK_LAUNCH("orthogonalize(product)");
+    return GAN_OK;
+}
+
+int64_t tiles_of(const Lay& l, int kind, int T) {
+    const int64_t tm = (l.mp + T - 1) / T, tn = (l.np + T - 1) / T;
+    return kind <= POLY ? tm * (tm + 1) / 2 : tm * tn;
+}
+
+// One product of every matrix: one launch, and one more that joins slices where there are any.
 int products(const gan_matrix* mats, int n, int kind, int cur, Ops& s, char* ws, int dtype, hipStream_t st) {
-    constexpr int T = 64, NST = 2;
-    int64_t blocks = 0;
+    // The largest tile with which there is a workgroup for every CU: the larger, the fewer bytes go through LDS for a product.
+    int T = 256;
+    for (; T > 64; T >>= 1) {
+        int64_t all = 0;
+        for (int k = 0; k < n; ++k) {
+            const Lay l = lay_of(mats[k].rows, mats[k].cols);
+            all += tiles_of(l, kind, T) * (kind == GRAM ? splits_of(l.mp, l.np) : 1) * mats[k].batch;
+        }
+        if (all >= 256) break;
+    }
+    int64_t blocks = 0, join = 0;
     s.count = n;
     for (int k = 0; k < n; ++k) {
         const gan_matrix& g = mats[k];
@@ -444,14 +536,32 @@ int products(const gan_matrix* mats, int n, int kind, int cur, Ops& s, char* ws,
         q.cols = (int)g.cols;
         q.kind = kind;
         q.cur = cur;
-        const int64_t tm = (l.mp + T - 1) / T, tn = (l.np + T - 1) / T;
-        q.tiles = (int)(kind <= POLY ? tm * (tm + 1) / 2 : tm * tn);
+        q.tiles = (int)tiles_of(l, kind, T);
+        const int steps = (int)((kind == GRAM ? l.np : l.mp) / 32), cut = kind == GRAM ? splits_of(l.mp, l.np) : 1;
+        q.steps = (steps + cut - 1) / cut;
+        q.cut = (steps + q.steps - 1) / q.steps;
         q.first = (int)blocks;
-        blocks += (int64_t)q.tiles * g.batch;
+        blocks += (int64_t)q.tiles * q.cut * g.batch;
         ws += l.bytes * g.batch;
     }
-    hipLaunchKernelGGL((ortho_gemm_k<T, NST>), dim3((unsigned)blocks), dim3(256), NST * 4 * T * 64, st, s, dtype);
-    GAN_CHECK_LAUNCH("orthogonalize(product)");
+    if (int rc = T == 256   ? launch_gemm<256, 2>((unsigned)blocks, s, dtype, st)
+                 : T == 128 ? launch_gemm<128, 2>((unsigned)blocks, s, dtype, st)
+                            : launch_gemm<64, 4>((unsigned)blocks, s, dtype, st))
+        return rc;
+    // the matrices whose products were cut
+    int m = 0;
+    for (int k = 0; k < n; ++k) {
+        if (s.mat[k].cut == 1) continue;
+        s.mat[m] = s.mat[k];
+        s.mat[m++].first = (int)join;
+        join += (int64_t)s.mat[m - 1].tiles * mats[k].batch * (T * T / 1024);
+    }
+    if (!m) return GAN_OK;
+    s.count = m;
+    if (T == 256) hipLaunchKernelGGL((ortho_join_k<256>), dim3((unsigned)join), dim3(256), 0, st, s, dtype);
+    else if (T == 128) hipLaunchKernelGGL((ortho_join_k<128>), dim3((unsigned)join), dim3(256), 0, st, s, dtype);
+    else hipLaunchKernelGGL((ortho_join_k<64>), dim3((unsigned)join), dim3(256), 0, st, s, dtype);
+    GAN_CHECK_LAUNCH("orthogonalize(join)");
     return GAN_OK;
 }
 
@@ -544,7 +654,7 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, Mats&
         const gan_matrix& g = all[k];
         GAN_CHECK_ARG(!g.batch || (g.g && g.out && (!o.update || g.buf)), "%s: null pointer", what);
         const Lay l = lay_of(g.rows, g.cols);
-        const int64_t tiles = l.mp / 64 * (l.np / 64);
+        const int64_t tiles = l.mp / 64 * (l.np / 64) + 4096;  // (slices stay below that)
         GAN_CHECK_ARG(g.batch <= MAXGRID / NOPS / (tiles > l.nparts ? tiles : l.nparts), "%s: %lld matrices of %lld x %lld are too many for one call",
                       what, (long long)g.batch, (long long)g.rows, (long long)g.cols);
     }
