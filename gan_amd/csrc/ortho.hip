@@ -17,7 +17,7 @@ typedef __attribute__((ext_vector_type(4))) _Float16 h16x4;
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 
 constexpr int PAD = 64;          // matrices are padded with zeros to multiples of this
-constexpr int CHUNK = 4096;      // elements of one partial sum of squares
+constexpr int MAXPARTS = 512;    // partial sums of squares of a matrix
 constexpr int NOPS = 32;         // matrices of one launch (their descriptions are kernel arguments: at most 4 KB)
 constexpr int64_t MAXGRID = 1LL << 31;
 constexpr float SX = 16384.f;    // |X| <= 3.9: fp16 ends at 65504
@@ -30,6 +30,13 @@ __device__ __forceinline__ void split(float v, h16& hi, h16& lo) {
     hi = (h16)v;
     lo = (h16)(v - (float)hi);
 }
+
+// elements of one partial sum of squares
+__host__ __device__ inline int64_t chunk_of(int64_t size) {
+    const int64_t c = (size + MAXPARTS - 1) / MAXPARTS;
+    return c < 4096 ? 4096 : (c + 1023) / 1024 * 1024;
+}
+__host__ __device__ inline int64_t parts_of(int64_t size) { return (size + chunk_of(size) - 1) / chunk_of(size); }
 
 // One group of equal matrices, `stride` bytes apart in the workspace.
 struct Mat {
@@ -58,19 +65,18 @@ __host__ __device__ inline int splits_of(int64_t mp, int64_t np) {
     return (int)(s < most ? (s > 1 ? s : 1) : (most > 1 ? most : 1));
 }
 
-// Byte offsets in one matrix's workspace: the scale, the partial sums, two X (each [m][n] and [n][m], hi plane then lo
+// Byte offsets in one matrix's workspace: the partial sums, two X (each [m][n] and [n][m], hi plane then lo
 // plane), A, P, the slices' tiles of a product that is cut.
 struct Lay {
-    int64_t mp, np, scale, part, nparts, xm[2], xt[2], a, p, join, bytes;
+    int64_t mp, np, part, nparts, xm[2], xt[2], a, p, join, bytes;
 };
 
 __host__ __device__ inline Lay lay_of(int64_t rows, int64_t cols) {
     Lay l;
     l.mp = up64(rows < cols ? rows : cols);
     l.np = up64(rows < cols ? cols : rows);
-    l.nparts = (rows * cols + CHUNK - 1) / CHUNK;
-    int64_t at = 256;
-    l.scale = 0;
+    l.nparts = parts_of(rows * cols);
+    int64_t at = 0;
     l.part = at;
     at += (l.nparts * 8 + 255) / 256 * 256;
     const int64_t x = l.mp * l.np * 4, sq = l.mp * l.mp * 4;
@@ -104,54 +110,70 @@ __device__ __forceinline__ int group_of(const S& s, int id) {
     return lo;
 }
 
-template <typename T>
-__device__ __forceinline__ float source(const Mats& s, const T* g, const float* buf, int64_t i) {
-    const float v = (float)g[i];
-    if (!buf) return v;
-    const float m = buf[i];
-    return s.nesterov ? fmaf(s.mu, m, (1.f - s.mu) * v) : m;
-}
+// what is orthogonalised, of gradient g and momentum m
+__device__ __forceinline__ float update_of(const Mats& s, float g, float m) { return s.nesterov ? fmaf(s.mu, m, (1.f - s.mu) * g) : m; }
 
 // ---- momentum and the partial sums of squares (doubles: no square of a finite fp32 leaves their range) ------------------
 template <typename T>
 __global__ void __launch_bounds__(256) ortho_norm_k(const Mats s) {
     __shared__ double red[4];
     const Mat& q = s.mat[group_of(s, blockIdx.x)];
-    const int64_t size = (int64_t)q.rows * q.cols, nparts = (size + CHUNK - 1) / CHUNK;
-    const int64_t local = blockIdx.x - q.first, b = local / nparts, c = local % nparts;
-    const T* g = (const T*)q.g + b * size;
-    float* buf = q.buf ? q.buf + b * size : nullptr;
-    const int64_t end = (c + 1) * CHUNK < size ? (c + 1) * CHUNK : size;
+    const int64_t size = (int64_t)q.rows * q.cols, chunk = chunk_of(size), nparts = parts_of(size);
+    const int local = (int)blockIdx.x - q.first, b = local / (int)nparts, c = local - b * (int)nparts;
+    const T* __restrict__ g = (const T*)q.g + b * size;
+    float* __restrict__ buf = q.buf ? q.buf + b * size : nullptr;
+    const int64_t end = (c + 1) * chunk < size ? (c + 1) * chunk : size;
     double sum = 0.;
-    for (int64_t i = c * CHUNK + threadIdx.x; i < end; i += 256) {
-        if (buf) buf[i] = fmaf(s.mu, buf[i], (1.f - s.mu) * (float)g[i]);
-        const float u = source(s, g, buf, i);
-        sum += (double)u * (double)u;
+    for (int64_t i0 = c * chunk; i0 < end; i0 += 1024) {  // four elements a thread and round, all requested at once
+        const int64_t i = i0 + threadIdx.x * 4;
+        float v[4], m[4];
+        if (i + 4 <= end) {
+            T t[4];
+            __builtin_memcpy(t, g + i, sizeof(t));
+            if (buf) __builtin_memcpy(m, buf + i, sizeof(m));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = i + e < end ? (float)g[i + e] : 0.f;
+                m[e] = buf && i + e < end ? buf[i + e] : 0.f;
+            }
+        }
+        if (buf) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                m[e] = fmaf(s.mu, m[e], (1.f - s.mu) * v[e]);
+                v[e] = update_of(s, v[e], m[e]);
+            }
+            if (i + 4 <= end) {
+                __builtin_memcpy(buf + i, m, sizeof(m));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + e < end) buf[i + e] = m[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += (double)v[e] * (double)v[e];
     }
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        char* ws = q.ws + b * q.stride;
-        ((double*)(ws + 256))[c] = red[0] + red[1] + red[2] + red[3];
-    }
+    if (threadIdx.x == 0) ((double*)(q.ws + b * q.stride))[c] = red[0] + red[1] + red[2] + red[3];
 }
 
-// SX / max(|u|, eps) of each matrix, the partial sums in their order; not finite: NaN, so that the whole matrix says so
-__global__ void __launch_bounds__(256) ortho_scale_k(const Mats s) {
+// SX / max(|u|, eps) of a matrix, every workgroup for itself and all the same: the partial sums in their order.  Not finite:
+// NaN, so that the whole matrix says so.
+__device__ __forceinline__ float scale_of(const double* part, int nparts, float eps) {
     __shared__ double red[4];
-    const Mat& q = s.mat[group_of(s, blockIdx.x)];
-    const int64_t size = (int64_t)q.rows * q.cols, nparts = (size + CHUNK - 1) / CHUNK;
-    char* ws = q.ws + (int64_t)(blockIdx.x - q.first) * q.stride;
     double sum = 0.;
-    for (int64_t i = threadIdx.x; i < nparts; i += 256) sum += ((const double*)(ws + 256))[i];
+    for (int i = threadIdx.x; i < nparts; i += 256) sum += part[i];
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        const double n = sqrt(red[0] + red[1] + red[2] + red[3]);
-        *(float*)ws = n < 1e300 ? (float)((double)SX / (n > (double)s.eps ? n : (double)s.eps)) : __builtin_nanf("");
-    }
+    const double n = sqrt(red[0] + red[1] + red[2] + red[3]);
+    return n < 1e300 ? (float)((double)SX / (n > (double)eps ? n : (double)eps)) : __builtin_nanf("");
 }
 
 // ---- the scaled source as two planes, [rows][cols] and [cols][rows], padded with zeros ---------------------------------
@@ -167,11 +189,22 @@ __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
     const T* g = (const T*)q.g + b * size;
     const float* buf = q.buf ? q.buf + b * size : nullptr;
     char* ws = q.ws + b * q.stride;
-    const float scale = *(const float*)ws;
-    for (int k = threadIdx.x; k < 64 * 64; k += 256) {
-        const int r = k >> 6, c = k & 63;
+    float v[16], m[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const int r = r0 + k * 4 + (threadIdx.x >> 6), c = c0 + (threadIdx.x & 63);
+        const bool in = r < q.rows && c < q.cols;
+        const int64_t at = in ? (int64_t)r * q.cols + c : 0;  // always loaded, cleared afterwards
+        v[k] = (float)g[at];
+        if (buf) m[k] = buf[at];
+        if (!in) v[k] = m[k] = 0.f;
+    }
+    const float scale = scale_of((const double*)ws, (int)parts_of(size), s.eps);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const int r = k * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
         const bool in = r0 + r < q.rows && c0 + c < q.cols;
-        tile[r][c] = in ? scale * source(s, g, buf, (int64_t)(r0 + r) * q.cols + c0 + c) : 0.f;
+        tile[r][c] = in ? scale * (buf ? update_of(s, v[k], m[k]) : v[k]) : 0.f;
     }
     __syncthreads();
     const Lay l = lay_of(q.rows, q.cols);
@@ -233,24 +266,69 @@ __device__ __forceinline__ int2 tile_of(int t, int n) {
     return make_int2(ti, ti + t);
 }
 
-// Rows i ... i + 3 of column j of a product, as accumulated.  mirror: the transposed place is another tile's.
-__device__ __forceinline__ void finish(const Ops& s, const Op& q, const Lay& l, char* ws, int b, int i, int j, float (&o)[4], bool mirror, int dtype) {
+// A wave's 32 x 32 block of a product at (i0, j0), as accumulated: lane holds column lane & 31, rows 8 (r / 4) + 4 (lane >> 5) +
+// r % 4.  It goes through `t` (the wave's own LDS) once, so that both the block and its transpose are stored 16 bytes a lane.
+// mirror: the transposed place is another block's (of a symmetric result).
+constexpr int TLD = 36;  // floats a row: 16-byte rows, and columns of eight spread over the banks
+constexpr int TBYTES = 32 * TLD * 4;
+
+__device__ __forceinline__ void finish(const Ops& s, const Op& q, const Lay& l, char* ws, int b, int i0, int j0, const f32x16& acc, bool mirror,
+                                       int dtype, float* t) {
+    const int lane = threadIdx.x & 63;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * TLD + (lane & 31)] = acc[r];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
     const int mp = (int)l.mp, np = (int)l.np;
     const int64_t sq = (int64_t)mp * mp;
     if (q.kind == RESULT) {
+        // eight consecutive elements of a row of the result a lane; a tall result is the transpose of the block
         const bool wide = q.rows <= q.cols;
+        const float step = s.update ? step_of(s, q.rows, q.cols) : 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int row = wide ? i + e : j, col = wide ? j : i + e;
-            if (row >= q.rows || col >= q.cols) continue;
+        for (int h = 0; h < 2; ++h) {
+            const int a = h * 16 + (lane >> 2), c = (lane & 3) * 8;
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = (wide ? t[a * TLD + c + e] : t[(c + e) * TLD + a]) * (1.f / (SP * SX));
+            const int row = (wide ? i0 : j0) + a, col = (wide ? j0 : i0) + c;
+            const int left = row < q.rows ? q.cols - col : 0;
             const int64_t at = ((int64_t)b * q.rows + row) * q.cols + col;
-            const float val = o[e] * (1.f / (SP * SX));
-            if (s.update == 0) {
-                if (dtype == GAN_F32) ((float*)q.out)[at] = val;
-                else ((bf16*)q.out)[at] = (bf16)val;
-            } else {
+            if (s.update) {
                 float* p = (float*)q.out + at;
-                *p = fmaf(-step_of(s, q.rows, q.cols), val, s.decay * *p);
+                float old[8];
+                if (left >= 8) {
+                    __builtin_memcpy(old, p, 32);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] = fmaf(-step, o[e], s.decay * old[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < left) o[e] = fmaf(-step, o[e], s.decay * p[e]);
+                }
+            }
+            if (dtype == GAN_F32) {
+                float* p = (float*)q.out + at;
+                if (left >= 8) {
+                    __builtin_memcpy(p, o, 32);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < left) p[e] = o[e];
+                }
+            } else {
+                bf16* p = (bf16*)q.out + at;
+                bf16 r[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[e] = (bf16)o[e];
+                if (left >= 8) {
+                    __builtin_memcpy(p, r, 16);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < left) p[e] = r[e];
+                }
             }
         }
         return;
@@ -259,43 +337,57 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, const Lay& l, 
     int64_t plane;
     int ldn = mp;
     if (q.kind == APPLY) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] *= 1.f / SP;
         dn = (h16*)(ws + (q.cur ? l.xm[0] : l.xm[1]));
         dt = (h16*)(ws + (q.cur ? l.xt[0] : l.xt[1]));
         plane = (int64_t)mp * np;
         ldn = np;
         mirror = true;
     } else {
-        if (q.kind == GRAM) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] *= SA / (SX * SX);
-        } else {
-            const h16* A = (const h16*)(ws + l.a) + (int64_t)j * mp + i;
-            const h16x4 ah = *(const h16x4*)A, al = *(const h16x4*)(A + sq);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float av = ((float)ah[e] + (float)al[e]) * (SP / SA);
-                o[e] = fmaf(s.c * (SP / (SA * SA)), o[e], s.b * av) + (i + e == j ? s.a * SP : 0.f);
-            }
-        }
         dn = dt = (h16*)(ws + (q.kind == GRAM ? l.a : l.p));
         plane = sq;
     }
-    h16x4 hi, lo;
+    const float gain = q.kind == APPLY ? 1.f / SP : q.kind == GRAM ? SA / (SX * SX) : s.c * (SP / (SA * SA));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        h16 p, w;
-        split(o[e], p, w);
-        hi[e] = p;
-        lo[e] = w;
-        dn[(int64_t)(i + e) * ldn + j] = p;
-        dn[plane + (int64_t)(i + e) * ldn + j] = w;
+    for (int h = 0; h < 2; ++h) {
+        const int a = h * 16 + (lane >> 2), c = (lane & 3) * 8, i = i0 + a, j = j0 + c;
+        h16x8 hi, lo, ah, al;
+        if (q.kind == POLY) {
+            const h16* A = (const h16*)(ws + l.a) + (int64_t)i * mp + j;
+            ah = *(const h16x8*)A;
+            al = *(const h16x8*)(A + sq);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float o = t[a * TLD + c + e] * gain;
+            if (q.kind == POLY) o += s.b * (((float)ah[e] + (float)al[e]) * (SP / SA)) + (i == j + e ? s.a * SP : 0.f);
+            if (mirror) t[a * TLD + c + e] = o;
+            h16 p, w;
+            split(o, p, w);
+            hi[e] = p;
+            lo[e] = w;
+        }
+        *(h16x8*)(dn + (int64_t)i * ldn + j) = hi;
+        *(h16x8*)(dn + plane + (int64_t)i * ldn + j) = lo;
     }
     if (mirror) {
-        *(h16x4*)(dt + (int64_t)j * mp + i) = hi;
-        *(h16x4*)(dt + plane + (int64_t)j * mp + i) = lo;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int a = h * 16 + (lane >> 2), c = (lane & 3) * 8;
+            h16x8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                h16 p, w;
+                split(t[(c + e) * TLD + a], p, w);
+                hi[e] = p;
+                lo[e] = w;
+            }
+            *(h16x8*)(dt + (int64_t)(j0 + a) * mp + i0 + c) = hi;
+            *(h16x8*)(dt + plane + (int64_t)(j0 + a) * mp + i0 + c) = lo;
+        }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
 // an address that is the same in every lane, in scalar registers
@@ -341,7 +433,8 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
     const int per = q.tiles * q.cut;
     const int b = __builtin_amdgcn_readfirstlane(((int)blockIdx.x - q.first) / per);
     const int in_b = (int)blockIdx.x - q.first - b * per;
-    const int slice = __builtin_amdgcn_readfirstlane(in_b / q.tiles), tile = in_b - slice * q.tiles;
+    // slices run fastest: workgroups go round the eight dies, so that a die's cache sees its slices' k only
+    const int tile = __builtin_amdgcn_readfirstlane(in_b / q.cut), slice = in_b - tile * q.cut;
     const Lay l = lay_of(q.rows, q.cols);
     char* ws = q.ws + b * q.stride;
     const int mp = (int)l.mp, np = (int)l.np;
@@ -452,45 +545,46 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
                     out[((x * FN + y) * 4 + r) * 64] = make_float4(acc[x][y][r * 4], acc[x][y][r * 4 + 1], acc[x][y][r * 4 + 2], acc[x][y][r * 4 + 3]);
         return;
     }
-    // lane holds column lane & 31, rows 8 r + 4 (lane >> 5) ... + 3 of each 32 x 32 block
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // (the stages are read: their LDS is free)
+    float* t = (float*)(lds + wave * TBYTES);
 #pragma unroll
-    for (int x = 0; x < FM; ++x) {
+    for (int x = 0; x < FM; ++x)
 #pragma unroll
         for (int y = 0; y < FN; ++y) {
-            const int i = i0 + wm * (T / 2) + x * 32 + 4 * (lane >> 5), j = j0 + wn * (T / WN) + y * 32 + (lane & 31);
-            if (i >= M || j >= N) continue;  // (whole blocks of 32 either way)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float o[4] = {acc[x][y][r * 4], acc[x][y][r * 4 + 1], acc[x][y][r * 4 + 2], acc[x][y][r * 4 + 3]};
-                finish(s, q, l, ws, b, i + 8 * r, j, o, sym && ti != tj, dtype);
-            }
+            const int i = i0 + wm * (T / 2) + x * 32, j = j0 + wn * (T / WN) + y * 32;
+            if (i < M && j < N) finish(s, q, l, ws, b, i, j, acc[x][y], sym && ti != tj, dtype, t);
         }
-    }
 }
 
-// The slices of a product that was cut, added in their order; one float4 (four rows of a column) a thread
+// The slices of a product that was cut, added in their order; a 32 x 32 block a wave
 template <int T>
 __global__ void __launch_bounds__(256) ortho_join_k(const Ops s, int dtype) {
-    constexpr int WAVES = T == 256 ? 8 : 4, WN = WAVES / 2, FN = T / 32 / WN, PERT = T * T / 1024;  // workgroups of this kernel per tile
+    constexpr int WAVES = gemm_threads<T>() / 64, WN = WAVES / 2, FN = T / 32 / WN, BLK = T * T / 1024;  // blocks of a tile
+    __shared__ __attribute__((aligned(16))) float lds[4][TBYTES / 4];
     const Op& q = s.mat[group_of(s, blockIdx.x)];
-    const int local = (int)blockIdx.x - q.first, tile_b = local / PERT, b = tile_b / q.tiles, tile = tile_b - b * q.tiles;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int local = ((int)blockIdx.x - q.first) * 4 + wv, tile_b = local / BLK, b = tile_b / q.tiles, tile = tile_b - b * q.tiles;
     const Lay l = lay_of(q.rows, q.cols);
     char* ws = q.ws + b * q.stride;
-    const int at = local % PERT * 256 + threadIdx.x;
-    const float4* in = (const float4*)(ws + l.join) + (int64_t)tile * (T * T / 4) + at;
-    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    const int blk = local % BLK, wave = blk / (BLK / WAVES), frag = blk % (BLK / WAVES);
+    const float4* in = (const float4*)(ws + l.join) + (int64_t)tile * (T * T / 4) + blk * 256 + lane;
+    f32x16 acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
     for (int c = 0; c < q.cut; ++c) {
-        const float4 v = in[(int64_t)c * q.tiles * (T * T / 4)];
-        o[0] += v.x;
-        o[1] += v.y;
-        o[2] += v.z;
-        o[3] += v.w;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float4 v = in[(int64_t)c * q.tiles * (T * T / 4) + r * 64];
+            acc[r * 4] += v.x;
+            acc[r * 4 + 1] += v.y;
+            acc[r * 4 + 2] += v.z;
+            acc[r * 4 + 3] += v.w;
+        }
     }
-    const int lane = at & 63, r = at >> 6 & 3, frag = (at >> 8) % (T * T / WAVES / 1024), wave = at / (T * T / 4 / WAVES);
     const int2 t = tile_of(tile, (int)(l.mp + T - 1) / T);
-    const int i = t.x * T + (wave / WN) * (T / 2) + frag / FN * 32 + 8 * r + 4 * (lane >> 5);
-    const int j = t.y * T + (wave % WN) * (T / WN) + frag % FN * 32 + (lane & 31);
-    if (i < l.mp && j < l.mp) finish(s, q, l, ws, b, i, j, o, t.x != t.y, dtype);
+    const int i = t.x * T + (wave / WN) * (T / 2) + frag / FN * 32, j = t.y * T + (wave % WN) * (T / WN) + frag % FN * 32;
+    if (i < l.mp && j < l.mp) finish(s, q, l, ws, b, i, j, acc, t.x != t.y, dtype, lds[wv]);
 }
 
 template <int T, int NST>
@@ -554,7 +648,7 @@ int products(const gan_matrix* mats, int n, int kind, int cur, Ops& s, char* ws,
         if (s.mat[k].cut == 1) continue;
         s.mat[m] = s.mat[k];
         s.mat[m++].first = (int)join;
-        join += (int64_t)s.mat[m - 1].tiles * mats[k].batch * (T * T / 1024);
+        join += (int64_t)s.mat[m - 1].tiles * mats[k].batch * (T * T / 4096);
     }
     if (!m) return GAN_OK;
     s.count = m;
@@ -609,10 +703,10 @@ int64_t total_bytes(const gan_matrix* mats, int count) {
     return n;
 }
 
-// The three launches in front of the products: momentum and norms, scales, planes.
+// The two launches in front of the products: momentum and norms, planes.
 template <typename T>
 int pack(const gan_matrix* mats, int n, char* ws, Mats& s, hipStream_t st) {
-    int64_t first[3][NOPS + 1] = {};
+    int64_t first[2][NOPS + 1] = {};
     s.count = n;
     for (int k = 0; k < n; ++k) {
         const gan_matrix& g = mats[k];
@@ -625,14 +719,13 @@ int pack(const gan_matrix* mats, int n, char* ws, Mats& s, hipStream_t st) {
         q.rows = (int)g.rows;
         q.cols = (int)g.cols;
         ws += l.bytes * g.batch;
-        const int64_t per[3] = {l.nparts, 1, l.mp / 64 * (l.np / 64)};
-        for (int j = 0; j < 3; ++j) first[j][k + 1] = first[j][k] + per[j] * g.batch;
+        const int64_t per[2] = {l.nparts, l.mp / 64 * (l.np / 64)};
+        for (int j = 0; j < 2; ++j) first[j][k + 1] = first[j][k] + per[j] * g.batch;
     }
-    for (int j = 0; j < 3; ++j) {
+    for (int j = 0; j < 2; ++j) {
         for (int k = 0; k < n; ++k) s.mat[k].first = (int)first[j][k];
         const dim3 grid((unsigned)first[j][n]), block(256);
         if (j == 0) hipLaunchKernelGGL((ortho_norm_k<T>), grid, block, 0, st, s);
-        else if (j == 1) hipLaunchKernelGGL(ortho_scale_k, grid, block, 0, st, s);
         else hipLaunchKernelGGL((ortho_pack_k<T>), grid, block, 0, st, s);
         GAN_CHECK_LAUNCH("orthogonalize(source)");
     }
