@@ -22,7 +22,7 @@ constexpr int NOPS = 32;         // matrices of one launch (their descriptions a
 constexpr int64_t MAXGRID = 1LL << 31;
 constexpr float SX = 16384.f;    // |X| <= 3.9: fp16 ends at 65504
 constexpr float SA = 4096.f;     // |A| <= 15.9
-constexpr float SP = 1024.f;     // |P| <= 63
+constexpr float SP = 16.f;       // |P| and products of two of them <= 4000
 
 __host__ __device__ inline int64_t up64(int64_t v) { return (v + PAD - 1) / PAD * PAD; }
 
@@ -44,6 +44,7 @@ struct Mat {
     float* buf;      // momentum (NULL: orthogonalise g itself)
     char* ws;        // workspace of the first
     int64_t stride;
+    int64_t nat, tra;  // offsets of the planes that lie as the source does, and transposed
     int rows, cols;
     int first;       // first workgroup of this launch that works on the group
 };
@@ -57,28 +58,55 @@ struct Mats {
     float eps;
 };
 
-// How a product over k is cut when its tiles alone would leave most of the chip idle (A = X X' of a long X): slices of at least
-// 512 k, together with the tiles no more than two 64 x 64 workgroups a CU.  By the matrix's own shape, so that its bits do
-// not depend on what else is in the call.
-__host__ __device__ inline int splits_of(int64_t mp, int64_t np) {
-    const int64_t t = mp / 64, tiles = t * (t + 1) / 2, most = np / 512, s = 512 / tiles;
-    return (int)(s < most ? (s > 1 ? s : 1) : (most > 1 ? most : 1));
-}
-
-// Byte offsets in one matrix's workspace: the partial sums, two X (each [m][n] and [n][m], hi plane then lo
-// plane), A, P, the slices' tiles of a product that is cut.
+// Byte offsets in one matrix's workspace: the partial sums, two X (each [m][n] and [n][m], hi plane then lo plane), five
+// symmetric m x m, the slices' tiles of a product that is cut.  All multiples of 256.
+enum { A0, A1, P0, P1, Q0, SQUARES };
 struct Lay {
-    int64_t mp, np, part, nparts, xm[2], xt[2], a, p, join, bytes;
+    int64_t mp, np, nparts, xm[2], xt[2], sq[SQUARES], join, bytes;
+    int cut;
 };
 
-__host__ __device__ inline Lay lay_of(int64_t rows, int64_t cols) {
+// What a product of `tiles` T x T tiles over `steps` steps of 32 k takes, in us, every tile's k in `cut` slices: workgroups run
+// in rounds, 256 (T = 256) or 512 of them at a time, a step of theirs as long as measured (T = 256: 2.8; T = 128: 0.55 alone
+// on a CU, 0.83 each where two share it; T = 64: 0.27 and 0.33), and slices are written and read again at 5 TB/s by one more launch.
+double cost_of(int T, int64_t tiles, int cut, int64_t steps) {
+    const int64_t wgs = tiles * cut, slots = T < 256 && wgs > 256 ? 512 : 256;
+    const double alone = T == 256 ? 2.8 : T == 128 ? 0.55 : 0.27, shared = T == 128 ? 1.66 : 0.66;
+    return (double)ceil_div64(wgs, slots) * (double)ceil_div64(steps, cut) * (slots == 512 ? shared : alone) +
+           (cut > 1 ? 5. + (double)wgs * T * T * 8e-6 / 5. : 0.);
+}
+
+int64_t tiles_of(int64_t M, int64_t N, bool sym, int T) {
+    const int64_t tm = (M + T - 1) / T, tn = (N + T - 1) / T;
+    return sym ? tm * (tm + 1) / 2 : tm * tn;
+}
+
+// Slices of A = X X' (a long k, few tiles), at least eight steps each.  By the matrix's own shape, so that its bits do not
+// depend on what else is in the call.
+int cut_of(int64_t mp, int64_t np) {
+    int best = 1;
+    double least = 1e30;
+    for (int T = 64; T <= 256; T *= 2) {
+        const int64_t tiles = tiles_of(mp, mp, true, T), steps = np / 32;
+        int64_t cut = 256 / tiles;
+        if (cut > steps / 8) cut = steps / 8;
+        if (cut < 1) cut = 1;
+        const double c = cost_of(T, tiles, (int)cut, steps);
+        if (c < least) {
+            least = c;
+            best = (int)cut;
+        }
+    }
+    const int64_t steps = np / 32, each = ceil_div64(steps, best);
+    return (int)ceil_div64(steps, each);
+}
+
+Lay lay_of(int64_t rows, int64_t cols) {
     Lay l;
     l.mp = up64(rows < cols ? rows : cols);
     l.np = up64(rows < cols ? cols : rows);
     l.nparts = parts_of(rows * cols);
-    int64_t at = 0;
-    l.part = at;
-    at += (l.nparts * 8 + 255) / 256 * 256;
+    int64_t at = MAXPARTS * 8;
     const int64_t x = l.mp * l.np * 4, sq = l.mp * l.mp * 4;
     for (int k = 0; k < 2; ++k) {
         l.xm[k] = at;
@@ -86,14 +114,14 @@ __host__ __device__ inline Lay lay_of(int64_t rows, int64_t cols) {
         l.xt[k] = at;
         at += x;
     }
-    l.a = at;
-    at += sq;
-    l.p = at;
-    at += sq;
+    for (int k = 0; k < SQUARES; ++k) {
+        l.sq[k] = at;
+        at += sq;
+    }
     l.join = at;
-    const int cut = splits_of(l.mp, l.np);
+    l.cut = cut_of(l.mp, l.np);
     const int64_t t = (l.mp + 255) / 256 * 4;  // in whole tiles of the largest size
-    if (cut > 1) at += cut * t * (t + 4) / 2 * 4096 * 4;
+    if (l.cut > 1) at += l.cut * t * (t + 4) / 2 * 4096 * 4;
     l.bytes = at;
     return l;
 }
@@ -207,11 +235,8 @@ __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
         tile[r][c] = in ? scale * (buf ? update_of(s, v[k], m[k]) : v[k]) : 0.f;
     }
     __syncthreads();
-    const Lay l = lay_of(q.rows, q.cols);
-    const bool wide = q.rows <= q.cols;
-    h16* nat = (h16*)(ws + (wide ? l.xm[0] : l.xt[0]));
-    h16* tra = (h16*)(ws + (wide ? l.xt[0] : l.xm[0]));
-    const int64_t plane = l.mp * l.np;
+    h16 *nat = (h16*)(ws + q.nat), *tra = (h16*)(ws + q.tra);
+    const int64_t plane = (int64_t)rp * cp;
     for (int k = threadIdx.x; k < 64 * 8; k += 256) {
         const int r = k >> 3, c = (k & 7) * 8;
         h16x8 hi, lo, thi, tlo;
@@ -234,22 +259,28 @@ __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
 }
 
 // ---- products ----------------------------------------------------------------------------------------------------------
-enum Kind { GRAM = 0, POLY = 1, APPLY = 2, RESULT = 3 };
+enum Kind { SCALED, POLY, RESULT };
 
+// C = U V' of one group of equal matrices
 struct Op {
-    char* ws;        // of the group's first matrix
+    char* ws;          // of the group's first matrix
     int64_t stride;
-    void* out;       // RESULT
-    int rows, cols;  // of the source
-    int first, tiles;  // first workgroup, workgroups per matrix
-    int kind, cur;     // cur: which X holds the iterate
+    void* out;         // RESULT
+    unsigned u, v;     // operands, results [i][j] and [j][i], POLY's A, slices: in 256 bytes from ws
+    unsigned dn, dt, aux, join;
+    int M, N, K;       // padded; symmetric results (dn == dt) have tiles on and above the diagonal only
+    int rows, cols;    // of the source
+    int first, tiles;  // first workgroup, tiles per matrix
     int cut, steps;    // slices of k, steps of 32 k in each but the last
+    int kind;
+    float gain;        // SCALED: result = gain * accumulator
 };
 
 struct Ops {
     Op mat[NOPS];
     int count;
     float a, b, c;
+    int sliced;         // some product of the launch is cut
     float decay, step;  // RESULT onto parameters: p = decay p - step_of(rows, cols) X
     int update;         // 0: out = X; 1: the parameters; 2, 3: the step scaled by the shape, see step_of
 };
@@ -272,7 +303,7 @@ __device__ __forceinline__ int2 tile_of(int t, int n) {
 constexpr int TLD = 36;  // floats a row: 16-byte rows, and columns of eight spread over the banks
 constexpr int TBYTES = 32 * TLD * 4;
 
-__device__ __forceinline__ void finish(const Ops& s, const Op& q, const Lay& l, char* ws, int b, int i0, int j0, const f32x16& acc, bool mirror,
+__device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int b, int i0, int j0, const f32x16& acc, bool mirror,
                                        int dtype, float* t) {
     const int lane = threadIdx.x & 63;
     __builtin_amdgcn_wave_barrier();
@@ -280,8 +311,6 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, const Lay& l, 
     for (int r = 0; r < 16; ++r) t[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * TLD + (lane & 31)] = acc[r];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
-    const int mp = (int)l.mp, np = (int)l.np;
-    const int64_t sq = (int64_t)mp * mp;
     if (q.kind == RESULT) {
         // eight consecutive elements of a row of the result a lane; a tall result is the transpose of the block
         const bool wide = q.rows <= q.cols;
@@ -333,28 +362,17 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, const Lay& l, 
         }
         return;
     }
-    h16 *dn, *dt;  // [i][j] and [j][i]
-    int64_t plane;
-    int ldn = mp;
-    if (q.kind == APPLY) {
-        dn = (h16*)(ws + (q.cur ? l.xm[0] : l.xm[1]));
-        dt = (h16*)(ws + (q.cur ? l.xt[0] : l.xt[1]));
-        plane = (int64_t)mp * np;
-        ldn = np;
-        mirror = true;
-    } else {
-        dn = dt = (h16*)(ws + (q.kind == GRAM ? l.a : l.p));
-        plane = sq;
-    }
-    const float gain = q.kind == APPLY ? 1.f / SP : q.kind == GRAM ? SA / (SX * SX) : s.c * (SP / (SA * SA));
+    h16 *dn = (h16*)(ws + (int64_t)q.dn * 256), *dt = (h16*)(ws + (int64_t)q.dt * 256);  // [i][j] and [j][i]
+    const int64_t plane = (int64_t)q.M * q.N;
+    const float gain = q.kind == SCALED ? q.gain : s.c * (SP / (SA * SA));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int a = h * 16 + (lane >> 2), c = (lane & 3) * 8, i = i0 + a, j = j0 + c;
         h16x8 hi, lo, ah, al;
         if (q.kind == POLY) {
-            const h16* A = (const h16*)(ws + l.a) + (int64_t)i * mp + j;
+            const h16* A = (const h16*)(ws + (int64_t)q.aux * 256) + (int64_t)i * q.N + j;
             ah = *(const h16x8*)A;
-            al = *(const h16x8*)(A + sq);
+            al = *(const h16x8*)(A + plane);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -366,8 +384,8 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, const Lay& l, 
             hi[e] = p;
             lo[e] = w;
         }
-        *(h16x8*)(dn + (int64_t)i * ldn + j) = hi;
-        *(h16x8*)(dn + plane + (int64_t)i * ldn + j) = lo;
+        *(h16x8*)(dn + (int64_t)i * q.N + j) = hi;
+        *(h16x8*)(dn + plane + (int64_t)i * q.N + j) = lo;
     }
     if (mirror) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -383,8 +401,8 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, const Lay& l, 
                 hi[e] = p;
                 lo[e] = w;
             }
-            *(h16x8*)(dt + (int64_t)(j0 + a) * mp + i0 + c) = hi;
-            *(h16x8*)(dt + plane + (int64_t)(j0 + a) * mp + i0 + c) = lo;
+            *(h16x8*)(dt + (int64_t)(j0 + a) * q.M + i0 + c) = hi;
+            *(h16x8*)(dt + plane + (int64_t)(j0 + a) * q.M + i0 + c) = lo;
         }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -396,19 +414,44 @@ __device__ __forceinline__ const char* scalar(const char* p) {
     const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
     return (const char*)(((uint64_t)hi << 32) | lo);
 }
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_from(const char* p) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)scalar(p), 0, 0xffffffffu, 0x00020000);
+// One LDS-DMA instruction: a wave's instruction j covers 1 KB = 16 rows of plane j / PP of the stage of k step `step` at `base`.
+// p: the planes' first rows.
+template <int WAVES, int PP>
+__device__ __forceinline__ void ortho_issue(char* base, int step, int wave, const char* const* p, const unsigned* off, int j) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)p[j / PP], 0, 0xffffffffu, 0x00020000),
+                                             (__attribute__((address_space(3))) void*)(base + (WAVES * j + wave) * 1024), 16, off[j], step * 64, 0, 0);
 }
 
-// LDS-DMA of k step `step` into `base`: a wave's instruction j covers 1 KB = 16 rows of plane j / PP
-template <int WAVES, int PP, int PER>
-__device__ __forceinline__ void ortho_issue(char* base, int step, int wave, __amdgpu_buffer_rsrc_t ru, __amdgpu_buffer_rsrc_t rul,
-                                            __amdgpu_buffer_rsrc_t rv, __amdgpu_buffer_rsrc_t rvl, const unsigned (&off)[PER]) {
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(j / PP == 0 ? ru : j / PP == 1 ? rul : j / PP == 2 ? rv : rvl,
-                                                 (__attribute__((address_space(3))) void*)(base + (WAVES * j + wave) * 1024), 16, off[j], step * 64,
-                                                 0, 0);
+// The fragments of 16 k of a wave's tile, from the stage at `base`: rows m0 ... of U, n0 ... of V
+template <int FM, int FN>
+struct Frags {
+    static constexpr int READS = 2 * (FM + FN), PRODUCTS = 3 * FM * FN;
+    h16x8 u[2][FM], v[2][FN];  // hi, lo
+    __device__ __forceinline__ void read(const char* base, int plane, int m0, int n0, int half, int lane, int r) {
+        const bool of_u = r < 2 * FM;
+        const int f = (of_u ? r : r - 2 * FM) >> 1, pl = r & 1, ch = half * 2 + (lane >> 5);
+        const int row = (of_u ? m0 : n0) + f * 32 + (lane & 31), at = row * 64 + ((ch ^ ((row >> 2) & 3)) << 4);
+        const h16x8 got = *(const h16x8*)(base + (of_u ? pl : 2 + pl) * plane + at);
+        if (of_u) u[pl][f] = got;
+        else v[pl][f] = got;
+    }
+    // hi lo, lo hi, hi hi, each over all of the wave's blocks (a block's accumulator then rests between two products)
+    __device__ __forceinline__ void multiply(f32x16 (&acc)[FM][FN], int i) const {
+        const int pass = i / (FM * FN), x = i % (FM * FN) / FN, y = i % FN;
+        acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[pass == 1][x], v[pass == 0][y], acc[x][y], 0, 0, 0);
+    }
+};
+
+// Waits until a stage is in LDS for everyone and everyone's earlier reads are done: this wave's last N requests may still be on
+// their way if all of them are (`full`: later stages), else none.
+template <int N>
+__device__ __forceinline__ void stage_arrived(bool full) {
+    if (full)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 template <int T>
@@ -427,34 +470,24 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
     constexpr int PER = STAGE / 1024 / WAVES;                      // DMA instructions per wave and stage
     constexpr int PP = PER / 4;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
-    const Op& q = s.mat[group_of(s, blockIdx.x)];
+    // Workgroups go round the eight dies, each with a cache of its own.  Slices run fastest, so that a die meets few of them;
+    // where nothing is cut, a die gets a run of tiles that share their rows of V.
+    int id = blockIdx.x;
+    if (!s.sliced) {
+        const int each = gridDim.x >> 3, rest = gridDim.x & 7, die = id & 7;
+        id = die * each + (die < rest ? die : rest) + (id >> 3);
+    }
+    const Op& q = s.mat[group_of(s, id)];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
     // (divisions run on vector registers: say that the results are the wave's, or every use of an address loops over lanes)
     const int per = q.tiles * q.cut;
-    const int b = __builtin_amdgcn_readfirstlane(((int)blockIdx.x - q.first) / per);
-    const int in_b = (int)blockIdx.x - q.first - b * per;
-    // slices run fastest: workgroups go round the eight dies, so that a die's cache sees its slices' k only
+    const int b = __builtin_amdgcn_readfirstlane((id - q.first) / per);
+    const int in_b = id - q.first - b * per;
     const int tile = __builtin_amdgcn_readfirstlane(in_b / q.cut), slice = in_b - tile * q.cut;
-    const Lay l = lay_of(q.rows, q.cols);
     char* ws = q.ws + b * q.stride;
-    const int mp = (int)l.mp, np = (int)l.np;
-    // operands
-    const bool sym = q.kind <= POLY;
-    const char *u, *v;
-    int M, N, K;
-    if (q.kind == GRAM) {
-        u = v = ws + (q.cur ? l.xm[1] : l.xm[0]);
-        M = N = mp;
-        K = np;
-    } else if (q.kind == POLY) {
-        u = v = ws + l.a;
-        M = N = K = mp;
-    } else {
-        u = ws + l.p;
-        v = ws + (q.cur ? l.xt[1] : l.xt[0]);
-        M = K = mp;
-        N = np;
-    }
+    const char *u = ws + (int64_t)q.u * 256, *v = ws + (int64_t)q.v * 256;
+    const int M = q.M, N = q.N, K = q.K;
+    const bool sym = q.kind != RESULT && q.dn == q.dt;
     int ti, tj;
     if (sym) {
         const int2 t = tile_of(tile, (M + T - 1) / T);
@@ -470,10 +503,8 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
     const unsigned kb = (unsigned)K * 2;
     unsigned off[PER];
     const int rsub = lane >> 2, pos = lane & 3;
-    const __amdgpu_buffer_rsrc_t ru = rows_from(u + (int64_t)i0 * kb);
-    const __amdgpu_buffer_rsrc_t rul = rows_from(u + ((int64_t)M + i0) * kb);
-    const __amdgpu_buffer_rsrc_t rv = rows_from(v + (int64_t)j0 * kb);
-    const __amdgpu_buffer_rsrc_t rvl = rows_from(v + ((int64_t)N + j0) * kb);
+    const char* const planes[4] = {scalar(u + (int64_t)i0 * kb), scalar(u + ((int64_t)M + i0) * kb), scalar(v + (int64_t)j0 * kb),
+                                   scalar(v + ((int64_t)N + j0) * kb)};
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         const int piece = WAVES * j + wave, pl = piece / (T / 16), row = piece % (T / 16) * 16 + rsub;
@@ -490,52 +521,68 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
     const int k0 = slice * q.steps, nk = (K / 32 - k0 < q.steps ? K / 32 - k0 : q.steps);
 #pragma unroll
-    for (int k = 0; k < NST - 1; ++k)
-        if (k < nk) ortho_issue<WAVES, PP, PER>(lds + k * STAGE, k0 + k, wave, ru, rul, rv, rvl, off);
-    for (int k = 0; k < nk; ++k) {
-        // this wave's share of stage k has arrived and its reads of the stage before are done ...
-        if (k + NST - 1 < nk + 1)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NST - 2) * PER) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        // ... and everyone's
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (k + NST - 1 < nk)
-            ortho_issue<WAVES, PP, PER>(lds + (k + NST - 1) % NST * STAGE, k0 + k + NST - 1, wave, ru, rul, rv, rvl, off);
-        const char* base = lds + k % NST * STAGE;
+    for (int k = 0; k < NST; ++k)
+        if (k < nk) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            h16x8 uh[FM], ul[FM], vh[FN], vl[FN];
-            const int ch = h * 2 + (lane >> 5);
-#pragma unroll
-            for (int x = 0; x < FM; ++x) {
-                const int row = wm * (T / 2) + x * 32 + (lane & 31), at = row * 64 + ((ch ^ ((row >> 2) & 3)) << 4);
-                uh[x] = *(const h16x8*)(base + at);
-                ul[x] = *(const h16x8*)(base + PLANE + at);
-            }
-#pragma unroll
-            for (int y = 0; y < FN; ++y) {
-                const int row = wn * (T / WN) + y * 32 + (lane & 31), at = row * 64 + ((ch ^ ((row >> 2) & 3)) << 4);
-                vh[y] = *(const h16x8*)(base + 2 * PLANE + at);
-                vl[y] = *(const h16x8*)(base + 3 * PLANE + at);
-            }
-#pragma unroll
-            for (int x = 0; x < FM; ++x)
-#pragma unroll
-                for (int y = 0; y < FN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh[x], vl[y], acc[x][y], 0, 0, 0);
-#pragma unroll
-            for (int x = 0; x < FM; ++x)
-#pragma unroll
-                for (int y = 0; y < FN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul[x], vh[y], acc[x][y], 0, 0, 0);
-#pragma unroll
-            for (int x = 0; x < FM; ++x)
-#pragma unroll
-                for (int y = 0; y < FN; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh[x], vh[y], acc[x][y], 0, 0, 0);
+            for (int j = 0; j < PER; ++j) ortho_issue<WAVES, PP>(lds + k * STAGE, k0 + k, wave, planes, off, j);
         }
+    // While the matrix instructions of one half of a stage (16 k) run, the other half's fragments are read and DMA is asked for,
+    // a piece behind each: eight requests in a row would hold the wave at the address unit (64 bytes a clock for the CU) for as
+    // long as a third of its products take.  The barrier lies between the halves, where the next stage has to be there and
+    // nobody reads this one any more; its place is then filled with stage k + NST, half of the requests before and half after
+    // the next half's turn.
+    using Fr = Frags<FM, FN>;
+    constexpr int HALF = PER / 2;
+    const int m0 = wm * (T / 2), n0 = wn * (T / WN);
+    Fr f0, f1;
+    stage_arrived<(NST - 1) * PER>(nk >= NST);
+#pragma unroll
+    for (int r = 0; r < Fr::READS; ++r) f0.read(lds, PLANE, m0, n0, 0, lane, r);
+    auto step = [&](int k, bool late, bool more) __attribute__((always_inline)) {
+        char *here = lds + k % NST * STAGE, *last = lds + (k + NST - 1) % NST * STAGE, *next = lds + (k + 1) % NST * STAGE;
+#pragma unroll
+        for (int i = 0; i < Fr::PRODUCTS; ++i) {
+            f0.multiply(acc, i);
+#pragma unroll
+            for (int r = 0; r < Fr::READS; ++r)
+                if (r * Fr::PRODUCTS / Fr::READS == i) f1.read(here, PLANE, m0, n0, 1, lane, r);
+            if (late) {
+#pragma unroll
+                for (int j = 0; j < HALF; ++j)
+                    if (j * Fr::PRODUCTS / HALF == i) ortho_issue<WAVES, PP>(last, k0 + k - 1 + NST, wave, planes, off, HALF + j);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        stage_arrived<(NST - 2) * PER>(k + NST - 1 < nk);  // stages k + 2 ... k + NST - 1 behind it
+#pragma unroll
+        for (int i = 0; i < Fr::PRODUCTS; ++i) {
+            f1.multiply(acc, i);
+#pragma unroll
+            for (int r = 0; r < Fr::READS; ++r)
+                if (r * Fr::PRODUCTS / Fr::READS == i) f0.read(next, PLANE, m0, n0, 0, lane, r);
+            if (more) {
+#pragma unroll
+                for (int j = 0; j < HALF; ++j)
+                    if (j * Fr::PRODUCTS / HALF == i) ortho_issue<WAVES, PP>(here, k0 + k + NST, wave, planes, off, j);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    if (nk > 1) step(0, false, NST < nk);
+    int k = 1;
+    for (; k + NST < nk; ++k) step(k, true, true);
+    for (; k + 1 < nk; ++k) step(k, k - 1 + NST < nk, false);
+    {
+        const char* here = lds + (nk - 1) % NST * STAGE;
+#pragma unroll
+        for (int r = 0; r < Fr::READS; ++r) f1.read(here, PLANE, m0, n0, 1, lane, r);
+#pragma unroll
+        for (int i = 0; i < Fr::PRODUCTS; ++i) f0.multiply(acc, i);
+#pragma unroll
+        for (int i = 0; i < Fr::PRODUCTS; ++i) f1.multiply(acc, i);
     }
     if (q.cut > 1) {  // this slice's sums, in the order that join_k reads them
-        float4* out = (float4*)(ws + l.join) + ((int64_t)slice * q.tiles + tile) * (T * T / 4) + wave * (T * T / 4 / WAVES) + lane;
+        float4* out = (float4*)(ws + (int64_t)q.join * 256) + ((int64_t)slice * q.tiles + tile) * (T * T / 4) + wave * (T * T / 4 / WAVES) + lane;
 #pragma unroll
         for (int x = 0; x < FM; ++x)
 #pragma unroll
@@ -553,7 +600,7 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
 #pragma unroll
         for (int y = 0; y < FN; ++y) {
             const int i = i0 + wm * (T / 2) + x * 32, j = j0 + wn * (T / WN) + y * 32;
-            if (i < M && j < N) finish(s, q, l, ws, b, i, j, acc[x][y], sym && ti != tj, dtype, t);
+            if (i < M && j < N) finish(s, q, ws, b, i, j, acc[x][y], !sym || ti != tj, dtype, t);
         }
 }
 
@@ -565,10 +612,9 @@ __global__ void __launch_bounds__(256) ortho_join_k(const Ops s, int dtype) {
     const Op& q = s.mat[group_of(s, blockIdx.x)];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int local = ((int)blockIdx.x - q.first) * 4 + wv, tile_b = local / BLK, b = tile_b / q.tiles, tile = tile_b - b * q.tiles;
-    const Lay l = lay_of(q.rows, q.cols);
     char* ws = q.ws + b * q.stride;
     const int blk = local % BLK, wave = blk / (BLK / WAVES), frag = blk % (BLK / WAVES);
-    const float4* in = (const float4*)(ws + l.join) + (int64_t)tile * (T * T / 4) + blk * 256 + lane;
+    const float4* in = (const float4*)(ws + (int64_t)q.join * 256) + (int64_t)tile * (T * T / 4) + blk * 256 + lane;
     f32x16 acc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] = 0.f;
@@ -582,9 +628,9 @@ __global__ void __launch_bounds__(256) ortho_join_k(const Ops s, int dtype) {
             acc[r * 4 + 3] += v.w;
         }
     }
-    const int2 t = tile_of(tile, (int)(l.mp + T - 1) / T);
+    const int2 t = tile_of(tile, (q.M + T - 1) / T);
     const int i = t.x * T + (wave / WN) * (T / 2) + frag / FN * 32, j = t.y * T + (wave % WN) * (T / WN) + frag % FN * 32;
-    if (i < l.mp && j < l.mp) finish(s, q, l, ws, b, i, j, acc, t.x != t.y, dtype, lds[wv]);
+    if (i < q.M && j < q.N) finish(s, q, ws, b, i, j, acc, t.x != t.y, dtype, lds[wv]);
 }
 
 template <int T, int NST>
@@ -600,57 +646,129 @@ int launch_gemm(unsigned blocks, const Ops& s, int dtype, hipStream_t st) {
     return GAN_OK;
 }
 
-int64_t tiles_of(const Lay& l, int kind, int T) {
-    const int64_t tm = (l.mp + T - 1) / T, tn = (l.np + T - 1) / T;
-    return kind <= POLY ? tm * (tm + 1) / 2 : tm * tn;
-}
+// What a matrix does in the launches, one after another: stages of one or two iterations, each from A = X X' anew.
+//   one:  P = poly(A);                                                     X <- P X
+//   two:  P = poly(A), T = P A, A2 = P T (= X2 X2'), P2 = poly(A2), Q = P2 P;  X <- Q X
+// Two iterations at a time replace a product with X and one into it by three m x m ones: 6 m^2 n + 2 m^3 against
+// 3 m^2 n + 5 m^3, which pays from n = 2 m on.  Not more at a time: an error of A, 2^-22 of its largest singular value, weighs
+// the more on the smallest ones the longer the iteration runs on A alone (error against 64 bits, 512 x 4608 with a spectrum that
+// falls like 1 / i: 1.9e-6 step by step, 3.1e-6 like this, 7.8e-6 in stages of two and three, 1.7e-4 in one).  The first
+// stage is a single iteration: the small values are smallest there.
+int stage_of(const Lay& l, int left, int steps) { return l.np >= 2 * l.mp && left < steps && left >= 2 ? 2 : 1; }
 
-// One product of every matrix: one launch, and one more that joins slices where there are any.
-int products(const gan_matrix* mats, int n, int kind, int cur, Ops& s, char* ws, int dtype, hipStream_t st) {
-    // The largest tile with which there is a workgroup for every CU: the larger, the fewer bytes go through LDS for a product.
-    int T = 256;
-    for (; T > 64; T >>= 1) {
-        int64_t all = 0;
-        for (int k = 0; k < n; ++k) {
-            const Lay l = lay_of(mats[k].rows, mats[k].cols);
-            all += tiles_of(l, kind, T) * (kind == GRAM ? splits_of(l.mp, l.np) : 1) * mats[k].batch;
+struct Walk {
+    Lay l;
+    int left, size, at, cur;  // iterations left, this stage's size, the next product within it, the X that holds the iterate
+    void next(Op& q, int steps) {
+        if (at == 0) size = stage_of(l, left, steps);
+        auto sq = [&](int k) { return (unsigned)(l.sq[k] / 256); };
+        auto mul = [&](int u, int v, int to, float gain) {
+            q.u = sq(u);
+            q.v = sq(v);
+            q.dn = q.dt = sq(to);
+            q.gain = gain;
+            q.M = q.N = q.K = (int)l.mp;
+        };
+        q.kind = SCALED;
+        q.cut = 1;
+        q.aux = 0;
+        const int last = size == 1 ? 2 : 6;
+        if (at == 0) {
+            mul(0, 0, A0, SA / (SX * SX));
+            q.u = q.v = (unsigned)(l.xm[cur] / 256);
+            q.K = (int)l.np;
+            q.cut = l.cut;
+        } else if (at == last) {
+            const bool end = left == size;
+            q.kind = end ? RESULT : SCALED;
+            q.u = sq(size == 1 ? P0 : Q0);
+            q.v = (unsigned)(l.xt[cur] / 256);
+            q.dn = (unsigned)(l.xm[cur ^ 1] / 256);
+            q.dt = (unsigned)(l.xt[cur ^ 1] / 256);
+            q.gain = 1.f / SP;
+            q.M = q.K = (int)l.mp;
+            q.N = (int)l.np;
+        } else if (at == 1) {
+            mul(A0, A0, P0, 0.f);
+            q.kind = POLY;
+            q.aux = sq(A0);
+        } else if (at == 2) {
+            mul(P0, A0, Q0, 1.f / SP);
+        } else if (at == 3) {
+            mul(P0, Q0, A1, 1.f / SP);
+        } else if (at == 4) {
+            mul(A1, A1, P1, 0.f);
+            q.kind = POLY;
+            q.aux = sq(A1);
+        } else {
+            mul(P1, P0, Q0, 1.f / SP);
         }
-        if (all >= 256) break;
+        if (at++ == last) {
+            left -= size;
+            cur ^= 1;
+            at = 0;
+        }
     }
-    int64_t blocks = 0, join = 0;
-    s.count = n;
+};
+
+// The next product of every matrix that has one left: one launch, and one more that joins slices where there are any.
+int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char* ws, int dtype, hipStream_t st) {
+    s.count = s.sliced = 0;
+    int64_t batch[NOPS];
     for (int k = 0; k < n; ++k) {
-        const gan_matrix& g = mats[k];
-        const Lay l = lay_of(g.rows, g.cols);
+        Walk& w = walks[k];
+        if (w.left) {
+            batch[s.count] = mats[k].batch;
+            Op& q = s.mat[s.count++];
+            q.ws = ws;
+            q.stride = w.l.bytes;
+            q.out = mats[k].out;
+            q.rows = (int)mats[k].rows;
+            q.cols = (int)mats[k].cols;
+            q.join = (unsigned)(w.l.join / 256);
+            w.next(q, steps);
+            q.steps = (int)ceil_div64(q.K / 32, q.cut);
+            s.sliced |= q.cut > 1;
+        }
+        ws += w.l.bytes * mats[k].batch;
+    }
+    // one tile size for the launch: the one that takes least, counted as if all its workgroups ran over the longest k
+    int T = 64;
+    double least = 1e30;
+    for (int t = 64; t <= 256; t *= 2) {
+        int64_t wgs = 0, longest = 0;
+        for (int k = 0; k < s.count; ++k) {
+            const Op& q = s.mat[k];
+            wgs += tiles_of(q.M, q.N, q.kind != RESULT && q.dn == q.dt, t) * q.cut * batch[k];
+            if (q.steps > longest) longest = q.steps;
+        }
+        const double c = cost_of(t, wgs, 1, longest);
+        if (c < least) {
+            least = c;
+            T = t;
+        }
+    }
+    int64_t blocks = 0;
+    for (int k = 0; k < s.count; ++k) {
         Op& q = s.mat[k];
-        q.ws = ws;
-        q.stride = l.bytes;
-        q.out = g.out;
-        q.rows = (int)g.rows;
-        q.cols = (int)g.cols;
-        q.kind = kind;
-        q.cur = cur;
-        q.tiles = (int)tiles_of(l, kind, T);
-        const int steps = (int)((kind == GRAM ? l.np : l.mp) / 32), cut = kind == GRAM ? splits_of(l.mp, l.np) : 1;
-        q.steps = (steps + cut - 1) / cut;
-        q.cut = (steps + q.steps - 1) / q.steps;
+        q.tiles = (int)tiles_of(q.M, q.N, q.kind != RESULT && q.dn == q.dt, T);
         q.first = (int)blocks;
-        blocks += (int64_t)q.tiles * q.cut * g.batch;
-        ws += l.bytes * g.batch;
+        blocks += (int64_t)q.tiles * q.cut * batch[k];
     }
-    if (int rc = T == 256   ? launch_gemm<256, 2>((unsigned)blocks, s, dtype, st)
-                 : T == 128 ? launch_gemm<128, 2>((unsigned)blocks, s, dtype, st)
-                            : launch_gemm<64, 4>((unsigned)blocks, s, dtype, st))
+    if (int rc = T == 256                  ? launch_gemm<256, 2>((unsigned)blocks, s, dtype, st)
+                 : T == 64                 ? launch_gemm<64, 4>((unsigned)blocks, s, dtype, st)
+                 : blocks > 256            ? launch_gemm<128, 2>((unsigned)blocks, s, dtype, st)  // two a CU
+                                           : launch_gemm<128, 4>((unsigned)blocks, s, dtype, st))
         return rc;
-    // the matrices whose products were cut
+    if (!s.sliced) return GAN_OK;
+    int64_t join = 0;
     int m = 0;
-    for (int k = 0; k < n; ++k) {
+    for (int k = 0; k < s.count; ++k) {
         if (s.mat[k].cut == 1) continue;
         s.mat[m] = s.mat[k];
-        s.mat[m++].first = (int)join;
-        join += (int64_t)s.mat[m - 1].tiles * mats[k].batch * (T * T / 4096);
+        s.mat[m].first = (int)join;
+        join += (int64_t)s.mat[m++].tiles * batch[k] * (T * T / 4096);
     }
-    if (!m) return GAN_OK;
     s.count = m;
     if (T == 256) hipLaunchKernelGGL((ortho_join_k<256>), dim3((unsigned)join), dim3(256), 0, st, s, dtype);
     else if (T == 128) hipLaunchKernelGGL((ortho_join_k<128>), dim3((unsigned)join), dim3(256), 0, st, s, dtype);
@@ -716,6 +834,8 @@ int pack(const gan_matrix* mats, int n, char* ws, Mats& s, hipStream_t st) {
         q.buf = g.buf;
         q.ws = ws;
         q.stride = l.bytes;
+        q.nat = g.rows <= g.cols ? l.xm[0] : l.xt[0];
+        q.tra = g.rows <= g.cols ? l.xt[0] : l.xm[0];
         q.rows = (int)g.rows;
         q.cols = (int)g.cols;
         ws += l.bytes * g.batch;
@@ -765,10 +885,12 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, Mats&
         if (!n) break;
         int rc = dtype == GAN_F32 ? pack<float>(some, n, at, s, st) : pack<bf16>(some, n, at, s, st);
         if (rc) return rc;
-        for (int k = 0; k < steps; ++k) {
-            if ((rc = products(some, n, GRAM, k & 1, o, at, dtype, st))) return rc;
-            if ((rc = products(some, n, POLY, k & 1, o, at, dtype, st))) return rc;
-            if ((rc = products(some, n, k + 1 < steps ? APPLY : RESULT, k & 1, o, at, dtype, st))) return rc;
+        Walk walks[NOPS];
+        for (int k = 0; k < n; ++k) walks[k] = Walk{lay_of(some[k].rows, some[k].cols), steps, 1, 0, 0};
+        for (bool more = true; more;) {
+            if ((rc = products(some, walks, n, steps, o, at, dtype, st))) return rc;
+            more = false;
+            for (int k = 0; k < n; ++k) more |= walks[k].left > 0;
         }
         at += used;
     }
