@@ -49,13 +49,16 @@ struct Mat {
     int first;       // first workgroup of this launch that works on the group
 };
 
+// momentum: u = mu buf + (1 - mu) g, buf before u; nesterov: u = mu buf + (1 - mu) g once more
+struct Source {
+    float mu, eps;
+    int nesterov;
+};
+
 struct Mats {
     Mat mat[NOPS];
     int count;
-    // momentum: u = mu buf + (1 - mu) g, buf before u; nesterov: u = mu buf + (1 - mu) g once more
-    float mu;
-    int nesterov;
-    float eps;
+    Source from;
 };
 
 // Byte offsets in one matrix's workspace: the partial sums, two X (each [m][n] and [n][m], hi plane then lo plane), five
@@ -139,7 +142,7 @@ __device__ __forceinline__ int group_of(const S& s, int id) {
 }
 
 // what is orthogonalised, of gradient g and momentum m
-__device__ __forceinline__ float update_of(const Mats& s, float g, float m) { return s.nesterov ? fmaf(s.mu, m, (1.f - s.mu) * g) : m; }
+__device__ __forceinline__ float update_of(const Source& s, float g, float m) { return s.nesterov ? fmaf(s.mu, m, (1.f - s.mu) * g) : m; }
 
 // ---- momentum and the partial sums of squares (doubles: no square of a finite fp32 leaves their range) ------------------
 template <typename T>
@@ -171,8 +174,8 @@ __global__ void __launch_bounds__(256) ortho_norm_k(const Mats s) {
         if (buf) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                m[e] = fmaf(s.mu, m[e], (1.f - s.mu) * v[e]);
-                v[e] = update_of(s, v[e], m[e]);
+                m[e] = fmaf(s.from.mu, m[e], (1.f - s.from.mu) * v[e]);
+                v[e] = update_of(s.from, v[e], m[e]);
             }
             if (i + 4 <= end) {
                 __builtin_memcpy(buf + i, m, sizeof(m));
@@ -227,12 +230,12 @@ __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
         if (buf) m[k] = buf[at];
         if (!in) v[k] = m[k] = 0.f;
     }
-    const float scale = scale_of((const double*)ws, (int)parts_of(size), s.eps);
+    const float scale = scale_of((const double*)ws, (int)parts_of(size), s.from.eps);
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
         const int r = k * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
         const bool in = r0 + r < q.rows && c0 + c < q.cols;
-        tile[r][c] = in ? scale * (buf ? update_of(s, v[k], m[k]) : v[k]) : 0.f;
+        tile[r][c] = in ? scale * (buf ? update_of(s.from, v[k], m[k]) : v[k]) : 0.f;
     }
     __syncthreads();
     h16 *nat = (h16*)(ws + q.nat), *tra = (h16*)(ws + q.tra);
@@ -276,16 +279,21 @@ struct Op {
     float gain;        // SCALED: result = gain * accumulator
 };
 
-struct Ops {
-    Op mat[NOPS];
-    int count;
+// the polynomial, and what becomes of the result
+struct Rule {
     float a, b, c;
-    int sliced;         // some product of the launch is cut
     float decay, step;  // RESULT onto parameters: p = decay p - step_of(rows, cols) X
     int update;         // 0: out = X; 1: the parameters; 2, 3: the step scaled by the shape, see step_of
 };
 
-__device__ __forceinline__ float step_of(const Ops& s, int rows, int cols) {
+struct Ops {
+    Op mat[NOPS];
+    int count;
+    int sliced;  // some product of the launch is cut
+    Rule rule;
+};
+
+__device__ __forceinline__ float step_of(const Rule& s, int rows, int cols) {
     const float r = (float)rows, c = (float)cols;
     return s.update == 2 ? s.step * sqrtf(fmaxf(1.f, r / c)) : s.update == 3 ? s.step * 0.2f * sqrtf(fmaxf(r, c)) : s.step;
 }
@@ -314,7 +322,7 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int 
     if (q.kind == RESULT) {
         // eight consecutive elements of a row of the result a lane; a tall result is the transpose of the block
         const bool wide = q.rows <= q.cols;
-        const float step = s.update ? step_of(s, q.rows, q.cols) : 0.f;
+        const float step = s.rule.update ? step_of(s.rule, q.rows, q.cols) : 0.f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int a = h * 16 + (lane >> 2), c = (lane & 3) * 8;
@@ -324,17 +332,17 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int 
             const int row = (wide ? i0 : j0) + a, col = (wide ? j0 : i0) + c;
             const int left = row < q.rows ? q.cols - col : 0;
             const int64_t at = ((int64_t)b * q.rows + row) * q.cols + col;
-            if (s.update) {
+            if (s.rule.update) {
                 float* p = (float*)q.out + at;
                 float old[8];
                 if (left >= 8) {
                     __builtin_memcpy(old, p, 32);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] = fmaf(-step, o[e], s.decay * old[e]);
+                    for (int e = 0; e < 8; ++e) o[e] = fmaf(-step, o[e], s.rule.decay * old[e]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (e < left) o[e] = fmaf(-step, o[e], s.decay * p[e]);
+                        if (e < left) o[e] = fmaf(-step, o[e], s.rule.decay * p[e]);
                 }
             }
             if (dtype == GAN_F32) {
@@ -364,7 +372,7 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int 
     }
     h16 *dn = (h16*)(ws + (int64_t)q.dn * 256), *dt = (h16*)(ws + (int64_t)q.dt * 256);  // [i][j] and [j][i]
     const int64_t plane = (int64_t)q.M * q.N;
-    const float gain = q.kind == SCALED ? q.gain : s.c * (SP / (SA * SA));
+    const float gain = q.kind == SCALED ? q.gain : s.rule.c * (SP / (SA * SA));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int a = h * 16 + (lane >> 2), c = (lane & 3) * 8, i = i0 + a, j = j0 + c;
@@ -377,7 +385,7 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float o = t[a * TLD + c + e] * gain;
-            if (q.kind == POLY) o += s.b * (((float)ah[e] + (float)al[e]) * (SP / SA)) + (i == j + e ? s.a * SP : 0.f);
+            if (q.kind == POLY) o += s.rule.b * (((float)ah[e] + (float)al[e]) * (SP / SA)) + (i == j + e ? s.rule.a * SP : 0.f);
             if (mirror) t[a * TLD + c + e] = o;
             h16 p, w;
             split(o, p, w);
@@ -777,6 +785,255 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
     return GAN_OK;
 }
 
+// ---- matrices that fit into LDS: one workgroup of sixteen waves each does everything, in one launch ---------------------------
+// Of X two copies are wanted, [m][n] for A = X X' and [n][m] for P X; the first one's place holds A and then P in between.  A
+// product's results wait in registers (two 32 x 32 blocks a wave) until everyone has read the operands that they replace.
+// Rows are 8 elements longer than they are, which spreads any sixteen of them over the banks.  The launches of the general
+// path cost about 5 us each, seventeen of them for five steps; a product of 128 x 128 matrices takes 2 us here.
+constexpr int SMALL_LDS = 160 * 1024 - 512;
+constexpr int SMALL_ELEMS = 20;  // source elements a thread
+
+struct SmallMat {
+    const void* g;
+    float* buf;
+    void* out;
+    int rows, cols, first;
+};
+struct Smalls {
+    SmallMat mat[NOPS];
+    int count, steps;
+};
+
+__host__ __device__ inline int up32(int v) { return (v + 31) & ~31; }
+
+bool is_small(const gan_matrix& g) {
+    const int64_t m = g.rows < g.cols ? g.rows : g.cols, n = g.rows < g.cols ? g.cols : g.rows;
+    if (n > 4096) return false;
+    const int64_t mp = up32((int)m), np = up32((int)n);
+    return (mp * (np + 8) + np * (mp + 8)) * 4 <= SMALL_LDS && g.rows * g.cols <= SMALL_ELEMS * 1024 && mp * np <= 32 * 1024;
+}
+
+// blocks wave, wave + 16 of a bm x bn grid of 32 x 32 blocks: acc += U V' over k, rows of U and V `lu` and `lv` elements long
+__device__ __forceinline__ void small_product(f32x16 (&acc)[2], const h16* u, int lu, int pu, const h16* v, int lv, int pv, int bm, int bn, int k) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+        const int blk = wave + 16 * z;
+        if (blk >= bm * bn) break;
+        const int bi = blk % bm, bj = blk / bm;
+        const h16 *pu_ = u + (bi * 32 + (lane & 31)) * lu + (lane >> 5) * 8, *pv_ = v + (bj * 32 + (lane & 31)) * lv + (lane >> 5) * 8;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[z][r] = 0.f;
+        for (int kk = 0; kk < k; kk += 16) {
+            const h16x8 uh = *(const h16x8*)(pu_ + kk), ul = *(const h16x8*)(pu_ + pu + kk);
+            const h16x8 vh = *(const h16x8*)(pv_ + kk), vl = *(const h16x8*)(pv_ + pv + kk);
+            acc[z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, vl, acc[z], 0, 0, 0);
+            acc[z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul, vh, acc[z], 0, 0, 0);
+            acc[z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, vh, acc[z], 0, 0, 0);
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) ortho_small_k(const Smalls s, const Source h, const Rule o) {
+    extern __shared__ __attribute__((aligned(1024))) char lds[];
+    __shared__ double red[16];
+    const SmallMat& q = s.mat[group_of(s, blockIdx.x)];
+    const int rows = q.rows, cols = q.cols, size = rows * cols;
+    const int64_t b = (int)blockIdx.x - q.first;
+    const bool wide = rows <= cols;
+    const int mp = up32(wide ? rows : cols), np = up32(wide ? cols : rows), lm = np + 8, lt = mp + 8, la = mp + 8;
+    const int pm = mp * lm, pt = np * lt, pa = mp * la;  // from hi to lo plane
+    h16 *xm = (h16*)lds, *xt = xm + 2 * pm, *sq = xm;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // ---- source: momentum, norm, planes
+    const T* g = (const T*)q.g + b * size;
+    float* buf = q.buf ? q.buf + b * size : nullptr;
+    float val[SMALL_ELEMS];
+#pragma unroll
+    for (int k = 0; k < SMALL_ELEMS; ++k) {
+        const int i = k * 1024 + tid;
+        val[k] = i < size ? (float)g[i] : 0.f;
+    }
+    if (buf) {
+        float m[SMALL_ELEMS];
+#pragma unroll
+        for (int k = 0; k < SMALL_ELEMS; ++k) {
+            const int i = k * 1024 + tid;
+            m[k] = i < size ? buf[i] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < SMALL_ELEMS; ++k) {
+            const int i = k * 1024 + tid;
+            m[k] = fmaf(h.mu, m[k], (1.f - h.mu) * val[k]);
+            val[k] = update_of(h, val[k], m[k]);
+            if (i < size) buf[i] = m[k];
+        }
+    }
+    for (int i = tid; i < (2 * pm + 2 * pt) / 8; i += 1024) ((uint4*)lds)[i] = make_uint4(0u, 0u, 0u, 0u);
+    double sum = 0.;
+#pragma unroll
+    for (int k = 0; k < SMALL_ELEMS; ++k) sum += (double)val[k] * (double)val[k];
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    sum = 0.;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) sum += red[w];
+    const double n = sqrt(sum);
+    const float scale = n < 1e300 ? (float)((double)SX / (n > (double)h.eps ? n : (double)h.eps)) : __builtin_nanf("");
+#pragma unroll
+    for (int k = 0; k < SMALL_ELEMS; ++k) {
+        const int e = k * 1024 + tid;
+        if (e < size) {
+            const int r = e / cols, c = e - r * cols, i = wide ? r : c, j = wide ? c : r;
+            h16 hi, lo;
+            split(val[k] * scale, hi, lo);
+            xm[i * lm + j] = xt[j * lt + i] = hi;
+            xm[pm + i * lm + j] = xt[pt + j * lt + i] = lo;
+        }
+    }
+    __syncthreads();
+    // ---- iterations; lane holds column lane & 31, rows 8 r + 4 (lane >> 5) ... + 3 of a block
+    const int bm = mp / 32, bn = np / 32;
+    f32x16 acc[2];
+    for (int step = 0; step < s.steps; ++step) {
+        small_product(acc, xm, lm, pm, xm, lm, pm, bm, bm, np);
+        __syncthreads();
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const int blk = wave + 16 * z;
+            if (blk >= bm * bm) break;
+            h16* to = sq + (blk / bm * 32 + (lane & 31)) * la + blk % bm * 32 + 4 * (lane >> 5);  // (symmetric: stored transposed)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                h16x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    h16 x, y;
+                    split(acc[z][r * 4 + e] * (SA / (SX * SX)), x, y);
+                    hi[e] = x;
+                    lo[e] = y;
+                }
+                *(h16x4*)(to + 8 * r) = hi;
+                *(h16x4*)(to + pa + 8 * r) = lo;
+            }
+        }
+        __syncthreads();
+        small_product(acc, sq, la, pa, sq, la, pa, bm, bm, mp);
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const int blk = wave + 16 * z;
+            if (blk >= bm * bm) break;
+            const int i0 = blk % bm * 32 + 4 * (lane >> 5), j = blk / bm * 32 + (lane & 31);
+            const h16* from = sq + j * la + i0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const h16x4 ah = *(const h16x4*)(from + 8 * r), al = *(const h16x4*)(from + pa + 8 * r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[z][r * 4 + e] = acc[z][r * 4 + e] * (o.c * (SP / (SA * SA))) + o.b * (((float)ah[e] + (float)al[e]) * (SP / SA)) +
+                                        (i0 + 8 * r + e == j ? o.a * SP : 0.f);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const int blk = wave + 16 * z;
+            if (blk >= bm * bm) break;
+            h16* to = sq + (blk / bm * 32 + (lane & 31)) * la + blk % bm * 32 + 4 * (lane >> 5);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                h16x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    h16 x, y;
+                    split(acc[z][r * 4 + e], x, y);
+                    hi[e] = x;
+                    lo[e] = y;
+                }
+                *(h16x4*)(to + 8 * r) = hi;
+                *(h16x4*)(to + pa + 8 * r) = lo;
+            }
+        }
+        __syncthreads();
+        small_product(acc, sq, la, pa, xt, lt, pt, bm, bn, mp);
+        if (step + 1 == s.steps) break;
+        __syncthreads();
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const int blk = wave + 16 * z;
+            if (blk >= bm * bn) break;
+            const int i0 = blk % bm * 32 + 4 * (lane >> 5), j = blk / bm * 32 + (lane & 31);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                h16x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    h16 x, y;
+                    split(acc[z][r * 4 + e] * (1.f / SP), x, y);
+                    hi[e] = x;
+                    lo[e] = y;
+                    xm[(i0 + 8 * r + e) * lm + j] = x;
+                    xm[pm + (i0 + 8 * r + e) * lm + j] = y;
+                }
+                *(h16x4*)(xt + j * lt + i0 + 8 * r) = hi;
+                *(h16x4*)(xt + pt + j * lt + i0 + 8 * r) = lo;
+            }
+        }
+        __syncthreads();
+    }
+    const float shaped = o.update ? step_of(o, rows, cols) : 0.f;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+        const int blk = wave + 16 * z;
+        if (blk >= bm * bn) break;
+        const int i0 = blk % bm * 32 + 4 * (lane >> 5), j = blk / bm * 32 + (lane & 31);
+        float old[16];
+        if (o.update) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int i = i0 + 8 * (r >> 2) + (r & 3), row = wide ? i : j, col = wide ? j : i;
+                old[r] = row < rows && col < cols ? ((const float*)q.out)[b * size + row * cols + col] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = i0 + 8 * (r >> 2) + (r & 3), row = wide ? i : j, col = wide ? j : i;
+            if (row < rows && col < cols) {
+                const float x = acc[z][r] * (1.f / (SP * SX));
+                const int64_t at = b * size + row * cols + col;
+                if (o.update) ((float*)q.out)[at] = fmaf(-shaped, x, o.decay * old[r]);
+                else ((T*)q.out)[at] = (T)x;
+            }
+        }
+    }
+}
+
+template <typename T>
+int run_small(const gan_matrix* mats, int n, int steps, const Source& h, const Rule& o, hipStream_t st) {
+    Smalls s;
+    int lds = 0, blocks = 0;
+    s.count = n;
+    s.steps = steps;
+    for (int k = 0; k < n; ++k) {
+        const gan_matrix& g = mats[k];
+        s.mat[k] = SmallMat{g.g, g.buf, g.out, (int)g.rows, (int)g.cols, blocks};
+        blocks += (int)g.batch;
+        const int m = up32((int)(g.rows < g.cols ? g.rows : g.cols)), w = up32((int)(g.rows < g.cols ? g.cols : g.rows));
+        const int need = (m * (w + 8) + w * (m + 8)) * 4;
+        lds = need > lds ? need : lds;
+    }
+    // more than 64 KB of dynamic LDS needs the attribute (set on every call: it is per device, and cheap)
+    if (lds > 64 * 1024 && hipFuncSetAttribute((const void*)ortho_small_k<T>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+        gan_set_error("orthogonalize: cannot reserve %d bytes of LDS", lds);
+        return GAN_ERR_LAUNCH;
+    }
+    hipLaunchKernelGGL((ortho_small_k<T>), dim3((unsigned)blocks), dim3(1024), lds, st, s, h, o);
+    GAN_CHECK_LAUNCH("orthogonalize(small)");
+    return GAN_OK;
+}
+
 // The largest factor that a singular value can have grown to after each step, from 1: extremes of x |a + b x^2 + c x^4| on [0, r].
 bool bounded(int steps, float a, float b, float c) {
     double r = 1.0;
@@ -809,6 +1066,7 @@ bool bounded(int steps, float a, float b, float c) {
 
 int64_t total_bytes(const gan_matrix* mats, int count) {
     int64_t n = 0;
+    bool small = true;
     for (int k = 0; k < count; ++k) {
         const gan_matrix& g = mats[k];
         if (g.rows < 1 || g.cols < 1 || g.batch < 0 || g.rows > (1 << 20) || g.cols > (1 << 20) || g.batch > (1 << 30)) return -1;
@@ -817,8 +1075,9 @@ int64_t total_bytes(const gan_matrix* mats, int count) {
         if (g.batch && one > (1LL << 60) / g.batch) return -1;
         n += one * g.batch;
         if (n > (1LL << 60)) return -1;
+        small = small && is_small(g);
     }
-    return n;
+    return small ? 0 : n;  // (all of them in LDS)
 }
 
 // The two launches in front of the products: momentum and norms, planes.
@@ -852,12 +1111,19 @@ int pack(const gan_matrix* mats, int n, char* ws, Mats& s, hipStream_t st) {
     return GAN_OK;
 }
 
-int run_all(const char* what, const gan_matrix* all, int count, int steps, Mats& s, Ops& o, int dtype, char* ws, int64_t bytes, hipStream_t st) {
+bool all_small(const gan_matrix* mats, int count) {
+    for (int k = 0; k < count; ++k)
+        if (!is_small(mats[k])) return false;
+    return true;
+}
+
+int run_all(const char* what, const gan_matrix* all, int count, int steps, const Source& source, const Rule& rule, int dtype, char* ws, int64_t bytes,
+            hipStream_t st) {
     GAN_CHECK_ARG(count >= 0 && (count == 0 || all), "%s: null list", what);
     GAN_CHECK_ARG(steps >= 1 && steps <= 100, "%s: 1 to 100 steps, got %d", what, steps);
-    GAN_CHECK_ARG(s.eps > 0.f && s.eps < 1e30f, "%s: eps must be positive, got %g", what, (double)s.eps);
-    GAN_CHECK_ARG(bounded(steps, o.a, o.b, o.c), "%s: with coefficients %g %g %g a singular value can grow beyond 3.5", what, (double)o.a,
-                  (double)o.b, (double)o.c);
+    GAN_CHECK_ARG(source.eps > 0.f && source.eps < 1e30f, "%s: eps must be positive, got %g", what, (double)source.eps);
+    GAN_CHECK_ARG(bounded(steps, rule.a, rule.b, rule.c), "%s: with coefficients %g %g %g a singular value can grow beyond 3.5", what, (double)rule.a,
+                  (double)rule.b, (double)rule.c);
     const int64_t need = total_bytes(all, count);
     GAN_CHECK_ARG(need >= 0, "%s: a matrix has a size that is not supported (1 to 2^20 either way, the smaller at most 32768)", what);
     GAN_CHECK_ARG(need == 0 || (ws && bytes >= need), "%s: workspace of %lld bytes wanted, %lld given", what, (long long)need,
@@ -865,12 +1131,17 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, Mats&
     GAN_CHECK_ARG(((uintptr_t)ws % 256) == 0, "%s: workspace must be 256-byte aligned", what);
     for (int k = 0; k < count; ++k) {
         const gan_matrix& g = all[k];
-        GAN_CHECK_ARG(!g.batch || (g.g && g.out && (!o.update || g.buf)), "%s: null pointer", what);
+        GAN_CHECK_ARG(!g.batch || (g.g && g.out && (!rule.update || g.buf)), "%s: null pointer", what);
         const Lay l = lay_of(g.rows, g.cols);
         const int64_t tiles = l.mp / 64 * (l.np / 64) + 4096;  // (slices stay below that)
         GAN_CHECK_ARG(g.batch <= MAXGRID / NOPS / (tiles > l.nparts ? tiles : l.nparts), "%s: %lld matrices of %lld x %lld are too many for one call",
                       what, (long long)g.batch, (long long)g.rows, (long long)g.cols);
     }
+    const bool small = all_small(all, count);
+    Mats s = {};
+    Ops o = {};
+    s.from = source;
+    o.rule = rule;
     gan_matrix some[NOPS];
     char* at = ws;
     for (int from = 0; from < count;) {
@@ -880,9 +1151,13 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, Mats&
             const gan_matrix& g = all[from++];
             if (!g.batch) continue;
             some[n++] = g;
-            used += lay_of(g.rows, g.cols).bytes * g.batch;
+            if (!small) used += lay_of(g.rows, g.cols).bytes * g.batch;
         }
         if (!n) break;
+        if (small) {
+            if (int rc = dtype == GAN_F32 ? run_small<float>(some, n, steps, source, rule, st) : run_small<bf16>(some, n, steps, source, rule, st)) return rc;
+            continue;
+        }
         int rc = dtype == GAN_F32 ? pack<float>(some, n, at, s, st) : pack<bf16>(some, n, at, s, st);
         if (rc) return rc;
         Walk walks[NOPS];
@@ -908,13 +1183,7 @@ extern "C" int gan_orthogonalize(const gan_matrix* mats, int count, int steps, f
                                  int64_t ws_bytes, gan_stream_t stream) {
     GAN_CHECK_ARG(dtype == GAN_F32 || dtype == GAN_BF16, "orthogonalize: bad dtype %d", dtype);
     for (int k = 0; mats && k < count; ++k) GAN_CHECK_ARG(!mats[k].buf, "orthogonalize: matrix %d has a momentum buffer", k);
-    Mats s = {};
-    Ops o = {};
-    s.eps = eps;
-    o.a = a;
-    o.b = b;
-    o.c = c;
-    return run_all("orthogonalize", mats, count, steps, s, o, dtype, (char*)ws, ws_bytes, (hipStream_t)stream);
+    return run_all("orthogonalize", mats, count, steps, Source{0.f, eps, 0}, Rule{a, b, c, 1.f, 0.f, 0}, dtype, (char*)ws, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int gan_muon_step(const gan_matrix* mats, int count, float lr, float momentum, int nesterov, float weight_decay, int scaling, int steps,
@@ -922,16 +1191,6 @@ extern "C" int gan_muon_step(const gan_matrix* mats, int count, float lr, float 
     GAN_CHECK_ARG(lr >= 0.f && momentum >= 0.f && momentum < 1.f && weight_decay >= 0.f,
                   "muon_step: bad hyper-parameters (lr %g, momentum %g, weight_decay %g)", (double)lr, (double)momentum, (double)weight_decay);
     GAN_CHECK_ARG(scaling >= 0 && scaling <= 2, "muon_step: bad scaling %d", scaling);
-    Mats s = {};
-    Ops o = {};
-    s.eps = eps;
-    s.mu = momentum;
-    s.nesterov = nesterov;
-    o.a = a;
-    o.b = b;
-    o.c = c;
-    o.update = 1 + scaling;
-    o.decay = 1.f - lr * weight_decay;
-    o.step = lr;
-    return run_all("muon_step", mats, count, steps, s, o, GAN_F32, (char*)ws, ws_bytes, (hipStream_t)stream);
+    return run_all("muon_step", mats, count, steps, Source{momentum, eps, nesterov}, Rule{a, b, c, 1.f - lr * weight_decay, lr, 1 + scaling}, GAN_F32,
+                   (char*)ws, ws_bytes, (hipStream_t)stream);
 }

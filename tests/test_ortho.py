@@ -235,7 +235,9 @@ def test_refusals():
     def run(m, steps=5, coeffs=COEFFS, eps=1e-7, dtype=0, ws=p, nbytes=1 << 40):
         return lib.gan_orthogonalize(ctypes.addressof(m), len(m), steps, *coeffs, eps, dtype, ws, nbytes, None)
 
-    ok = mats((p, None, p, 4, 8, 1))
+    ok = mats((p, None, p, 300, 256, 1))
+    tiny = mats((p, None, p, 4, 8, 1))  # fits into LDS: no workspace
+    assert lib.gan_orthogonalize_workspace(ctypes.addressof(tiny), 1) == 0 and run(tiny, steps=0) != 0 and run(tiny, eps=0.0) != 0
     need = lib.gan_orthogonalize_workspace(ctypes.addressof(ok), 1)
     assert need > 0
     assert run(ok, steps=0) != 0 and run(ok, steps=101) != 0
@@ -250,7 +252,7 @@ def test_refusals():
         assert lib.gan_orthogonalize_workspace(ctypes.addressof(bad), 1) < 0 and run(bad) != 0
     assert run(mats((p, None, p, 4, 8, 0))) == 0  # nothing to do
     assert lib.gan_orthogonalize(None, 1, 5, *COEFFS, 1e-7, 0, p, 1 << 40, None) != 0
-    step = mats((p, p, p, 4, 8, 1))
+    step = mats((p, p, p, 300, 256, 1))
 
     def muon(m, lr=0.1, mu=0.9, wd=0.0, scaling=1):
         return lib.gan_muon_step(ctypes.addressof(m), len(m), lr, mu, 1, wd, scaling, 5, *COEFFS, 1e-7, p, need - 1, None)
