@@ -2592,17 +2592,28 @@ def _layer_norm_ws(rows: int, d: int, code: int, order: int, columns: bool) -> i
     return n
 
 
+def _launch(family: str, tensors, tag, fn, *args) -> None:
+    """A call of the library on tensors[0]'s device and stream, measured where a profile is set.  (Called without a profile some
+    hundred times per iteration from the engine's threads: no closures.)"""
+    t = tensors[0]
+    with on_device(t):
+        if _PROFILE is None:
+            status = fn(*args, stream_of(t))
+        else:
+            status = _PROFILE.launch(family, 0, _nbytes(*tensors), lambda: fn(*args, stream_of(t)), tag)
+    if status:
+        check(status, fn.__name__)
+
+
 def raw_layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], d: int, eps: float):
     """(y, stats (rows, 2)) of contiguous x, normalised over its last d elements."""
-    y = torch.empty_like(x)
     rows, code = x.numel() // d, dtype_code(x)
+    y = torch.empty_like(x)
     n = _layer_norm_ws(rows, d, code, 0, False)
     stats = x.new_empty((rows, 2), dtype=torch.float32)
     ws = x.new_empty((n,), dtype=torch.float32) if n else None
-    with on_device(x):
-        check(_run("layernorm", 0, _nbytes(x, y),
-                   lambda: _lib.load().gan_layernorm_fwd(ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(stats), rows, d, eps, code, ptr(ws), n,
-                                                         stream_of(x)), (rows, d)), "gan_layernorm_fwd")
+    _launch("layernorm", (x, y), (rows, d), _lib.load().gan_layernorm_fwd, ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(stats), rows, d, eps, code,
+            ptr(ws), n)
     return y, stats
 
 
@@ -2615,10 +2626,8 @@ def raw_layer_norm_bwd(g: Tensor, x: Tensor, weight: Optional[Tensor], stats: Te
     gwb = x.new_empty((2, d), dtype=torch.float32) if need_cols else None
     n = _layer_norm_ws(rows, d, code, 1, need_cols)
     ws = x.new_empty((n,), dtype=torch.float32) if n else None
-    with on_device(x):
-        check(_run("layernorm_bwd", 0, _nbytes(g, x, gx),
-                   lambda: _lib.load().gan_layernorm_bwd(ptr(g), ptr(x), ptr(weight), ptr(stats), ptr(gx), ptr(gwb), rows, d, code, ptr(ws), n,
-                                                         stream_of(x)), (rows, d)), "gan_layernorm_bwd")
+    _launch("layernorm_bwd", (x, g, gx), (rows, d), _lib.load().gan_layernorm_bwd, ptr(g), ptr(x), ptr(weight), ptr(stats), ptr(gx), ptr(gwb), rows, d,
+            code, ptr(ws), n)
     return gx, gwb
 
 
@@ -2633,58 +2642,82 @@ def raw_layer_norm_bwd2(v: Tensor, cw: Optional[Tensor], cb: Optional[Tensor], g
     gww = x.new_empty((d,), dtype=torch.float32) if need_w else None
     n = _layer_norm_ws(rows, d, code, 2, need_w)
     ws = x.new_empty((n,), dtype=torch.float32) if n else None
-    with on_device(x):
-        check(_run("layernorm_bwd2", 0, _nbytes(v, g, x, gg, gxx),
-                   lambda: _lib.load().gan_layernorm_bwd2(ptr(v), ptr(cw), ptr(cb), ptr(g), ptr(x), ptr(weight), ptr(stats), ptr(gg), ptr(gxx),
-                                                          ptr(gww), rows, d, code, ptr(ws), n, stream_of(x)), (rows, d)), "gan_layernorm_bwd2")
+    _launch("layernorm_bwd2", (x, v, g, gg, gxx), (rows, d), _lib.load().gan_layernorm_bwd2, ptr(v), ptr(cw), ptr(cb), ptr(g), ptr(x), ptr(weight),
+            ptr(stats), ptr(gg), ptr(gxx), ptr(gww), rows, d, code, ptr(ws), n)
     return gg, gxx, gww
 
 
-def _not_a_leaf(t: Optional[Tensor]) -> Optional[Tensor]:
-    """t itself, or a view of it where it is a leaf that takes gradients.  Whether torch.autograd.grad() wants a leaf can only
-    be asked by way of an exception (_need), and raising one costs 15 us, six times what the view does."""
-    return t.view_as(t) if t is not None and t.requires_grad and t.is_leaf else t
+def _plain_f32(t: Optional[Tensor]) -> Optional[Tensor]:
+    """What the kernels read of a parameter: t itself where it is dense fp32, else a copy."""
+    return t if t is None or (t.dtype == torch.float32 and t.is_contiguous()) else _f32(t)
 
 
-class LayerNormFn(Function):
+def _shaped(g: Tensor, shape, dtype) -> Tensor:
+    """A (d,) fp32 gradient as its parameter is."""
+    g = g if len(shape) == 1 else g.view(shape)
+    return g if dtype == torch.float32 else g.to(dtype)
+
+
+def _wanted(ctx, edge: int) -> bool:
+    """Will the engine run what takes the gradient of the `edge`-th tensor argument (see _need)?  Asked of parameters only, which
+    `layer_norm` hands over as views: whether torch.autograd.grad() wants a leaf can only be asked by way of an exception,
+    and raising one costs 15 us, three times what the view does."""
+    if not _PRUNE_UNWANTED:
+        return True
+    fn = ctx.next_functions[edge][0]
+    if fn is None:
+        return False
+    try:
+        return bool(torch._C._will_engine_execute_node(fn))
+    except RuntimeError:  # a leaf that autograd.grad() was asked for
+        return True
+
+
+class LayerNormFn(_TorchFunction):
     """y = (x - mean) * rstd * weight + bias over the last d elements of contiguous x, one launch; the first and the second
     derivative are kernels too (a gradient penalty through a normalised critic, losses.py:89-103)."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, d, eps):
-        w32 = _f32(weight)
-        y, stats = raw_layer_norm(x.detach(), w32, _f32(bias), d, eps)
-        ctx.save_for_backward(x, weight, w32, stats)
+        y, stats = raw_layer_norm(x, _plain_f32(weight), _plain_f32(bias), d, eps)
+        ctx.save_for_backward(x, weight, stats)
         ctx.d = d
         ctx.bias_like = None if bias is None else (bias.shape, bias.dtype)
         return y
 
     @staticmethod
     def backward(ctx, g):
-        x, weight, w32, stats = ctx.saved_tensors
-        cols = _need(ctx, 1)  # the bias's gradient comes with the weight's: one question to the engine for both
-        need = _need(ctx, 0), cols, ctx.needs_input_grad[2] if cols else _need(ctx, 2)
+        x, weight, stats = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        # Under torch.autograd.grad(out, x, create_graph=True), a penalty's first pass, the parameters' sums would be thrown away.
+        # (The bias's comes with the weight's: one question to the engine for both.)
+        if need_w:
+            need_w = need_b = _wanted(ctx, 1)
+            need_b = need_b and ctx.needs_input_grad[2]
+        elif need_b:
+            need_b = _wanted(ctx, 1 if weight is None else 2)
         if torch.is_grad_enabled():
-            gx, gw, gb = LayerNormBwdFn.apply(_not_a_leaf(g), x, weight, w32, stats, ctx.d, need)
+            if g.is_leaf and g.requires_grad:
+                g = g.view_as(g)  # (see _wanted)
+            gx, gw, gb = LayerNormBwdFn.apply(g, x, weight, stats, ctx.d, (need_x, need_w, need_b))
         else:
-            gx, gwb = raw_layer_norm_bwd(g.to(x.dtype).contiguous(), x, w32, stats, ctx.d, need[0], need[1] or need[2])
+            gx, gwb = raw_layer_norm_bwd(g if g.dtype == x.dtype and g.is_contiguous() else g.to(x.dtype).contiguous(), x, _plain_f32(weight), stats,
+                                         ctx.d, need_x, need_w or need_b)
             gw, gb = (None, None) if gwb is None else gwb.unbind(0)
-        if need[1]:
-            gw = gw.view(weight.shape).to(weight.dtype)
-        if need[2]:
-            gb = gb.view(ctx.bias_like[0]).to(ctx.bias_like[1])
-        return gx, (gw if need[1] else None), (gb if need[2] else None), None, None
+        gw = _shaped(gw, weight.shape, weight.dtype) if need_w else None
+        gb = _shaped(gb, *ctx.bias_like) if need_b else None
+        return gx, gw, gb, None, None
 
 
-class LayerNormBwdFn(Function):
+class LayerNormBwdFn(_TorchFunction):
     """(g, x, weight) -> the three gradients of LayerNormFn (None where `need` says so) inside a create_graph region; its own
     backward is one more kernel.  Differentiating that one again is refused."""
 
     @staticmethod
-    def forward(ctx, g, x, weight, w32, stats, d, need):
-        gc = g.detach().to(x.dtype).contiguous()
-        gx, gwb = raw_layer_norm_bwd(gc, x.detach(), w32, stats, d, need[0], need[1] or need[2])
-        ctx.save_for_backward(gc, x, weight, w32, stats)
+    def forward(ctx, g, x, weight, stats, d, need):
+        gc = g if g.dtype == x.dtype and g.is_contiguous() else g.to(x.dtype).contiguous()
+        gx, gwb = raw_layer_norm_bwd(gc, x, _plain_f32(weight), stats, d, need[0], need[1] or need[2])
+        ctx.save_for_backward(gc, x, weight, stats)
         ctx.d, ctx.g_dtype = d, g.dtype
         ctx.set_materialize_grads(False)
         return gx, (gwb[0] if need[1] else None), (gwb[1] if need[2] else None)
@@ -2692,13 +2725,19 @@ class LayerNormBwdFn(Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, v, cw, cb):
-        gc, x, weight, w32, stats = ctx.saved_tensors
+        gc, x, weight, stats = ctx.saved_tensors
         if v is None and cw is None and cb is None:
-            return (None,) * 7
-        vc = torch.zeros_like(gc) if v is None else v.to(gc.dtype).contiguous()
-        gg, gxx, gww = raw_layer_norm_bwd2(vc, _f32(cw), _f32(cb), gc, x, w32, stats, ctx.d, _need(ctx, 0), _need(ctx, 1),
-                                           weight is not None and _need(ctx, 2))
-        return (None if gg is None else gg.to(ctx.g_dtype)), gxx, (None if gww is None else gww.view(weight.shape).to(weight.dtype)), None, None, None, None
+            return None, None, None, None, None, None
+        if v is None:
+            v = torch.zeros_like(gc)
+        elif v.dtype != gc.dtype or not v.is_contiguous():
+            v = v.to(gc.dtype).contiguous()
+        need = ctx.needs_input_grad
+        gg, gxx, gww = raw_layer_norm_bwd2(v, _plain_f32(cw), _plain_f32(cb), gc, x, _plain_f32(weight), stats, ctx.d, need[0], need[1],
+                                           need[2] and _wanted(ctx, 2))
+        if gg is not None and gg.dtype != ctx.g_dtype:
+            gg = gg.to(ctx.g_dtype)
+        return gg, gxx, (None if gww is None else _shaped(gww, weight.shape, weight.dtype)), None, None, None
 
 
 def layer_norm(x: Tensor, normalized_shape, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
@@ -2708,32 +2747,36 @@ def layer_norm(x: Tensor, normalized_shape, weight: Optional[Tensor] = None, bia
     mean and 1 / deviation.  A channels-last (N, C, H, W) tensor normalised over whole samples (C, H, W) is read and
     written as it lies; any other layout is made contiguous first."""
     shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
-    d = math.prod(shape)
     if not shape or min(shape) <= 0:
         raise _lib.GanAmdError(f"layer_norm: normalized_shape must be positive sizes, got {shape}")
     if x.shape[-len(shape):] != shape:
         raise _lib.GanAmdError(f"layer_norm: the trailing sizes of {tuple(x.shape)} are not normalized_shape {shape}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if t.shape != shape:
-            raise _lib.GanAmdError(f"layer_norm: {name} has shape {tuple(t.shape)}, normalized_shape is {shape}")
-        if not t.is_floating_point():
-            raise _lib.GanAmdError(f"layer_norm: {name} must be floating point, got {t.dtype}")
-        if t.device != x.device:
-            raise _lib.GanAmdError(f"layer_norm: x is on {x.device}, {name} on {t.device}")
+    if weight is not None:
+        _check_affine("weight", weight, x, shape)
+    if bias is not None:
+        _check_affine("bias", bias, x, shape)
     if not eps >= 0.0:
         raise _lib.GanAmdError(f"layer_norm: eps must not be negative, got {eps}")
     dtype_code(x)
     require_gpu(x)
-    if torch.is_grad_enabled():
-        x, weight = _not_a_leaf(x), _not_a_leaf(weight)
+    d = math.prod(shape)
+    if weight is not None and weight.is_leaf and weight.requires_grad and torch.is_grad_enabled():
+        weight = weight.view_as(weight)  # (see _wanted)
     if x.is_contiguous():
         return LayerNormFn.apply(x, weight, bias, d, eps)
     if x.dim() == 4 and len(shape) == 3 and x.is_contiguous(memory_format=CL):
         flat = [None if t is None else t.permute(1, 2, 0).reshape(d) for t in (weight, bias)]
         return LayerNormFn.apply(x.permute(0, 2, 3, 1), *flat, d, eps).permute(0, 3, 1, 2)
     return LayerNormFn.apply(x.contiguous(), weight, bias, d, eps)
+
+
+def _check_affine(name: str, t: Tensor, x: Tensor, shape) -> None:
+    if t.shape != shape:
+        raise _lib.GanAmdError(f"layer_norm: {name} has shape {tuple(t.shape)}, normalized_shape is {shape}")
+    if not t.is_floating_point():
+        raise _lib.GanAmdError(f"layer_norm: {name} must be floating point, got {t.dtype}")
+    if t.device != x.device:
+        raise _lib.GanAmdError(f"layer_norm: x is on {x.device}, {name} on {t.device}")
 
 
 class MbstdConcatFn(Function):
