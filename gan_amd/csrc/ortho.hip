@@ -46,7 +46,6 @@ struct Mat {
     int64_t stride;
     int64_t nat, tra;  // offsets of the planes that lie as the source does, and transposed
     int rows, cols;
-    int first;       // first workgroup of this launch that works on the group
 };
 
 // momentum: u = mu buf + (1 - mu) g, buf before u; nesterov: u = mu buf + (1 - mu) g once more
@@ -56,9 +55,10 @@ struct Source {
 };
 
 struct Mats {
-    Mat mat[NOPS];
     int count;
     Source from;
+    int first[NOPS];  // each group's first workgroup
+    Mat mat[NOPS];
 };
 
 // Byte offsets in one matrix's workspace: the partial sums, two X (each [m][n] and [n][m], hi plane then lo plane), five
@@ -70,12 +70,13 @@ struct Lay {
 };
 
 // What a product of `tiles` T x T tiles over `steps` steps of 32 k takes, in us, every tile's k in `cut` slices: workgroups run
-// in rounds, 256 (T = 256) or 512 of them at a time, a step of theirs as long as measured (T = 256: 2.8; T = 128: 0.55 alone
-// on a CU, 0.83 each where two share it; T = 64: 0.27 and 0.33), and slices are written and read again at 5 TB/s by one more launch.
+// in rounds, 256 (T = 256) or 512 of them at a time, a step of theirs as long as measured (T = 256: 2.8; T = 128: 0.48 alone
+// on a CU, 0.8 each where two share it; T = 64: 0.2 and 0.25), a round begins and ends in 5 to 9 us, and slices are written and
+// read again at 5 TB/s by one more launch.
 double cost_of(int T, int64_t tiles, int cut, int64_t steps) {
     const int64_t wgs = tiles * cut, slots = T < 256 && wgs > 256 ? 512 : 256;
-    const double alone = T == 256 ? 2.8 : T == 128 ? 0.55 : 0.27, shared = T == 128 ? 1.66 : 0.66;
-    return (double)ceil_div64(wgs, slots) * (double)ceil_div64(steps, cut) * (slots == 512 ? shared : alone) +
+    const double alone = T == 256 ? 2.8 : T == 128 ? 0.48 : 0.2, shared = T == 128 ? 1.6 : 0.5, ends = T == 256 ? 9. : T == 128 ? 7. : 5.;
+    return (double)ceil_div64(wgs, slots) * ((double)ceil_div64(steps, cut) * (slots == 512 ? shared : alone) + ends) +
            (cut > 1 ? 5. + (double)wgs * T * T * 8e-6 / 5. : 0.);
 }
 
@@ -135,7 +136,7 @@ __device__ __forceinline__ int group_of(const S& s, int id) {
     int lo = 0, hi = s.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (s.mat[mid].first <= id) lo = mid;
+        if (s.first[mid] <= id) lo = mid;
         else hi = mid - 1;
     }
     return lo;
@@ -148,9 +149,10 @@ __device__ __forceinline__ float update_of(const Source& s, float g, float m) { 
 template <typename T>
 __global__ void __launch_bounds__(256) ortho_norm_k(const Mats s) {
     __shared__ double red[4];
-    const Mat& q = s.mat[group_of(s, blockIdx.x)];
+    const int group = group_of(s, blockIdx.x);
+    const Mat q = s.mat[group];
     const int64_t size = (int64_t)q.rows * q.cols, chunk = chunk_of(size), nparts = parts_of(size);
-    const int local = (int)blockIdx.x - q.first, b = local / (int)nparts, c = local - b * (int)nparts;
+    const int local = (int)blockIdx.x - s.first[group], b = local / (int)nparts, c = local - b * (int)nparts;
     const T* __restrict__ g = (const T*)q.g + b * size;
     float* __restrict__ buf = q.buf ? q.buf + b * size : nullptr;
     const int64_t end = (c + 1) * chunk < size ? (c + 1) * chunk : size;
@@ -211,10 +213,11 @@ __device__ __forceinline__ float scale_of(const double* part, int nparts, float 
 template <typename T>
 __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
     __shared__ float tile[64][65];
-    const Mat& q = s.mat[group_of(s, blockIdx.x)];
+    const int group = group_of(s, blockIdx.x);
+    const Mat q = s.mat[group];
     const int rp = (int)up64(q.rows), cp = (int)up64(q.cols);
     const int tr = rp / 64, tc = cp / 64;
-    const int64_t local = blockIdx.x - q.first, b = local / ((int64_t)tr * tc);
+    const int64_t local = blockIdx.x - s.first[group], b = local / ((int64_t)tr * tc);
     const int t = (int)(local % ((int64_t)tr * tc)), r0 = t / tc * 64, c0 = t % tc * 64;
     const int64_t size = (int64_t)q.rows * q.cols;
     const T* g = (const T*)q.g + b * size;
@@ -273,7 +276,7 @@ struct Op {
     unsigned dn, dt, aux, join;
     int M, N, K;       // padded; symmetric results (dn == dt) have tiles on and above the diagonal only
     int rows, cols;    // of the source
-    int first, tiles;  // first workgroup, tiles per matrix
+    int tiles;         // per matrix
     int cut, steps;    // slices of k, steps of 32 k in each but the last
     int kind;
     float gain;        // SCALED: result = gain * accumulator
@@ -287,10 +290,10 @@ struct Rule {
 };
 
 struct Ops {
-    Op mat[NOPS];
     int count;
-    int sliced;  // some product of the launch is cut
     Rule rule;
+    int first[NOPS];  // each group's first workgroup
+    Op mat[NOPS];
 };
 
 __device__ __forceinline__ float step_of(const Rule& s, int rows, int cols) {
@@ -311,109 +314,101 @@ __device__ __forceinline__ int2 tile_of(int t, int n) {
 constexpr int TLD = 36;  // floats a row: 16-byte rows, and columns of eight spread over the banks
 constexpr int TBYTES = 32 * TLD * 4;
 
-__device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int b, int i0, int j0, const f32x16& acc, bool mirror,
-                                       int dtype, float* t) {
+// eight values to the two planes
+__device__ __forceinline__ void store_planes(h16* to, int64_t plane, const float (&o)[8]) {
+    h16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        h16 p, w;
+        split(o[e], p, w);
+        hi[e] = p;
+        lo[e] = w;
+    }
+    *(h16x8*)to = hi;
+    *(h16x8*)(to + plane) = lo;
+}
+
+// eight values of a row of the result, `left` of them inside it: stored, or taken off the parameters there
+template <typename T>
+__device__ __forceinline__ void store_result(const Rule& rule, T* to, float (&o)[8], int left, float step) {
+    if (left >= 8) {
+        if (rule.update) {
+            T old[8];
+            __builtin_memcpy(old, to, sizeof(old));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = fmaf(-step, o[e], rule.decay * (float)old[e]);
+        }
+        T r[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = (T)o[e];
+        __builtin_memcpy(to, r, sizeof(r));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+            if (e < left) to[e] = (T)(rule.update ? fmaf(-step, o[e], rule.decay * (float)to[e]) : o[e]);
+    }
+}
+
+__device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int b, int i0, int j0, f32x16& acc, bool mirror, int dtype, float* t) {
     const int lane = threadIdx.x & 63;
+    const int64_t plane = (int64_t)q.M * q.N;
+    // the values first, where the accumulators hold them: no branch or load stands between the trips through LDS
+    if (q.kind == POLY) {  // (A is symmetric: its rows for the columns held here)
+        const h16* A = (const h16*)(ws + (int64_t)q.aux * 256) + (int64_t)(j0 + (lane & 31)) * q.N + i0 + 4 * (lane >> 5);
+        h16x4 ah[4], al[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            ah[r] = *(const h16x4*)(A + 8 * r);
+            al[r] = *(const h16x4*)(A + plane + 8 * r);
+        }
+        const float c = s.rule.c * (SP / (SA * SA)), bb = s.rule.b * (SP / SA), aa = s.rule.a * SP;
+        const int on = j0 + (lane & 31) - i0 - 4 * (lane >> 5);  // the row of the diagonal
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            acc[r] = acc[r] * c + bb * ((float)ah[r >> 2][r & 3] + (float)al[r >> 2][r & 3]) + (on == 8 * (r >> 2) + (r & 3) ? aa : 0.f);
+    } else {
+        const float gain = q.kind == SCALED ? q.gain : 1.f / (SP * SX);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] *= gain;
+    }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int r = 0; r < 16; ++r) t[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * TLD + (lane & 31)] = acc[r];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_wave_barrier();
+    const int a = lane >> 2, c = (lane & 3) * 8;  // eight values a lane: columns c ... of rows a and a + 16, or the other way round
+    float o[2][8], x[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            o[h][e] = t[(h * 16 + a) * TLD + c + e];
+            x[h][e] = t[(c + e) * TLD + h * 16 + a];
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the next block may overwrite them)
     if (q.kind == RESULT) {
-        // eight consecutive elements of a row of the result a lane; a tall result is the transpose of the block
-        const bool wide = q.rows <= q.cols;
+        const bool wide = q.rows <= q.cols;  // a tall result is the transpose of the block
         const float step = s.rule.update ? step_of(s.rule, q.rows, q.cols) : 0.f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int a = h * 16 + (lane >> 2), c = (lane & 3) * 8;
-            float o[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = (wide ? t[a * TLD + c + e] : t[(c + e) * TLD + a]) * (1.f / (SP * SX));
-            const int row = (wide ? i0 : j0) + a, col = (wide ? j0 : i0) + c;
+            const int row = (wide ? i0 : j0) + h * 16 + a, col = (wide ? j0 : i0) + c;
             const int left = row < q.rows ? q.cols - col : 0;
             const int64_t at = ((int64_t)b * q.rows + row) * q.cols + col;
-            if (s.rule.update) {
-                float* p = (float*)q.out + at;
-                float old[8];
-                if (left >= 8) {
-                    __builtin_memcpy(old, p, 32);
+            float v[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] = fmaf(-step, o[e], s.rule.decay * old[e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e < left) o[e] = fmaf(-step, o[e], s.rule.decay * p[e]);
-                }
-            }
-            if (dtype == GAN_F32) {
-                float* p = (float*)q.out + at;
-                if (left >= 8) {
-                    __builtin_memcpy(p, o, 32);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e < left) p[e] = o[e];
-                }
-            } else {
-                bf16* p = (bf16*)q.out + at;
-                bf16 r[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) r[e] = (bf16)o[e];
-                if (left >= 8) {
-                    __builtin_memcpy(p, r, 16);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e < left) p[e] = r[e];
-                }
-            }
+            for (int e = 0; e < 8; ++e) v[e] = wide ? o[h][e] : x[h][e];
+            if (dtype == GAN_F32) store_result(s.rule, (float*)q.out + at, v, left, step);
+            else store_result(s.rule, (bf16*)q.out + at, v, left, step);
         }
         return;
     }
     h16 *dn = (h16*)(ws + (int64_t)q.dn * 256), *dt = (h16*)(ws + (int64_t)q.dt * 256);  // [i][j] and [j][i]
-    const int64_t plane = (int64_t)q.M * q.N;
-    const float gain = q.kind == SCALED ? q.gain : s.rule.c * (SP / (SA * SA));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int a = h * 16 + (lane >> 2), c = (lane & 3) * 8, i = i0 + a, j = j0 + c;
-        h16x8 hi, lo, ah, al;
-        if (q.kind == POLY) {
-            const h16* A = (const h16*)(ws + (int64_t)q.aux * 256) + (int64_t)i * q.N + j;
-            ah = *(const h16x8*)A;
-            al = *(const h16x8*)(A + plane);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float o = t[a * TLD + c + e] * gain;
-            if (q.kind == POLY) o += s.rule.b * (((float)ah[e] + (float)al[e]) * (SP / SA)) + (i == j + e ? s.rule.a * SP : 0.f);
-            if (mirror) t[a * TLD + c + e] = o;
-            h16 p, w;
-            split(o, p, w);
-            hi[e] = p;
-            lo[e] = w;
-        }
-        *(h16x8*)(dn + (int64_t)i * q.N + j) = hi;
-        *(h16x8*)(dn + plane + (int64_t)i * q.N + j) = lo;
-    }
+    for (int h = 0; h < 2; ++h) store_planes(dn + (int64_t)(i0 + h * 16 + a) * q.N + j0 + c, plane, o[h]);
     if (mirror) {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int a = h * 16 + (lane >> 2), c = (lane & 3) * 8;
-            h16x8 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                h16 p, w;
-                split(t[(c + e) * TLD + a], p, w);
-                hi[e] = p;
-                lo[e] = w;
-            }
-            *(h16x8*)(dt + (int64_t)(j0 + a) * q.M + i0 + c) = hi;
-            *(h16x8*)(dt + plane + (int64_t)(j0 + a) * q.M + i0 + c) = lo;
-        }
+        for (int h = 0; h < 2; ++h) store_planes(dt + (int64_t)(j0 + h * 16 + a) * q.M + i0 + c, plane, x[h]);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
 // an address that is the same in every lane, in scalar registers
@@ -443,10 +438,12 @@ struct Frags {
         if (of_u) u[pl][f] = got;
         else v[pl][f] = got;
     }
-    // hi lo, lo hi, hi hi, each over all of the wave's blocks (a block's accumulator then rests between two products)
-    __device__ __forceinline__ void multiply(f32x16 (&acc)[FM][FN], int i) const {
-        const int pass = i / (FM * FN), x = i % (FM * FN) / FN, y = i % FN;
-        acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[pass == 1][x], v[pass == 0][y], acc[x][y], 0, 0, 0);
+    // hi lo, lo hi, hi hi, each over all of the wave's blocks (a block's accumulator then rests between two products); a wave with
+    // one block only has an accumulator for each of the three
+    static constexpr int NACC = FM * FN == 1 ? 3 : 1;
+    __device__ __forceinline__ void multiply(f32x16 (&acc)[NACC][FM][FN], int i) const {
+        const int pass = i / (FM * FN), x = i % (FM * FN) / FN, y = i % FN, a = NACC == 3 ? pass : 0;
+        acc[a][x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[pass == 1][x], v[pass == 0][y], acc[a][x][y], 0, 0, 0);
     }
 };
 
@@ -478,20 +475,18 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
     constexpr int PER = STAGE / 1024 / WAVES;                      // DMA instructions per wave and stage
     constexpr int PP = PER / 4;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
-    // Workgroups go round the eight dies, each with a cache of its own.  Slices run fastest, so that a die meets few of them;
-    // where nothing is cut, a die gets a run of tiles that share their rows of V.
-    int id = blockIdx.x;
-    if (!s.sliced) {
-        const int each = gridDim.x >> 3, rest = gridDim.x & 7, die = id & 7;
-        id = die * each + (die < rest ? die : rest) + (id >> 3);
-    }
-    const Op& q = s.mat[group_of(s, id)];
+    // Workgroups go round the eight dies, each with a cache of its own: a die gets a run of them.  Tiles follow one another along
+    // the rows of U, sharing their rows of V, and a slice's tiles lie together.
+    const int each = gridDim.x >> 3, rest = gridDim.x & 7, die = blockIdx.x & 7;
+    const int id = die * each + (die < rest ? die : rest) + ((int)blockIdx.x >> 3);
+    const int group = group_of(s, id);
+    const Op q = s.mat[group];  // (a copy: one batch of scalar loads)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
     // (divisions run on vector registers: say that the results are the wave's, or every use of an address loops over lanes)
     const int per = q.tiles * q.cut;
-    const int b = __builtin_amdgcn_readfirstlane((id - q.first) / per);
-    const int in_b = id - q.first - b * per;
-    const int tile = __builtin_amdgcn_readfirstlane(in_b / q.cut), slice = in_b - tile * q.cut;
+    const int b = __builtin_amdgcn_readfirstlane((id - s.first[group]) / per);
+    const int in_b = id - s.first[group] - b * per;
+    const int slice = __builtin_amdgcn_readfirstlane(in_b / q.tiles), tile = in_b - slice * q.tiles;
     char* ws = q.ws + b * q.stride;
     const char *u = ws + (int64_t)q.u * 256, *v = ws + (int64_t)q.v * 256;
     const int M = q.M, N = q.N, K = q.K;
@@ -520,13 +515,16 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
         const int lim = pl < 2 ? M - i0 : N - j0;
         off[j] = (unsigned)(row < lim ? row : lim - 1) * kb + (unsigned)((pos ^ ((row >> 2) & 3)) * 16);
     }
-    f32x16 acc[FM][FN];
+    using Fr = Frags<FM, FN>;
+    f32x16 sums[Fr::NACC][FM][FN];
 #pragma unroll
-    for (int x = 0; x < FM; ++x)
+    for (int a = 0; a < Fr::NACC; ++a)
 #pragma unroll
-        for (int y = 0; y < FN; ++y)
+        for (int x = 0; x < FM; ++x)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
+            for (int y = 0; y < FN; ++y)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sums[a][x][y][r] = 0.f;
     const int k0 = slice * q.steps, nk = (K / 32 - k0 < q.steps ? K / 32 - k0 : q.steps);
 #pragma unroll
     for (int k = 0; k < NST; ++k)
@@ -539,7 +537,6 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
     // long as a third of its products take.  The barrier lies between the halves, where the next stage has to be there and
     // nobody reads this one any more; its place is then filled with stage k + NST, half of the requests before and half after
     // the next half's turn.
-    using Fr = Frags<FM, FN>;
     constexpr int HALF = PER / 2;
     const int m0 = wm * (T / 2), n0 = wn * (T / WN);
     Fr f0, f1;
@@ -550,28 +547,28 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
         char *here = lds + k % NST * STAGE, *last = lds + (k + NST - 1) % NST * STAGE, *next = lds + (k + 1) % NST * STAGE;
 #pragma unroll
         for (int i = 0; i < Fr::PRODUCTS; ++i) {
-            f0.multiply(acc, i);
+            f0.multiply(sums, i);
 #pragma unroll
             for (int r = 0; r < Fr::READS; ++r)
-                if (r * Fr::PRODUCTS / Fr::READS == i) f1.read(here, PLANE, m0, n0, 1, lane, r);
+                if (r * Fr::PRODUCTS / (2 * Fr::READS) == i) f1.read(here, PLANE, m0, n0, 1, lane, r);
             if (late) {
 #pragma unroll
                 for (int j = 0; j < HALF; ++j)
-                    if (j * Fr::PRODUCTS / HALF == i) ortho_issue<WAVES, PP>(last, k0 + k - 1 + NST, wave, planes, off, HALF + j);
+                    if ((j + 1) * Fr::PRODUCTS / HALF - 1 == i) ortho_issue<WAVES, PP>(last, k0 + k - 1 + NST, wave, planes, off, HALF + j);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         stage_arrived<(NST - 2) * PER>(k + NST - 1 < nk);  // stages k + 2 ... k + NST - 1 behind it
 #pragma unroll
         for (int i = 0; i < Fr::PRODUCTS; ++i) {
-            f1.multiply(acc, i);
+            f1.multiply(sums, i);
 #pragma unroll
             for (int r = 0; r < Fr::READS; ++r)
-                if (r * Fr::PRODUCTS / Fr::READS == i) f0.read(next, PLANE, m0, n0, 0, lane, r);
+                if (r * Fr::PRODUCTS / (2 * Fr::READS) == i) f0.read(next, PLANE, m0, n0, 0, lane, r);
             if (more) {
 #pragma unroll
                 for (int j = 0; j < HALF; ++j)
-                    if (j * Fr::PRODUCTS / HALF == i) ortho_issue<WAVES, PP>(here, k0 + k + NST, wave, planes, off, j);
+                    if ((j + 1) * Fr::PRODUCTS / HALF - 1 == i) ortho_issue<WAVES, PP>(here, k0 + k + NST, wave, planes, off, j);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -585,9 +582,14 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
 #pragma unroll
         for (int r = 0; r < Fr::READS; ++r) f1.read(here, PLANE, m0, n0, 1, lane, r);
 #pragma unroll
-        for (int i = 0; i < Fr::PRODUCTS; ++i) f0.multiply(acc, i);
+        for (int i = 0; i < Fr::PRODUCTS; ++i) f0.multiply(sums, i);
 #pragma unroll
-        for (int i = 0; i < Fr::PRODUCTS; ++i) f1.multiply(acc, i);
+        for (int i = 0; i < Fr::PRODUCTS; ++i) f1.multiply(sums, i);
+    }
+    f32x16(&acc)[FM][FN] = sums[0];
+    if (Fr::NACC == 3) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[0][0][r] = sums[Fr::NACC - 1][0][0][r] + (acc[0][0][r] + sums[Fr::NACC / 2][0][0][r]);
     }
     if (q.cut > 1) {  // this slice's sums, in the order that join_k reads them
         float4* out = (float4*)(ws + (int64_t)q.join * 256) + ((int64_t)slice * q.tiles + tile) * (T * T / 4) + wave * (T * T / 4 / WAVES) + lane;
@@ -603,42 +605,56 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();  // (the stages are read: their LDS is free)
     float* t = (float*)(lds + wave * TBYTES);
+    // one block after another through the same code: unrolled, its instructions would be fetched for every block anew
+#pragma unroll 1
+    for (int f = 0; f < FM * FN; ++f) {
+        f32x16 one = acc[0][0];
 #pragma unroll
-    for (int x = 0; x < FM; ++x)
-#pragma unroll
-        for (int y = 0; y < FN; ++y) {
-            const int i = i0 + wm * (T / 2) + x * 32, j = j0 + wn * (T / WN) + y * 32;
-            if (i < M && j < N) finish(s, q, ws, b, i, j, acc[x][y], !sym || ti != tj, dtype, t);
-        }
+        for (int k = 1; k < FM * FN; ++k)
+            if (f == k) one = acc[k / FN][k % FN];
+        const int i = i0 + wm * (T / 2) + f / FN * 32, j = j0 + wn * (T / WN) + f % FN * 32;
+        if (i < M && j < N) finish(s, q, ws, b, i, j, one, !sym || ti != tj, dtype, t);
+    }
 }
 
-// The slices of a product that was cut, added in their order; a 32 x 32 block a wave
+// The slices of a product that was cut, added in their order; a 32 x 32 block a workgroup of one wave
 template <int T>
-__global__ void __launch_bounds__(256) ortho_join_k(const Ops s, int dtype) {
+__global__ void __launch_bounds__(64) ortho_join_k(const Ops s, int dtype) {
     constexpr int WAVES = gemm_threads<T>() / 64, WN = WAVES / 2, FN = T / 32 / WN, BLK = T * T / 1024;  // blocks of a tile
-    __shared__ __attribute__((aligned(16))) float lds[4][TBYTES / 4];
-    const Op& q = s.mat[group_of(s, blockIdx.x)];
-    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int local = ((int)blockIdx.x - q.first) * 4 + wv, tile_b = local / BLK, b = tile_b / q.tiles, tile = tile_b - b * q.tiles;
+    __shared__ __attribute__((aligned(16))) float lds[TBYTES / 4];
+    const int group = group_of(s, blockIdx.x);
+    const Op q = s.mat[group];
+    const int lane = threadIdx.x;
+    const int local = (int)blockIdx.x - s.first[group], tile_b = local / BLK, b = tile_b / q.tiles, tile = tile_b - b * q.tiles;
     char* ws = q.ws + b * q.stride;
     const int blk = local % BLK, wave = blk / (BLK / WAVES), frag = blk % (BLK / WAVES);
     const float4* in = (const float4*)(ws + (int64_t)q.join * 256) + (int64_t)tile * (T * T / 4) + blk * 256 + lane;
+    const int64_t next = (int64_t)q.tiles * (T * T / 4);
     f32x16 acc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] = 0.f;
-    for (int c = 0; c < q.cut; ++c) {
+    constexpr int AHEAD = 8;  // slices requested at a time
+    for (int c = 0; c < q.cut; c += AHEAD) {
+        float4 v[AHEAD][4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float4 v = in[(int64_t)c * q.tiles * (T * T / 4) + r * 64];
-            acc[r * 4] += v.x;
-            acc[r * 4 + 1] += v.y;
-            acc[r * 4 + 2] += v.z;
-            acc[r * 4 + 3] += v.w;
-        }
+        for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[k][r] = in[(c + k < q.cut ? c + k : c) * next + r * 64];
+        __builtin_amdgcn_sched_barrier(0);  // (or the loads are moved to their uses, one wait each)
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool in_cut = c + k < q.cut;
+                acc[r * 4] += in_cut ? v[k][r].x : 0.f;
+                acc[r * 4 + 1] += in_cut ? v[k][r].y : 0.f;
+                acc[r * 4 + 2] += in_cut ? v[k][r].z : 0.f;
+                acc[r * 4 + 3] += in_cut ? v[k][r].w : 0.f;
+            }
     }
     const int2 t = tile_of(tile, (q.M + T - 1) / T);
     const int i = t.x * T + (wave / WN) * (T / 2) + frag / FN * 32, j = t.y * T + (wave % WN) * (T / WN) + frag % FN * 32;
-    if (i < q.M && j < q.N) finish(s, q, ws, b, i, j, acc, t.x != t.y, dtype, lds[wv]);
+    if (i < q.M && j < q.N) finish(s, q, ws, b, i, j, acc, t.x != t.y, dtype, lds);
 }
 
 template <int T, int NST>
@@ -721,7 +737,8 @@ struct Walk {
 
 // The next product of every matrix that has one left: one launch, and one more that joins slices where there are any.
 int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char* ws, int dtype, hipStream_t st) {
-    s.count = s.sliced = 0;
+    s.count = 0;
+    bool sliced = false;
     int64_t batch[NOPS];
     for (int k = 0; k < n; ++k) {
         Walk& w = walks[k];
@@ -736,7 +753,7 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
             q.join = (unsigned)(w.l.join / 256);
             w.next(q, steps);
             q.steps = (int)ceil_div64(q.K / 32, q.cut);
-            s.sliced |= q.cut > 1;
+            sliced |= q.cut > 1;
         }
         ws += w.l.bytes * mats[k].batch;
     }
@@ -760,27 +777,28 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
     for (int k = 0; k < s.count; ++k) {
         Op& q = s.mat[k];
         q.tiles = (int)tiles_of(q.M, q.N, q.kind != RESULT && q.dn == q.dt, T);
-        q.first = (int)blocks;
+        s.first[k] = (int)blocks;
         blocks += (int64_t)q.tiles * q.cut * batch[k];
     }
     if (int rc = T == 256                  ? launch_gemm<256, 2>((unsigned)blocks, s, dtype, st)
-                 : T == 64                 ? launch_gemm<64, 4>((unsigned)blocks, s, dtype, st)
-                 : blocks > 256            ? launch_gemm<128, 2>((unsigned)blocks, s, dtype, st)  // two a CU
-                                           : launch_gemm<128, 4>((unsigned)blocks, s, dtype, st))
+                 : T == 64 && blocks > 512 ? launch_gemm<64, 2>((unsigned)blocks, s, dtype, st)   // five a CU fit, and hide more than a longer ring
+                 : T == 64                 ? launch_gemm<64, 4>((unsigned)blocks, s, dtype, st)   // (576 tiles of k = 512: 16.7 us against 17.9)
+                 : blocks > 256            ? launch_gemm<128, 2>((unsigned)blocks, s, dtype, st)  // two a CU; 222 us against 237 with a ring of four
+                                           : launch_gemm<128, 4>((unsigned)blocks, s, dtype, st))  // alone: 131 us against 167 with a ring of two
         return rc;
-    if (!s.sliced) return GAN_OK;
+    if (!sliced) return GAN_OK;
     int64_t join = 0;
     int m = 0;
     for (int k = 0; k < s.count; ++k) {
         if (s.mat[k].cut == 1) continue;
         s.mat[m] = s.mat[k];
-        s.mat[m].first = (int)join;
-        join += (int64_t)s.mat[m++].tiles * batch[k] * (T * T / 4096);
+        s.first[m] = (int)join;
+        join += (int64_t)s.mat[m++].tiles * batch[k] * (T * T / 1024);
     }
     s.count = m;
-    if (T == 256) hipLaunchKernelGGL((ortho_join_k<256>), dim3((unsigned)join), dim3(256), 0, st, s, dtype);
-    else if (T == 128) hipLaunchKernelGGL((ortho_join_k<128>), dim3((unsigned)join), dim3(256), 0, st, s, dtype);
-    else hipLaunchKernelGGL((ortho_join_k<64>), dim3((unsigned)join), dim3(256), 0, st, s, dtype);
+    if (T == 256) hipLaunchKernelGGL((ortho_join_k<256>), dim3((unsigned)join), dim3(64), 0, st, s, dtype);
+    else if (T == 128) hipLaunchKernelGGL((ortho_join_k<128>), dim3((unsigned)join), dim3(64), 0, st, s, dtype);
+    else hipLaunchKernelGGL((ortho_join_k<64>), dim3((unsigned)join), dim3(64), 0, st, s, dtype);
     GAN_CHECK_LAUNCH("orthogonalize(join)");
     return GAN_OK;
 }
@@ -797,11 +815,12 @@ struct SmallMat {
     const void* g;
     float* buf;
     void* out;
-    int rows, cols, first;
+    int rows, cols;
 };
 struct Smalls {
-    SmallMat mat[NOPS];
     int count, steps;
+    int first[NOPS];
+    SmallMat mat[NOPS];
 };
 
 __host__ __device__ inline int up32(int v) { return (v + 31) & ~31; }
@@ -838,9 +857,10 @@ template <typename T>
 __global__ void __launch_bounds__(1024) ortho_small_k(const Smalls s, const Source h, const Rule o) {
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     __shared__ double red[16];
-    const SmallMat& q = s.mat[group_of(s, blockIdx.x)];
+    const int group = group_of(s, blockIdx.x);
+    const SmallMat q = s.mat[group];
     const int rows = q.rows, cols = q.cols, size = rows * cols;
-    const int64_t b = (int)blockIdx.x - q.first;
+    const int64_t b = (int)blockIdx.x - s.first[group];
     const bool wide = rows <= cols;
     const int mp = up32(wide ? rows : cols), np = up32(wide ? cols : rows), lm = np + 8, lt = mp + 8, la = mp + 8;
     const int pm = mp * lm, pt = np * lt, pa = mp * la;  // from hi to lo plane
@@ -1018,7 +1038,8 @@ int run_small(const gan_matrix* mats, int n, int steps, const Source& h, const R
     s.steps = steps;
     for (int k = 0; k < n; ++k) {
         const gan_matrix& g = mats[k];
-        s.mat[k] = SmallMat{g.g, g.buf, g.out, (int)g.rows, (int)g.cols, blocks};
+        s.mat[k] = SmallMat{g.g, g.buf, g.out, (int)g.rows, (int)g.cols};
+        s.first[k] = blocks;
         blocks += (int)g.batch;
         const int m = up32((int)(g.rows < g.cols ? g.rows : g.cols)), w = up32((int)(g.rows < g.cols ? g.cols : g.rows));
         const int need = (m * (w + 8) + w * (m + 8)) * 4;
@@ -1102,7 +1123,7 @@ int pack(const gan_matrix* mats, int n, char* ws, Mats& s, hipStream_t st) {
         for (int j = 0; j < 2; ++j) first[j][k + 1] = first[j][k] + per[j] * g.batch;
     }
     for (int j = 0; j < 2; ++j) {
-        for (int k = 0; k < n; ++k) s.mat[k].first = (int)first[j][k];
+        for (int k = 0; k < n; ++k) s.first[k] = (int)first[j][k];
         const dim3 grid((unsigned)first[j][n]), block(256);
         if (j == 0) hipLaunchKernelGGL((ortho_norm_k<T>), grid, block, 0, st, s);
         else hipLaunchKernelGGL((ortho_pack_k<T>), grid, block, 0, st, s);
