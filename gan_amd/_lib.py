@@ -104,6 +104,7 @@ _SIGNATURES = {
     "gan_orthogonalize_workspace": (c_int64, [c_void_p, c_int]),
     "gan_orthogonalize": (c_int, [c_void_p, c_int, c_int] + [c_float] * 4 + [c_int, c_void_p, c_int64, c_void_p]),
     "gan_muon_step": (c_int, [c_void_p, c_int, c_float, c_float, c_int, c_float, c_int, c_int] + [c_float] * 4 + [c_void_p, c_int64, c_void_p]),
+    "gan_adam_step_ranges": (c_int, [c_void_p] * 5 + [c_int, c_void_p, c_int] + [c_float] * 5 + [c_int, c_void_p]),
     "gan_adam_step": (c_int, [c_void_p] * 4 + [c_int64, c_void_p, c_int] + [c_float] * 5 + [c_int, c_void_p]),
 }
 

@@ -6,7 +6,10 @@
 module's flat parameter / gradient arenas (gan_amd/utils.py: FlatArena) with the step count on the device, so the
 whole optimizer step is two launches and can be captured in a HIP graph.  torch's own Adam needs capturable=True
 for that, which costs a launch per parameter tensor for each bias-correction scalar (~600 launches per iteration
-for the two StyleGAN2 networks)."""
+for the two StyleGAN2 networks).
+
+`muon_step` / `FlatMuon` take matrices by their orthogonalised momentum instead (functional.orthogonalize), all of a
+network's in shared launches; optimizer="Muon" in the train step."""
 from __future__ import annotations
 
 import ctypes
@@ -22,6 +25,7 @@ from ._lib import check, ptr, require_gpu, stream_of
 from .utils import FlatArena, arena_of
 
 _FLAT_KEYS = {"betas", "eps", "weight_decay"}
+_MUON_KEYS = {"weight_decay", "momentum", "nesterov", "ns_coefficients", "eps", "ns_steps", "adjust_lr_fn", "adam_lr", "betas", "adam_eps"}
 
 
 class FlatAdam(torch.optim.Optimizer):
@@ -155,7 +159,6 @@ def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentum_buffer
         raise _lib.GanAmdError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momentum_buffers)} momentum buffers")
     if adjust_lr_fn not in _SCALINGS:
         raise _lib.GanAmdError(f"muon_step: adjust_lr_fn must be None, 'original', 'match_rms_adamw' or 'none', got {adjust_lr_fn!r}")
-    a, b, c = (float(v) for v in coefficients)
     held, mats, seen = [], [], set()
     for p, g, m in zip(params, grads, momentum_buffers):
         if p.dim() < 2:
@@ -177,24 +180,137 @@ def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentum_buffer
                 raise _lib.GanAmdError("muon_step: a parameter or momentum buffer is given twice")
             seen.add(t.data_ptr())
         mats.append((g.data_ptr(), m.data_ptr(), p.data_ptr(), *_as_matrix(p.shape), 1))
+    if any(g.data_ptr() in seen for g in held):
+        raise _lib.GanAmdError("muon_step: a gradient lies where a parameter or momentum buffer does")
     require_gpu(*params[:1])
     if not mats:
         return
-    array = (_lib.Matrix * len(mats))(*mats)
-    ws, nbytes = GF.matrix_workspace(array, params[0].device)
-    flops = sum(GF.ortho_flops(t[3], t[4], steps) for t in mats)
-    with _lib.on_device(params[0]):
-        check(GF._run("muon_step", flops, 20 * sum(t[3] * t[4] for t in mats),
-                      lambda: _lib.load().gan_muon_step(ctypes.addressof(array), len(mats), float(lr), float(momentum), int(bool(nesterov)),
-                                                        float(weight_decay), _SCALINGS[adjust_lr_fn], int(steps), a, b, c, float(eps), ptr(ws),
-                                                        nbytes, stream_of(params[0]))), "gan_muon_step")
+    _muon_launch((_lib.Matrix * len(mats))(*mats), params[0], lr, momentum, nesterov, weight_decay, adjust_lr_fn, steps, coefficients, eps)
     # written through raw pointers: cached GEMM images of the old values would still match their keys
     GF.invalidate_packed(params)
 
 
+def _muon_launch(mats, like: Tensor, lr, momentum, nesterov, weight_decay, adjust_lr_fn, steps, coefficients, eps) -> None:
+    a, b, c = (float(v) for v in coefficients)
+    ws, nbytes = GF.matrix_workspace(mats, like.device)
+    with _lib.on_device(like):
+        check(GF._run("muon_step", sum(GF.ortho_flops(t.rows, t.cols, steps) for t in mats) if GF._PROFILE is not None else 0,
+                      20 * sum(t.rows * t.cols for t in mats) if GF._PROFILE is not None else 0,
+                      lambda: _lib.load().gan_muon_step(ctypes.addressof(mats), len(mats), float(lr), float(momentum), int(bool(nesterov)),
+                                                        float(weight_decay), _SCALINGS[adjust_lr_fn], int(steps), a, b, c, float(eps), ptr(ws),
+                                                        nbytes, stream_of(like))), "gan_muon_step")
+
+
+class FlatMuon(torch.optim.Optimizer):
+    """muon_step over a FlatArena for the matrices of a network, Adam for the rest of it (biases, norm scales, and whatever is a
+    vector in a matrix's shape: one row or one column), in place on the arenas.
+
+    * two `param_groups`: the matrices (`lr`, `weight_decay`, `momentum`, `nesterov`, `ns_coefficients`, `eps`, `ns_steps`,
+      `adjust_lr_fn`: torch.optim.Muon's names and update rule, its products in 22 bits instead of bfloat16's 8) and the rest
+      (`lr` = `adam_lr`, by default the matrices' lr; `betas`, `eps` = `adam_eps`, `weight_decay` 0), read at every step
+      (under HIP-graph capture the values at capture time are baked in);
+    * `state[p]` is `momentum_buffer` for a matrix, `step` / `exp_avg` / `exp_avg_sq` for the rest (FlatAdam's: one shared step);
+    * parameters whose `.grad` is None, and frozen ones, are skipped.
+
+    torch.optim.Muon itself takes two-dimensional parameters only; here a convolution counts as the matrix (out, in kh kw)."""
+
+    def __init__(self, arena: FlatArena, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95, nesterov: bool = True,
+                 ns_coefficients=GF.NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5, adjust_lr_fn: Optional[str] = None, *,
+                 adam_lr: Optional[float] = None, betas: Tuple[float, float] = (0.9, 0.999), adam_eps: float = 1e-8):
+        if arena.grad is None:
+            raise ValueError("FlatMuon needs an arena with a gradient buffer (arena_of(module, with_grad=True))")
+        if adjust_lr_fn not in _SCALINGS:
+            raise ValueError(f"FlatMuon: adjust_lr_fn must be None, 'original', 'match_rms_adamw' or 'none', got {adjust_lr_fn!r}")
+        self.arena = arena
+        self._matrix = [p.dim() >= 2 and min(_as_matrix(p.shape)) > 1 for p in arena.params]
+        matrices = [p for p, m in zip(arena.params, self._matrix) if m]
+        rest = [p for p, m in zip(arena.params, self._matrix) if not m]
+        groups = []
+        if matrices:
+            groups.append(dict(params=matrices, lr=float(lr), weight_decay=float(weight_decay), momentum=float(momentum), nesterov=bool(nesterov),
+                               ns_coefficients=tuple(float(c) for c in ns_coefficients), eps=float(eps), ns_steps=int(ns_steps),
+                               adjust_lr_fn=adjust_lr_fn))
+        if rest:
+            groups.append(dict(params=rest, lr=float(lr if adam_lr is None else adam_lr), betas=(float(betas[0]), float(betas[1])),
+                               eps=float(adam_eps), weight_decay=0.0))
+        super().__init__(groups, {})
+        dev = arena.data.device
+        self.exp_avg = torch.zeros_like(arena.data)  # the matrices' momentum too
+        self.exp_avg_sq = torch.zeros_like(arena.data)
+        self.step_t = torch.zeros(4, dtype=torch.float32, device=dev)  # [0] = updates done so far
+        self._mats: Dict[Tuple[bool, ...], object] = {}
+        self._point_state()
+
+    def _point_state(self) -> None:
+        step = self.step_t[0]
+        for p, o, m in zip(self.arena.params, self.arena.offsets, self._matrix):
+            n = p.numel()
+            avg = self.exp_avg[o:o + n].view(p.shape)
+            self.state[p] = {"momentum_buffer": avg} if m else {"step": step, "exp_avg": avg, "exp_avg_sq": self.exp_avg_sq[o:o + n].view(p.shape)}
+
+    def _matrices(self, present: Tuple[bool, ...]):
+        """The library's list of the matrices that take part (addresses in the arenas: they stay where they are)."""
+        if present not in self._mats:
+            a = self.arena
+            rows = [(a.grad.data_ptr() + 4 * o, self.exp_avg.data_ptr() + 4 * o, a.data.data_ptr() + 4 * o, *_as_matrix(p.shape), 1)
+                    for p, o, m, ok in zip(a.params, a.offsets, self._matrix, present) if m and ok]
+            vecs = [v for p, o, m, ok in zip(a.params, a.offsets, self._matrix, present) if ok and not m for v in (o, p.numel())]
+            self._mats[present] = ((_lib.Matrix * len(rows))(*rows), (ctypes.c_int64 * len(vecs))(*vecs))
+        return self._mats[present]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        arena = self.arena
+        if not arena.intact():
+            raise RuntimeError("FlatMuon: parameters were moved after flattening (model.to(...) / .half()); rebuild the optimizer")
+        require_gpu(arena.data)
+        base = arena.grad.data_ptr()
+        present = tuple(p.grad is not None and p.requires_grad for p in arena.params)
+        if any(p.grad is not None and p.grad.data_ptr() != base + 4 * o for p, o in zip(arena.params, arena.offsets)):
+            arena.gather_grads()  # re-attaches every slice; `present` remembers who really had a gradient
+        mats, ranges = self._matrices(present)
+        groups = {("momentum" in g): g for g in self.param_groups}
+        if len(mats):
+            g = groups[True]
+            _muon_launch(mats, arena.data, g["lr"], g["momentum"], g["nesterov"], g["weight_decay"], g["adjust_lr_fn"], g["ns_steps"],
+                         g["ns_coefficients"], g["eps"])
+        if len(ranges):
+            g = groups[False]
+            with _lib.on_device(arena.data):
+                check(_lib.load().gan_adam_step_ranges(ptr(arena.data), ptr(arena.grad), ptr(self.exp_avg), ptr(self.exp_avg_sq),
+                                                       ctypes.addressof(ranges), len(ranges) // 2, ptr(self.step_t), 1, float(g["lr"]),
+                                                       float(g["betas"][0]), float(g["betas"][1]), float(g["eps"]), float(g["weight_decay"]), 0,
+                                                       stream_of(arena.data)), "gan_adam_step_ranges")
+        # the kernels wrote through raw pointers (see FlatAdam.step)
+        GF.invalidate_packed(arena.params)
+        return loss
+
+    zero_grad = FlatAdam.zero_grad
+
+    def load_state_dict(self, state_dict) -> None:
+        """The per-tensor entries are copied into the flat buffers, which stay the storage."""
+        super().load_state_dict(state_dict)
+        with torch.no_grad():
+            for p, o, m in zip(self.arena.params, self.arena.offsets, self._matrix):
+                s, n = self.state.get(p), p.numel()
+                if not s:
+                    continue
+                if m:
+                    self.exp_avg[o:o + n].copy_(s["momentum_buffer"].reshape(-1))
+                else:
+                    self.exp_avg[o:o + n].copy_(s["exp_avg"].reshape(-1))
+                    self.exp_avg_sq[o:o + n].copy_(s["exp_avg_sq"].reshape(-1))
+                    self.step_t[0] = float(s["step"])
+        self._point_state()
+
+
 def make_optimizer(name: str, module: nn.Module, lr: float, kwargs: Dict, *, capturable: bool = False) -> torch.optim.Optimizer:
     """The optimizer `name` (a torch.optim class name, train_celeba.py:75) for `module`'s parameters.  Adam / AdamW with
-    only betas / eps / weight_decay set run as FlatAdam on a ROCm device; everything else is torch's own class
+    only betas / eps / weight_decay set run as FlatAdam on a ROCm device, Muon as FlatMuon; everything else is torch's own class
     (with capturable=True where it exists and the step is going to be captured in a HIP graph)."""
     params = list(module.parameters())
     on_gpu = bool(params) and all(p.is_cuda and p.dtype == torch.float32 for p in params)
@@ -204,6 +320,8 @@ def make_optimizer(name: str, module: nn.Module, lr: float, kwargs: Dict, *, cap
         if name == "AdamW":
             kw.setdefault("weight_decay", 1e-2)  # torch.optim.AdamW's default
         return FlatAdam(arena, lr, decoupled=name == "AdamW", **kw)
+    if name == "Muon" and on_gpu and set(kwargs) <= _MUON_KEYS:
+        return FlatMuon(arena_of(module, with_grad=True), lr, **kwargs)
     cls = getattr(torch.optim, name)
     kw = dict(kwargs)
     if capturable and name in ("Adam", "AdamW", "NAdam", "RAdam", "Adamax", "Adadelta", "Adagrad", "ASGD", "RMSprop", "Rprop"):

@@ -439,6 +439,11 @@ int gan_ema_lerp(float* ema, const float* p, int64_t n, float weight, gan_stream
 int gan_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float* step, int advance, float lr, float beta1,
                   float beta2, float eps, float weight_decay, int decoupled, gan_stream_t stream);
 
+/* The same update over `count` parts of the arenas, ranges[2k] = first element, ranges[2k + 1] = elements (a host array, read
+ * during the call; parts must not overlap): the parameters of a network that another rule does not take. */
+int gan_adam_step_ranges(float* p, const float* g, float* m, float* v, const int64_t* ranges, int count, float* step, int advance, float lr,
+                         float beta1, float beta2, float eps, float weight_decay, int decoupled, gan_stream_t stream);
+
 /* ---- orthogonalised updates: X = G / max(|G|, eps) (Frobenius norm; m x n, m <= n, a tall G as its transpose), then `steps`
  * times X <- (a I + b A + c A A) X with A = X X' (Newton-Schulz).  A gan_matrix is `batch` (0: none) dense row-major
  * (rows, cols) matrices one behind the other; a call takes a list of them, of any sizes.

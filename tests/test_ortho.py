@@ -196,6 +196,171 @@ def test_same_bits_other_stream_and_graph(dev):
             assert all(torch.equal(a, b) for a, b in zip(eager, h)), k
 
 
+def adam_ref(p, g, m, v, t, lr, betas, eps):
+    m.mul_(betas[0]).add_(g, alpha=1 - betas[0])
+    v.mul_(betas[1]).addcmul_(g, g, value=1 - betas[1])
+    p.addcdiv_(m / (1 - betas[0] ** t), (v / (1 - betas[1] ** t)).sqrt().add_(eps), value=-lr)
+
+
+@pytest.mark.gpu
+def test_flat_muon(dev):
+    """make_optimizer("Muon"): matrices by muon_step's rule, the rest by Adam's, against both in 64 bits over four steps in which
+    one matrix and one bias each skip a step; state_dict and back; frozen parameters."""
+    from torch import nn
+
+    from gan_amd.optim import FlatMuon, make_optimizer
+
+    torch.manual_seed(0)
+
+    def build():
+        net = nn.Sequential(nn.Conv2d(3, 20, 3), nn.LayerNorm(20), nn.Linear(30, 11), nn.Conv2d(9, 1, 2), nn.Linear(6, 6, bias=False)).to(dev)
+        net.register_parameter("scale", nn.Parameter(torch.ones(7, 1, 1, device=dev)))
+        net[4].weight.requires_grad_(False)
+        return net
+
+    net = build()
+    opt = make_optimizer("Muon", net, 0.05, {"weight_decay": 0.02, "momentum": 0.8, "adam_lr": 2e-3, "betas": [0.5, 0.9]})
+    assert isinstance(opt, FlatMuon) and len(opt.param_groups) == 2
+    params = list(net.parameters())
+    ref = [p.detach().double().cpu().clone() for p in params]
+    m, v = ([torch.zeros_like(r) for r in ref] for _ in range(2))
+    is_matrix = [r.dim() >= 2 and min(r.shape[0], r[0].numel()) > 1 for r in ref]
+    assert sum(is_matrix) == 3 and len(opt.param_groups[0]["params"]) == 3
+    frozen = params[-2] if not params[-2].requires_grad else next(p for p in params if not p.requires_grad)
+    held = frozen.detach().clone()
+    for step in range(4):
+        for i, (p, r) in enumerate(zip(params, ref)):
+            if (step == 2 and i in (0, 1)) or not p.requires_grad:
+                p.grad = None
+                continue
+            g = torch.randn(p.shape) * 10.0 ** (i - 3)
+            p.grad = g.to(dev)
+            if is_matrix[i]:
+                r.copy_(step_ref(r, g, m[i], 0.05, 0.8, True, 0.02, None)[0])
+                m[i].mul_(0.8).add_(g.double(), alpha=1 - 0.8)
+            else:
+                adam_ref(r, g.double(), m[i], v[i], step + 1, 2e-3, (0.5, 0.9), 1e-8)
+        before = [p.detach().clone() for p in params]
+        opt.step()
+        for i, (p, r) in enumerate(zip(params, ref)):
+            if step == 2 and i in (0, 1):
+                assert torch.equal(p, before[i])
+            elif p.requires_grad:
+                # (p ~ 0.1 ... 1 with its own rounding; four updates of 0.05 x 1 / sqrt(n) an entry within 6e-4 of themselves)
+                assert float((p.detach().double().cpu() - r).norm()) <= 1e-5 * float(r.norm()) + 4 * 6e-4 * 0.05 * math.sqrt(min(r.shape[0], r[0].numel()) if is_matrix[i] else 0), (step, i)
+    assert torch.equal(frozen, held)
+    # a second optimizer continues from the state
+    saved = opt.state_dict()
+    keys = [set(s) for s in saved["state"].values()]
+    assert {"momentum_buffer"} in keys and {"step", "exp_avg", "exp_avg_sq"} in keys
+    twin = build()
+    twin.load_state_dict(net.state_dict())
+    opt2 = make_optimizer("Muon", twin, 1.0, {})
+    opt2.load_state_dict(saved)
+    for p, q in zip(params, twin.parameters()):
+        if p.requires_grad:
+            p.grad = torch.randn_like(p)
+            q.grad = p.grad.clone()
+    opt.step(), opt2.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, twin.parameters()))
+    # a bad coefficient is refused at the step, other classes stay torch's
+    assert isinstance(make_optimizer("Muon", nn.Linear(3, 3, bias=False), 0.1, {}), torch.optim.Muon)  # (not on the device)
+    with pytest.raises(ValueError):
+        make_optimizer("Muon", build(), 0.1, {"adjust_lr_fn": "x"})
+
+
+@pytest.mark.gpu
+def test_norm_penalty_and_step_together(dev):
+    """What the operators are for: a critic that normalises whole samples, trained by WGAN-GP (its penalty differentiates the
+    norm's backward) with the orthogonalised step.  Gradients against the same critic in 64 bits; the update against the
+    rule; then the whole step replayed as a HIP graph against the eager one."""
+    from torch import nn
+
+    from gan_amd.losses import wgan_gp_regularizer
+    from gan_amd.modelling.common import Conv2d, LayerNorm, LeakyReLU
+    from gan_amd.optim import make_optimizer
+
+    torch.manual_seed(5)
+
+    class Critic(nn.Module):
+        def __init__(self, conv, norm, act):
+            super().__init__()
+            self.conv, self.norm, self.act, self.head = conv(3, 24, 3, padding=1), norm((24, 8, 8)), act(0.2), nn.Linear(24 * 64, 1)
+
+        def forward(self, x):
+            return self.head(self.act(self.norm(self.conv(x))).flatten(1))[:, 0]
+
+    net = Critic(Conv2d, LayerNorm, LeakyReLU).to(dev)
+    with torch.no_grad():
+        net.norm.weight.normal_(1, 0.3), net.norm.bias.normal_(0, 0.3)
+    ref = Critic(nn.Conv2d, nn.LayerNorm, nn.LeakyReLU).double()
+    ref.load_state_dict({k: t.double().cpu() for k, t in net.state_dict().items()})
+    reals, fakes, alpha = torch.randn(6, 3, 8, 8), torch.randn(6, 3, 8, 8), torch.rand(6, 1, 1, 1)
+    inter = (reals + alpha * (fakes - reals)).double().requires_grad_()
+    (gx,) = torch.autograd.grad(ref(inter).sum(), inter, create_graph=True)
+    penalty = (gx.flatten(1).norm(dim=1) - 1).square().mean() * 10
+    (penalty + ref(fakes.double()).mean() - ref(reals.double()).mean()).backward()
+
+    opt = make_optimizer("Muon", net, 0.02, {"weight_decay": 0.0})
+    opt.zero_grad()
+    real_rand = torch.rand
+    try:
+        torch.rand = lambda *a, **k: alpha.to(dev)
+        loss = wgan_gp_regularizer(net, reals.to(dev), fakes.to(dev), None) + net(fakes.to(dev)).mean() - net(reals.to(dev)).mean()
+    finally:
+        torch.rand = real_rand
+    loss.backward()
+    for (name, p), q in zip(net.named_parameters(), ref.parameters()):
+        assert rel_err(p.grad, q.grad) < 1e-4, name  # (fp32 convolutions of 27 and products of 1536 terms, twice differentiated)
+    before = {n: p.detach().double().cpu().clone() for n, p in net.named_parameters()}
+    opt.step()
+    w = net.conv.weight
+    want, _ = step_ref(before["conv.weight"], w.grad, torch.zeros_like(w), 0.02, 0.95, True, 0.0, None)
+    upd = w.detach().double().cpu() - before["conv.weight"]
+    assert float((upd - (want - before["conv.weight"])).norm()) <= 6e-4 * float((want - before["conv.weight"]).norm()) + 2.0**-23 * float(want.norm())
+    del loss
+
+    # ---- captured and replayed: a multilayer critic (library products: the same bits every time)
+    def build():
+        torch.manual_seed(9)
+        return nn.Sequential(nn.Linear(40, 96), LayerNorm(96), nn.Tanh(), nn.Linear(96, 96), LayerNorm(96), nn.Tanh(), nn.Linear(96, 1)).to(dev)
+
+    def trainer(net):
+        opt = make_optimizer("Muon", net, 0.02, {"weight_decay": 0.01, "adam_lr": 1e-3})
+
+        def step(x):
+            opt.zero_grad()
+            xi = x.detach().requires_grad_()
+            (g,) = torch.autograd.grad(net(xi).sum(), xi, create_graph=True)
+            ((g.norm(dim=1) - 1).square().mean() + net(x).mean()).backward()
+            opt.step()
+
+        return step
+
+    nets = build(), build()
+    eager, graphed = trainer(nets[0]), trainer(nets[1])
+    batches = [torch.randn(32, 40, device=dev) for _ in range(7)]
+    x = batches[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for b in batches[:3]:
+            x.copy_(b)
+            graphed(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        graphed(x)
+    for k, b in enumerate(batches):
+        eager(b)
+        if k >= 3:
+            x.copy_(b)
+            graph.replay()
+            torch.cuda.synchronize()
+            for p, q in zip(*(n.parameters() for n in nets)):
+                assert rel_err(q, p) < 1e-4, k
+
+
 def test_refusals():
     from gan_amd import _lib
     from gan_amd import functional as GF
@@ -218,7 +383,9 @@ def test_refusals():
         (([x], [x.t()], [x]), {}),
         (([x.double()], [x], [x]), {}),
         (([x.t()], [x.t()], [x.t()]), {}),
-        (([x, x], [x, x], [x.clone(), x.clone()]), {}),
+        (([x, x], [x.clone(), x.clone()], [x.clone(), x.clone()]), {}),
+        (([x], [x], [x.clone()]), {}),
+        (([x], [x.clone()], [x]), {}),
         (([x], [x.clone()], [x.clone()]), dict(adjust_lr_fn="other")),
     ):
         with pytest.raises(_lib.GanAmdError):
