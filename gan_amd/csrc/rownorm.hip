@@ -8,8 +8,8 @@
 //             gxx = r P(g cw - r (v mean(h t) + h mean(v t))) - r^2 t (mean(v h) - mean v mean h - mean(v t) mean(h t))
 //             gww = sum_rows g r P(v)
 // All three move a few bytes per flop: HBM bounds them.  Each row is read once and kept in registers, 16 bytes a lane and
-// load, between its statistics and its results; a row belongs to TPR threads (16 ... 512) with one or two
-// such vectors each (four in the widest), so that short rows need no LDS and registers leave room for many waves.  Longer rows are cut into pieces
+// load, between its statistics and its results; a row belongs to TPR threads (16 and more) with one or two
+// such vectors each (up to 1024 and four in the widest), so that short rows need no LDS and registers leave room for many waves.  Longer rows are cut into pieces
 // that first sum and then, in a second launch, join the sums and write.
 // Column sums: where a workgroup walks over many rows, its threads keep their columns' sums in registers and write one
 // partial row per workgroup (fold_cols_k adds those in a fixed order: no atomics, the same bits on every run); where there
@@ -76,6 +76,16 @@ struct RowRegs {
         }
     }
     __device__ __forceinline__ float at(int k, int e) const { return (float)v[k].e[e]; }
+    // Between a row's sums and its results: what was computed from the elements is computed again, the packed words alone stay
+    // (kept as floats beside them, a row of three bf16 tensors takes four times the registers).
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            uint4 w = __builtin_bit_cast(uint4, v[k]);
+            asm volatile("" : "+v"(w.x), "+v"(w.y), "+v"(w.z), "+v"(w.w));
+            v[k] = __builtin_bit_cast(Vec<T, V>, w);
+        }
+    }
     // elements of vector k that exist
     static __device__ __forceinline__ int count(int k, int lane, int n) {
         const int left = n - (lane + k * TPR) * V;
@@ -130,6 +140,29 @@ __device__ __forceinline__ void row_sum(float (&s)[N], float* lds, int& flip) {
     }
 }
 
+// Side vectors of a kernel whose threads walk over many rows stay in registers (HOLD); where a row takes 512 threads and more,
+// registers are short and they are read again for each row, vector by vector.
+template <int V, int K, int TPR, bool HOLD>
+struct Cols {
+    float held[HOLD ? K : 1][V];
+    const float* p;
+    float def;
+    __device__ __forceinline__ Cols(const float* p_, float def_, int lane, int n) : p(p_), def(def_) {
+        if constexpr (HOLD) load_cols<V, K, TPR>(p_, def_, held, lane, n);
+    }
+    __device__ __forceinline__ void get(int k, int lane, int n, float (&o)[V]) const {
+        if constexpr (HOLD) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = held[k][e];
+        } else {
+            float one[1][V];
+            load_cols<V, 1, TPR>(p ? p + (int64_t)k * TPR * V : nullptr, def, one, lane, n - k * TPR * V);
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = one[0][e];
+        }
+    }
+};
+
 struct RowArgs {
     const void *x, *g, *v;
     const float *w, *b, *cw, *cb;
@@ -142,6 +175,8 @@ struct RowArgs {
     int D;
     float eps;
     int pieces, piece;  // long rows: pieces per row, elements in each but the last
+    int row_blocks, col_tiles;  // backward in one launch with its column sums: workgroups of the rows, tiles of columns
+    int64_t chunk;              // and rows in a chunk
 };
 
 template <int TPR>
@@ -157,9 +192,7 @@ __global__ void __launch_bounds__(block_of<TPR>()) ln_fwd_k(const RowArgs a) {
     int flip = 0;
     const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
     const int D = a.D;
-    float w[K][V], b[K][V];
-    load_cols<V, K, TPR>(a.w, 1.f, w, lane, D);
-    load_cols<V, K, TPR>(a.b, 0.f, b, lane, D);
+    const Cols<V, K, TPR, (TPR < 512)> w(a.w, 1.f, lane, D), b(a.b, 0.f, lane, D);
     const float inv = 1.f / (float)D;
     for (int64_t row = (int64_t)blockIdx.x * G + grp; row < a.rows; row += (int64_t)gridDim.x * G) {
         RowRegs<T, V, K, TPR> x;
@@ -170,6 +203,7 @@ __global__ void __launch_bounds__(block_of<TPR>()) ln_fwd_k(const RowArgs a) {
 #pragma unroll
             for (int e = 0; e < V; ++e) s[0] += x.at(k, e);
         row_sum<1, TPR>(s, lds, flip);
+        x.settle();
         const float m = s[0] / (float)D;  // (a division: a row of one value has that mean, and 1 / r may be 300 times the rounding)
         float q[1] = {0.f};
 #pragma unroll
@@ -182,12 +216,17 @@ __global__ void __launch_bounds__(block_of<TPR>()) ln_fwd_k(const RowArgs a) {
             }
         }
         row_sum<1, TPR>(q, lds, flip);
+        x.settle();
         const float r = rsqrtf(q[0] * inv + a.eps);
         if (lane == 0) a.stats[row] = make_float2(m, r);
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            float wk[V], bk[V];
+            w.get(k, lane, D, wk);
+            b.get(k, lane, D, bk);
 #pragma unroll
-            for (int e = 0; e < V; ++e) x.v[k].e[e] = (T)fmaf((x.at(k, e) - m) * r, w[k][e], b[k][e]);
+            for (int e = 0; e < V; ++e) x.v[k].e[e] = (T)fmaf((x.at(k, e) - m) * r, wk[e], bk[e]);
+        }
         x.store((T*)a.y + row * D, lane, D);
     }
 }
@@ -222,55 +261,139 @@ __device__ __forceinline__ void write_partials(float (&acc)[NC][K][V], float* pa
     }
 }
 
+// ---- column sums down the rows -------------------------------------------------------------------------------------
+// 16 lanes across a vector of columns each, the workgroup's other threads down the rows of chunk `chunk_id`.  PASS 1: (g t, g),
+// 2: g r P(v).  out: [chunks][NC][D].
+template <typename T, int PASS, int BLK>
+__device__ __forceinline__ void col_sums(const RowArgs& a, float* __restrict__ out, int64_t chunk, int tile, int chunk_id) {
+    constexpr int V = VecOf<T>::V, NC = PASS == 1 ? 2 : 1, CG = BLK / 16, NW = BLK / 64;
+    __shared__ float red[NC][NW][16 * V];
+    const int lane = threadIdx.x & 15, grp = threadIdx.x >> 4, wave = threadIdx.x >> 6;
+    const int c0 = (tile * 16 + lane) * V;
+    const int left = a.D - c0;
+    float acc[NC][V];
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[j][e] = 0.f;
+    const int64_t r0 = (int64_t)chunk_id * chunk, r1 = r0 + chunk < a.rows ? r0 + chunk : a.rows;
+    for (int64_t row = r0 + grp; row < r1; row += CG) {
+        const float2 st = a.stats[row];
+        const float2 vs = PASS == 2 ? a.vstats[row] : make_float2(0.f, 0.f);
+        Vec<T, V> x, g, v;
+        const int64_t at = row * a.D + c0;
+        if (left >= V) {
+            x = ldv<T, V>((const T*)a.x + at);
+            g = ldv<T, V>((const T*)a.g + at);
+            if (PASS == 2) v = ldv<T, V>((const T*)a.v + at);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                x.e[e] = e < left ? ((const T*)a.x)[at + e] : (T)0.f;
+                g.e[e] = e < left ? ((const T*)a.g)[at + e] : (T)0.f;
+                if (PASS == 2) v.e[e] = e < left ? ((const T*)a.v)[at + e] : (T)0.f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float t = ((float)x.e[e] - st.x) * st.y, gv = (float)g.e[e];
+            if constexpr (PASS == 1) {
+                acc[0][e] = fmaf(gv, t, acc[0][e]);
+                acc[1][e] += gv;
+            } else {
+                acc[0][e] = fmaf(gv, st.y * ((float)v.e[e] - vs.x - t * vs.y), acc[0][e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            acc[j][e] += __shfl_xor(acc[j][e], 16);
+            acc[j][e] += __shfl_xor(acc[j][e], 32);
+            if ((threadIdx.x & 63) < 16) red[j][wave][lane * V + e] = acc[j][e];
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < NC * 16 * V; i += BLK) {
+        const int j = i / (16 * V), c = i % (16 * V), col = tile * 16 * V + c;
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < NW; ++k) s += red[j][k][c];
+        if (col < a.D) out[((int64_t)chunk_id * NC + j) * a.D + col] = s;
+    }
+}
+
+template <typename T, int PASS>
+__global__ void __launch_bounds__(TPB) ln_cols_k(const RowArgs a, float* __restrict__ out, int64_t chunk) {
+    col_sums<T, PASS, TPB>(a, out, chunk, blockIdx.x, blockIdx.y);
+}
+
 // ---- backward ----------------------------------------------------------------------------------------------------
-template <typename T, int TPR, int K, bool COLS>
+// COLS 1: column sums kept by the threads.  2: the workgroups behind `a.row_blocks` sum the columns down the rows (they need the
+// forward's statistics only), in the same launch.
+template <typename T, int TPR, int K, int COLS>
 __global__ void __launch_bounds__(block_of<TPR>()) ln_bwd_k(const RowArgs a) {
     constexpr int V = VecOf<T>::V, BLK = block_of<TPR>(), G = BLK / TPR;
+    if constexpr (COLS == 2) {
+        if ((int)blockIdx.x >= a.row_blocks) {
+            const int i = (int)blockIdx.x - a.row_blocks;
+            col_sums<T, 1, BLK>(a, a.part, a.chunk, i % a.col_tiles, i / a.col_tiles);
+            return;
+        }
+    }
     __shared__ float lds[2 * 2 * 16];
     int flip = 0;
     const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
-    const int D = a.D;
-    float w[K][V], acc[2][K][V];
-    load_cols<V, K, TPR>(a.w, 1.f, w, lane, D);
-    if (COLS) {
+    const int D = a.D, blocks = COLS == 2 ? a.row_blocks : (int)gridDim.x;
+    const Cols<V, K, TPR, (TPR < 512)> w(a.w, 1.f, lane, D);
+    float acc[2][COLS == 1 ? K : 1][V];
+    if (COLS == 1) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int e = 0; e < V; ++e) acc[0][k][e] = acc[1][k][e] = 0.f;
     }
     const float inv = 1.f / (float)D;
-    for (int64_t row = (int64_t)blockIdx.x * G + grp; row < a.rows; row += (int64_t)gridDim.x * G) {
+    for (int64_t row = (int64_t)blockIdx.x * G + grp; row < a.rows; row += (int64_t)blocks * G) {
         RowRegs<T, V, K, TPR> x, g;
         x.load((const T*)a.x + row * D, lane, D);
         g.load((const T*)a.g + row * D, lane, D);
         const float2 st = a.stats[row];
         float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            float wk[V];
+            w.get(k, lane, D, wk);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float gv = g.at(k, e), t = (x.at(k, e) - st.x) * st.y, h = gv * w[k][e];
+                const float gv = g.at(k, e), t = (x.at(k, e) - st.x) * st.y, h = gv * wk[e];
                 s[0] += h;
                 s[1] = fmaf(h, t, s[1]);
-                if (COLS) {
+                if (COLS == 1) {
                     acc[0][k][e] = fmaf(gv, t, acc[0][k][e]);
                     acc[1][k][e] += gv;
                 }
             }
+        }
         if (a.y) {
             row_sum<2, TPR>(s, lds, flip);
+            x.settle();
+            g.settle();
             const float s1 = s[0] * inv, s2 = s[1] * inv;
 #pragma unroll
-            for (int k = 0; k < K; ++k)
+            for (int k = 0; k < K; ++k) {
+                float wk[V];
+                w.get(k, lane, D, wk);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const float t = (x.at(k, e) - st.x) * st.y;
-                    g.v[k].e[e] = (T)(st.y * (g.at(k, e) * w[k][e] - s1 - t * s2));
+                    g.v[k].e[e] = (T)(st.y * (g.at(k, e) * wk[e] - s1 - t * s2));
                 }
+            }
             g.store((T*)a.y + row * D, lane, D);
         }
     }
-    if (COLS) write_partials<2, V, K, TPR>(acc, a.part, lane, grp, D);
+    if constexpr (COLS == 1) write_partials<2, V, K, TPR>(acc, a.part, lane, grp, D);
 }
 
 // ---- second order ------------------------------------------------------------------------------------------------
@@ -311,20 +434,21 @@ struct SecondRow {
     }
 };
 
-template <typename T, int TPR, int K, bool COLS, bool CC>  // CC: cotangents of the column sums are there
+template <typename T, int TPR, int K, int COLS, bool CC>  // CC: cotangents of the column sums are there
 __global__ void __launch_bounds__(block_of<TPR>()) ln_bwd2_k(const RowArgs a) {
     constexpr int V = VecOf<T>::V, BLK = block_of<TPR>(), G = BLK / TPR;
     __shared__ float lds[2 * NS2 * 16];
     int flip = 0;
     const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
     const int D = a.D;
-    float acc[1][K][V];
-    if (COLS) {
+    float acc[1][COLS == 1 ? K : 1][V];
+    if (COLS == 1) {
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int e = 0; e < V; ++e) acc[0][k][e] = 0.f;
     }
+    const Cols<V, K, TPR, false> w(a.w, 1.f, lane, D), cw(a.cw, 0.f, lane, D), cb(a.cb, 0.f, lane, D);
     const float inv = 1.f / (float)D;
     for (int64_t row = (int64_t)blockIdx.x * G + grp; row < a.rows; row += (int64_t)gridDim.x * G) {
         RowRegs<T, V, K, TPR> x, g, v;
@@ -332,34 +456,42 @@ __global__ void __launch_bounds__(block_of<TPR>()) ln_bwd2_k(const RowArgs a) {
         g.load((const T*)a.g + row * D, lane, D);
         v.load((const T*)a.v + row * D, lane, D);
         const float2 st = a.stats[row];
-        float w[K][V], cw[K][V], cb[K][V];
-        load_cols<V, K, TPR>(a.w, 1.f, w, lane, D);
-        if (CC) {
-            load_cols<V, K, TPR>(a.cw, 0.f, cw, lane, D);
-            load_cols<V, K, TPR>(a.cb, 0.f, cb, lane, D);
-        }
         float s[NS2] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            float wk[V], cwk[V];
+            w.get(k, lane, D, wk);
+            if (CC) cw.get(k, lane, D, cwk);
 #pragma unroll
-            for (int e = 0; e < V; ++e) second_sums(x.at(k, e), g.at(k, e), v.at(k, e), w[k][e], CC ? cw[k][e] : 0.f, st, s);
+            for (int e = 0; e < V; ++e) second_sums(x.at(k, e), g.at(k, e), v.at(k, e), wk[e], CC ? cwk[e] : 0.f, st, s);
+        }
         row_sum<NS2, TPR>(s, lds, flip);
+        x.settle();
+        g.settle();
+        v.settle();
         const SecondRow sr(st, s, inv);
         if (a.vstats && lane == 0) a.vstats[row] = make_float2(sr.vm, sr.vt);
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            float wk[V], cwk[V], cbk[V];
+            w.get(k, lane, D, wk);
+            if (CC) {
+                cw.get(k, lane, D, cwk);
+                cb.get(k, lane, D, cbk);
+            }
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 float gxx, gg, gw;
-                sr.at(x.at(k, e), g.at(k, e), v.at(k, e), w[k][e], CC ? cw[k][e] : 0.f, CC ? cb[k][e] : 0.f, gxx, gg, gw);
+                sr.at(x.at(k, e), g.at(k, e), v.at(k, e), wk[e], CC ? cwk[e] : 0.f, CC ? cbk[e] : 0.f, gxx, gg, gw);
                 x.v[k].e[e] = (T)gxx;
                 v.v[k].e[e] = (T)gg;
-                if (COLS) acc[0][k][e] += gw;
+                if (COLS == 1) acc[0][k][e] += gw;
             }
+        }
         if (a.y) v.store((T*)a.y + row * D, lane, D);
         if (a.y2) x.store((T*)a.y2 + row * D, lane, D);
     }
-    if (COLS) write_partials<1, V, K, TPR>(acc, a.part, lane, grp, D);
+    if constexpr (COLS == 1) write_partials<1, V, K, TPR>(acc, a.part, lane, grp, D);
 }
 
 // ---- long rows: pieces of a row sum, then join and write -----------------------------------------------------------
@@ -514,66 +646,6 @@ __global__ void __launch_bounds__(TPB) ln_long_apply_k(const RowArgs a) {
     }
 }
 
-// ---- column sums down the rows -------------------------------------------------------------------------------------
-// 16 lanes across a vector of columns each, 16 row groups; chunk blockIdx.y of the rows.  PASS 1: (g t, g), 2: g r P(v).
-// out: [chunks][NC][D].
-constexpr int CG = 16;
-
-template <typename T, int PASS>
-__global__ void __launch_bounds__(TPB) ln_cols_k(const RowArgs a, float* __restrict__ out, int64_t chunk) {
-    constexpr int V = VecOf<T>::V, NC = PASS == 1 ? 2 : 1;
-    __shared__ float red[NC][CG][16 * V];
-    const int lane = threadIdx.x & 15, grp = threadIdx.x >> 4;
-    const int c0 = (blockIdx.x * 16 + lane) * V;
-    const int left = a.D - c0;
-    float acc[NC][V];
-#pragma unroll
-    for (int j = 0; j < NC; ++j)
-#pragma unroll
-        for (int e = 0; e < V; ++e) acc[j][e] = 0.f;
-    const int64_t r0 = (int64_t)blockIdx.y * chunk, r1 = r0 + chunk < a.rows ? r0 + chunk : a.rows;
-    for (int64_t row = r0 + grp; row < r1; row += CG) {
-        const float2 st = a.stats[row];
-        const float2 vs = PASS == 2 ? a.vstats[row] : make_float2(0.f, 0.f);
-        Vec<T, V> x, g, v;
-        const int64_t at = row * a.D + c0;
-        if (left >= V) {
-            x = ldv<T, V>((const T*)a.x + at);
-            g = ldv<T, V>((const T*)a.g + at);
-            if (PASS == 2) v = ldv<T, V>((const T*)a.v + at);
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                x.e[e] = e < left ? ((const T*)a.x)[at + e] : (T)0.f;
-                g.e[e] = e < left ? ((const T*)a.g)[at + e] : (T)0.f;
-                if (PASS == 2) v.e[e] = e < left ? ((const T*)a.v)[at + e] : (T)0.f;
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float t = ((float)x.e[e] - st.x) * st.y, gv = (float)g.e[e];
-            if constexpr (PASS == 1) {
-                acc[0][e] = fmaf(gv, t, acc[0][e]);
-                acc[1][e] += gv;
-            } else {
-                acc[0][e] = fmaf(gv, st.y * ((float)v.e[e] - vs.x - t * vs.y), acc[0][e]);
-            }
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < NC; ++j)
-#pragma unroll
-        for (int e = 0; e < V; ++e) red[j][grp][lane * V + e] = acc[j][e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < NC * 16 * V; i += TPB) {
-        const int j = i / (16 * V), c = i % (16 * V), col = blockIdx.x * 16 * V + c;
-        float s = 0.f;
-#pragma unroll
-        for (int k = 0; k < CG; ++k) s += red[j][k][c];
-        if (col < a.D) out[((int64_t)blockIdx.y * NC + j) * a.D + col] = s;
-    }
-}
-
 // out[c] = sum_p part[p][c] over `n` partial rows of `width` columns, in a fixed order: 16 columns x 64 slices a workgroup.
 // The first `split` columns go to out0, the others to out1 (either may be NULL).
 __global__ void __launch_bounds__(1024) fold_cols_k(const float* __restrict__ part, int n, int64_t width, float* __restrict__ out0,
@@ -623,15 +695,15 @@ Plan plan_of(int64_t rows, int64_t D, int dtype, int pass, bool cols) {
     } else if (nv <= 512) {
         p.tpr = nv <= 128 ? 64 : 256;
         p.k = nv <= 128 || nv > 256 ? 2 : 1;
-    } else if (nv <= 2048) {
-        p.tpr = 512;
-        p.k = nv <= 1024 ? 2 : 4;
+    } else if (nv <= (pass == 2 ? 2048 : 4096)) {  // (three tensors of a row in 1024 threads' 128 registers spill)
+        p.tpr = nv <= 1024 || pass == 2 ? 512 : 1024;
+        p.k = nv <= 1024 || (nv <= 2048 && pass < 2) ? 2 : 4;
     }
     if (p.tpr) {
         const int g = p.tpr >= TPB ? 1 : TPB / p.tpr;
         const int64_t need = ceil_div64(rows, g);
         p.blocks = (int)(need < MAXB ? need : MAXB);
-        if (cols && pass > 0) {
+        if (cols && pass > 0 && p.tpr <= 512) {
             // A partial row of ncol D floats per workgroup is written and read again, next to at least three tensor rows of D
             // elements that a row costs anyway: few enough workgroups keep that under a sixth.  Where so few are left that
             // they would not fill the chip, a kernel down the columns reads the tensors a second time instead.
@@ -661,30 +733,35 @@ Plan plan_of(int64_t rows, int64_t D, int dtype, int pass, bool cols) {
     return p;
 }
 
-template <typename T, int PASS, bool COLS, int TPR, int K>
-void launch_row(const Plan& p, const RowArgs& a, hipStream_t st) {
+template <typename T, int PASS, int COLS, int TPR, int K>
+void launch_row(int blocks, const RowArgs& a, hipStream_t st) {
     constexpr int BLK = block_of<TPR>();
-    const size_t lds = COLS && TPR < TPB ? sizeof(float) * (PASS == 2 ? 1 : 2) * (size_t)a.D : 0;
+    const size_t lds = COLS == 1 && TPR < TPB ? sizeof(float) * (PASS == 2 ? 1 : 2) * (size_t)a.D : 0;
     if constexpr (PASS == 0)
-        hipLaunchKernelGGL((ln_fwd_k<T, TPR, K>), dim3(p.blocks), dim3(BLK), 0, st, a);
+        hipLaunchKernelGGL((ln_fwd_k<T, TPR, K>), dim3(blocks), dim3(BLK), 0, st, a);
     else if constexpr (PASS == 1)
-        hipLaunchKernelGGL((ln_bwd_k<T, TPR, K, COLS>), dim3(p.blocks), dim3(BLK), lds, st, a);
+        hipLaunchKernelGGL((ln_bwd_k<T, TPR, K, COLS>), dim3(blocks), dim3(BLK), lds, st, a);
     else if (a.cw || a.cb)
-        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS, true>), dim3(p.blocks), dim3(BLK), lds, st, a);
+        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS, true>), dim3(blocks), dim3(BLK), lds, st, a);
     else
-        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS, false>), dim3(p.blocks), dim3(BLK), lds, st, a);
+        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS, false>), dim3(blocks), dim3(BLK), lds, st, a);
 }
 
-template <typename T, int PASS, bool COLS>
-void launch_rows(const Plan& p, const RowArgs& a, hipStream_t st) {
+template <typename T, int PASS, int COLS>
+void launch_rows(const Plan& p, int blocks, const RowArgs& a, hipStream_t st) {
     switch (p.tpr * 8 + p.k) {
-        case 16 * 8 + 1: return launch_row<T, PASS, COLS, 16, 1>(p, a, st);
-        case 64 * 8 + 1: return launch_row<T, PASS, COLS, 64, 1>(p, a, st);
-        case 64 * 8 + 2: return launch_row<T, PASS, COLS, 64, 2>(p, a, st);
-        case 256 * 8 + 1: return launch_row<T, PASS, COLS, 256, 1>(p, a, st);
-        case 256 * 8 + 2: return launch_row<T, PASS, COLS, 256, 2>(p, a, st);
-        case 512 * 8 + 2: return launch_row<T, PASS, COLS, 512, 2>(p, a, st);
-        default: return launch_row<T, PASS, COLS, 512, 4>(p, a, st);
+        case 16 * 8 + 1: return launch_row<T, PASS, COLS, 16, 1>(blocks, a, st);
+        case 64 * 8 + 1: return launch_row<T, PASS, COLS, 64, 1>(blocks, a, st);
+        case 64 * 8 + 2: return launch_row<T, PASS, COLS, 64, 2>(blocks, a, st);
+        case 256 * 8 + 1: return launch_row<T, PASS, COLS, 256, 1>(blocks, a, st);
+        case 256 * 8 + 2: return launch_row<T, PASS, COLS, 256, 2>(blocks, a, st);
+        case 512 * 8 + 2: return launch_row<T, PASS, COLS, 512, 2>(blocks, a, st);
+    }
+    if constexpr (PASS == 2) {
+        launch_row<T, PASS, COLS, 512, 4>(blocks, a, st);
+    } else if constexpr (COLS != 1) {
+        if (p.k == 2) launch_row<T, PASS, COLS, 1024, 2>(blocks, a, st);
+        else launch_row<T, PASS, COLS, 1024, 4>(blocks, a, st);
     }
 }
 
@@ -699,7 +776,7 @@ int run_pass(const Plan& p, RowArgs a, float* gw, float* gb, float* ws, hipStrea
         if (p.fused) {
             a.part = at;
             at += (int64_t)p.blocks * NC * D;
-            if constexpr (PASS > 0) launch_rows<T, PASS, true>(p, a, st);
+            if constexpr (PASS > 0) launch_rows<T, PASS, 1>(p, p.blocks, a, st);
             GAN_CHECK_LAUNCH("layernorm");
             hipLaunchKernelGGL(fold_cols_k, dim3((unsigned)ceil_div64(NC * D, 16)), dim3(1024), 0, st, a.part, p.blocks, (int64_t)NC * D, gw, gb, D);
             GAN_CHECK_LAUNCH("layernorm(fold)");
@@ -716,9 +793,24 @@ int run_pass(const Plan& p, RowArgs a, float* gw, float* gb, float* ws, hipStrea
         a.vstats = (float2*)at;
         at += 2 * a.rows;
     }
+    bool summed = !cols;
+    float* const sums = p.chunks > 1 ? at : gw;  // one chunk: the kernel's [NC][D] are the gradients
     if (rows_out) {
         if (p.tpr) {
-            launch_rows<T, PASS, false>(p, a, st);
+            if constexpr (PASS == 1) {
+                if (cols) {  // the columns in the same launch: tiles of them behind the rows' workgroups
+                    a.row_blocks = p.blocks;
+                    a.col_tiles = (int)ceil_div64(D, 16 * VecOf<T>::V);
+                    a.chunk = p.chunk;
+                    a.part = sums;
+                    launch_rows<T, 1, 2>(p, p.blocks + a.col_tiles * p.chunks, a, st);
+                    summed = true;
+                } else {
+                    launch_rows<T, 1, 0>(p, p.blocks, a, st);
+                }
+            } else {
+                launch_rows<T, PASS, 0>(p, p.blocks, a, st);
+            }
         } else {
             const dim3 grid((unsigned)(a.rows * p.pieces));
             hipLaunchKernelGGL((ln_long_sum_k<T, PASS>), grid, dim3(TPB), 0, st, a);
@@ -728,16 +820,14 @@ int run_pass(const Plan& p, RowArgs a, float* gw, float* gb, float* ws, hipStrea
         GAN_CHECK_LAUNCH("layernorm(rows)");
     }
     if constexpr (PASS > 0) {
-        if (cols) {
-            constexpr int V = VecOf<T>::V;
-            const dim3 grid((unsigned)ceil_div64(D, 16 * V), (unsigned)p.chunks);
-            // with one chunk the kernel writes [NC][D]: straight into a gradient pair that lies so, else through the fold
-            hipLaunchKernelGGL((ln_cols_k<T, PASS>), grid, dim3(TPB), 0, st, a, p.chunks > 1 ? at : gw, p.chunk);
+        if (!summed) {
+            const dim3 grid((unsigned)ceil_div64(D, 16 * VecOf<T>::V), (unsigned)p.chunks);
+            hipLaunchKernelGGL((ln_cols_k<T, PASS>), grid, dim3(TPB), 0, st, a, sums, p.chunk);
             GAN_CHECK_LAUNCH("layernorm(columns)");
-            if (p.chunks > 1) {
-                hipLaunchKernelGGL(fold_cols_k, dim3((unsigned)ceil_div64(NC * D, 16)), dim3(1024), 0, st, at, p.chunks, (int64_t)NC * D, gw, gb, D);
-                GAN_CHECK_LAUNCH("layernorm(fold)");
-            }
+        }
+        if (cols && p.chunks > 1) {
+            hipLaunchKernelGGL(fold_cols_k, dim3((unsigned)ceil_div64(NC * D, 16)), dim3(1024), 0, st, sums, p.chunks, (int64_t)NC * D, gw, gb, D);
+            GAN_CHECK_LAUNCH("layernorm(fold)");
         }
     }
     return GAN_OK;

@@ -361,6 +361,40 @@ def test_norm_penalty_and_step_together(dev):
                 assert rel_err(q, p) < 1e-4, k
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("hip_graph", [False, True])
+def test_trainer_with_muon(dev, hip_graph, tmp_path):
+    """TrainConfig(optimizer="Muon"): the train step runs, eager and as HIP graphs, and a checkpoint continues with the same
+    optimizer state."""
+    from gan_amd.optim import FlatMuon
+    from gan_amd.train_celeba import TrainConfig, Trainer
+
+    torch.manual_seed(1)
+    cfg = TrainConfig(model="dcgan", img_size=32, gen_kwargs={"base_dim": 16}, disc_kwargs={"base_dim": 16, "norm": "none"}, method="wgan",
+                      regularizer="wgan-gp", batch_size=8, optimizer="Muon", optimizer_kwargs={"weight_decay": 0.0, "adam_lr": 1e-4}, lr=2e-3,
+                      device="cuda", mixed_precision=True, hip_graph=hip_graph, graph_warmup=2)
+    reals = torch.randn(8, 3, 32, 32, device=dev)
+    a = Trainer(cfg, dev)
+    assert isinstance(a.optim_d, FlatMuon) and isinstance(a.optim_g, FlatMuon)
+    before = [p.detach().clone() for p in a.gen.parameters()]
+    for _ in range(5):
+        logs = a.train_step(lambda: reals)
+        assert all(math.isfinite(float(v)) for v in logs.values())
+    assert (a._graph is not None) == hip_graph and a.cfg.hip_graph == hip_graph  # (a capture that fails falls back)
+    assert all(torch.isfinite(p).all() for p in a.disc.parameters())
+    assert not any(torch.equal(p, q) for p, q in zip(a.gen.parameters(), before))
+    path = str(tmp_path / "c.pt")
+    a.save_checkpoint(path)
+    b = Trainer(cfg, dev)
+    b.load_checkpoint(path)
+    for x, y in ((a.optim_g, b.optim_g), (a.optim_d, b.optim_d)):
+        # (the arenas' padding between parameters belongs to no state)
+        for p, q in zip(x.arena.params, y.arena.params):
+            assert torch.equal(p, q)
+            assert all(torch.equal(x.state[p][k], y.state[q][k]) for k in x.state[p])
+    b.train_step(lambda: reals)
+
+
 def test_refusals():
     from gan_amd import _lib
     from gan_amd import functional as GF
