@@ -7,6 +7,9 @@
 // a third of the dense 2.5 PFLOP/s; fp32 matrix instructions stop at 0.16.
 // All matrices of a call share the launches (one per product), their tiles side by side in the grid; A and P are symmetric,
 // only the tiles on and above the diagonal are computed and the others mirrored.
+#include <type_traits>
+#include <utility>
+
 #include "common.h"
 
 namespace {
@@ -31,6 +34,20 @@ __device__ __forceinline__ void split(float v, h16& hi, h16& lo) {
     lo = (h16)(v - (float)hi);
 }
 
+// eight values to the two planes
+__device__ __forceinline__ void store_planes(h16* to, int64_t plane, const float (&o)[8]) {
+    h16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        h16 p, w;
+        split(o[e], p, w);
+        hi[e] = p;
+        lo[e] = w;
+    }
+    *(h16x8*)to = hi;
+    *(h16x8*)(to + plane) = lo;
+}
+
 // elements of one partial sum of squares
 __host__ __device__ inline int64_t chunk_of(int64_t size) {
     const int64_t c = (size + MAXPARTS - 1) / MAXPARTS;
@@ -44,7 +61,7 @@ struct Mat {
     float* buf;      // momentum (NULL: orthogonalise g itself)
     char* ws;        // workspace of the first
     int64_t stride;
-    int64_t nat, tra;  // offsets of the planes that lie as the source does, and transposed
+    int64_t x;       // offset of the planes
     int rows, cols;
 };
 
@@ -61,22 +78,23 @@ struct Mats {
     Mat mat[NOPS];
 };
 
-// Byte offsets in one matrix's workspace: the partial sums, two X (each [m][n] and [n][m], hi plane then lo plane), five
+// Byte offsets in one matrix's workspace: the partial sums, two X ([m][n], hi plane then lo plane), five
 // symmetric m x m, the slices' tiles of a product that is cut.  All multiples of 256.
 enum { A0, A1, P0, P1, Q0, SQUARES };
 struct Lay {
-    int64_t mp, np, nparts, xm[2], xt[2], sq[SQUARES], join, bytes;
+    int64_t mp, np, nparts, x[2], sq[SQUARES], join, bytes;
     int cut;
 };
 
 // What a product of `tiles` T x T tiles over `steps` steps of 32 k takes, in us, every tile's k in `cut` slices: workgroups run
-// in rounds, 256 (T = 256) or 512 of them at a time, a step of theirs as long as measured (T = 256: 2.8; T = 128: 0.48 alone
+// in rounds, 256 (T = 256) or 512 of them at a time, a step of theirs as long as measured (T = 256: 2.8; T = 128: 0.55 alone
 // on a CU, 0.8 each where two share it; T = 64: 0.2 and 0.25), a round begins and ends in 5 to 9 us, and slices are written and
 // read again at 5 TB/s by one more launch.
 double cost_of(int T, int64_t tiles, int cut, int64_t steps) {
-    const int64_t wgs = tiles * cut, slots = T < 256 && wgs > 256 ? 512 : 256;
-    const double alone = T == 256 ? 2.8 : T == 128 ? 0.48 : 0.2, shared = T == 128 ? 1.6 : 0.5, ends = T == 256 ? 9. : T == 128 ? 7. : 5.;
-    return (double)ceil_div64(wgs, slots) * ((double)ceil_div64(steps, cut) * (slots == 512 ? shared : alone) + ends) +
+    const int64_t wgs = tiles * cut, slots = T < 256 && wgs > 256 ? 512 : 256, left = wgs % slots;
+    const double alone = T == 256 ? 2.8 : T == 128 ? 0.55 : 0.2, shared = T == 128 ? 1.6 : 0.5, ends = T == 256 ? 9. : T == 128 ? 7. : 5.;
+    const double n = (double)ceil_div64(steps, cut);
+    return (double)(wgs / slots) * (n * (slots == 512 ? shared : alone) + ends) + (left ? n * (left > 256 ? shared : alone) + ends : 0.) +
            (cut > 1 ? 5. + (double)wgs * T * T * 8e-6 / 5. : 0.);
 }
 
@@ -113,9 +131,7 @@ Lay lay_of(int64_t rows, int64_t cols) {
     int64_t at = MAXPARTS * 8;
     const int64_t x = l.mp * l.np * 4, sq = l.mp * l.mp * 4;
     for (int k = 0; k < 2; ++k) {
-        l.xm[k] = at;
-        at += x;
-        l.xt[k] = at;
+        l.x[k] = at;
         at += x;
     }
     for (int k = 0; k < SQUARES; ++k) {
@@ -209,7 +225,7 @@ __device__ __forceinline__ float scale_of(const double* part, int nparts, float 
     return n < 1e300 ? (float)((double)SX / (n > (double)eps ? n : (double)eps)) : __builtin_nanf("");
 }
 
-// ---- the scaled source as two planes, [rows][cols] and [cols][rows], padded with zeros ---------------------------------
+// ---- the scaled source as two planes [m][n], padded with zeros (a tall source transposed) ------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
     __shared__ float tile[64][65];
@@ -241,40 +257,30 @@ __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
         tile[r][c] = in ? scale * (buf ? update_of(s.from, v[k], m[k]) : v[k]) : 0.f;
     }
     __syncthreads();
-    h16 *nat = (h16*)(ws + q.nat), *tra = (h16*)(ws + q.tra);
+    h16* to = (h16*)(ws + q.x);
     const int64_t plane = (int64_t)rp * cp;
+    const bool wide = q.rows <= q.cols;
     for (int k = threadIdx.x; k < 64 * 8; k += 256) {
         const int r = k >> 3, c = (k & 7) * 8;
-        h16x8 hi, lo, thi, tlo;
+        float o[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            h16 x, y;
-            split(tile[r][c + e], x, y);
-            hi[e] = x;
-            lo[e] = y;
-            split(tile[c + e][r], x, y);
-            thi[e] = x;
-            tlo[e] = y;
-        }
-        const int64_t at = (int64_t)(r0 + r) * cp + c0 + c, ta = (int64_t)(c0 + r) * rp + r0 + c;
-        *(h16x8*)(nat + at) = hi;
-        *(h16x8*)(nat + plane + at) = lo;
-        *(h16x8*)(tra + ta) = thi;
-        *(h16x8*)(tra + plane + ta) = tlo;
+        for (int e = 0; e < 8; ++e) o[e] = wide ? tile[r][c + e] : tile[c + e][r];
+        store_planes(to + (wide ? (int64_t)(r0 + r) * cp + c0 + c : (int64_t)(c0 + r) * rp + r0 + c), plane, o);
     }
 }
 
 // ---- products ----------------------------------------------------------------------------------------------------------
 enum Kind { SCALED, POLY, RESULT };
 
-// C = U V' of one group of equal matrices
+// C = U V' (or U V) of one group of equal matrices
 struct Op {
     char* ws;          // of the group's first matrix
     int64_t stride;
     void* out;         // RESULT
-    unsigned u, v;     // operands, results [i][j] and [j][i], POLY's A, slices: in 256 bytes from ws
-    unsigned dn, dt, aux, join;
-    int M, N, K;       // padded; symmetric results (dn == dt) have tiles on and above the diagonal only
+    unsigned u, v;     // operands, result, POLY's A, slices: in 256 bytes from ws
+    unsigned to, aux, join;
+    int M, N, K;       // padded
+    int apply;         // C = U V with V [K][N] as it lies, not transposed; else C is symmetric: tiles on and above the diagonal
     int rows, cols;    // of the source
     int tiles;         // per matrix
     int cut, steps;    // slices of k, steps of 32 k in each but the last
@@ -292,7 +298,7 @@ struct Rule {
 struct Ops {
     int count;
     Rule rule;
-    int first[NOPS];  // each group's first workgroup
+    int first[NOPS + 1];  // each group's first workgroup, and behind the last
     Op mat[NOPS];
 };
 
@@ -309,24 +315,10 @@ __device__ __forceinline__ int2 tile_of(int t, int n) {
 }
 
 // A wave's 32 x 32 block of a product at (i0, j0), as accumulated: lane holds column lane & 31, rows 8 (r / 4) + 4 (lane >> 5) +
-// r % 4.  It goes through `t` (the wave's own LDS) once, so that both the block and its transpose are stored 16 bytes a lane.
-// mirror: the transposed place is another block's (of a symmetric result).
+// r % 4.  It goes through `t` (the wave's own LDS) once, so that the block and, of a symmetric result, its transpose (mirror: where
+// that is another block's place) are stored 16 bytes a lane.
 constexpr int TLD = 36;  // floats a row: 16-byte rows, and columns of eight spread over the banks
 constexpr int TBYTES = 32 * TLD * 4;
-
-// eight values to the two planes
-__device__ __forceinline__ void store_planes(h16* to, int64_t plane, const float (&o)[8]) {
-    h16x8 hi, lo;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        h16 p, w;
-        split(o[e], p, w);
-        hi[e] = p;
-        lo[e] = w;
-    }
-    *(h16x8*)to = hi;
-    *(h16x8*)(to + plane) = lo;
-}
 
 // eight values of a row of the result, `left` of them inside it: stored, or taken off the parameters there
 template <typename T>
@@ -402,27 +394,49 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int 
         }
         return;
     }
-    h16 *dn = (h16*)(ws + (int64_t)q.dn * 256), *dt = (h16*)(ws + (int64_t)q.dt * 256);  // [i][j] and [j][i]
+    h16* to = (h16*)(ws + (int64_t)q.to * 256);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) store_planes(dn + (int64_t)(i0 + h * 16 + a) * q.N + j0 + c, plane, o[h]);
+    for (int h = 0; h < 2; ++h) store_planes(to + (int64_t)(i0 + h * 16 + a) * q.N + j0 + c, plane, o[h]);
     if (mirror) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) store_planes(dt + (int64_t)(j0 + h * 16 + a) * q.M + i0 + c, plane, x[h]);
+        for (int h = 0; h < 2; ++h) store_planes(to + (int64_t)(j0 + h * 16 + a) * q.N + i0 + c, plane, x[h]);
     }
 }
 
-// an address that is the same in every lane, in scalar registers
+// An address that is the same in every lane, in scalar registers.  (Five wait states lie between a vector instruction's write of a
+// scalar register and its use by a memory instruction; the compiler does not see the one in ortho_issue.)
 __device__ __forceinline__ const char* scalar(const char* p) {
     const uint64_t v = (uint64_t)p;
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+    uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+    asm volatile("s_nop 4" : "+s"(lo), "+s"(hi));
     return (const char*)(((uint64_t)hi << 32) | lo);
 }
-// One LDS-DMA instruction: a wave's instruction j covers 1 KB = 16 rows of plane j / PP of the stage of k step `step` at `base`.
-// p: the planes' first rows.
+
+// One LDS-DMA instruction: a wave's instruction j covers 1 KB of plane j / PP of the stage at `base`.  p: the planes' first bytes,
+// at: the stage's bytes from there in U and in V.  Written out, since the compiler would wait for every request on its way in
+// front of any transposing read of LDS (it cannot tell the stages apart); stage_arrived() waits for what is needed.
 template <int WAVES, int PP>
-__device__ __forceinline__ void ortho_issue(char* base, int step, int wave, const char* const* p, const unsigned* off, int j) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(__builtin_amdgcn_make_buffer_rsrc((void*)p[j / PP], 0, 0xffffffffu, 0x00020000),
-                                             (__attribute__((address_space(3))) void*)(base + (WAVES * j + wave) * 1024), 16, off[j], step * 64, 0, 0);
+__device__ __forceinline__ void ortho_issue(char* base, unsigned at_u, unsigned at_v, int wave, const char* const* p, const unsigned* off, int j) {
+    typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+    const uint64_t from = (uint64_t)p[j / PP];
+    const u32x4 rsrc = {(unsigned)from, (unsigned)(from >> 32), 0xffffffffu, 0x00020000u};
+    const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)(base + (WAVES * j + wave) * 1024);
+    const unsigned at = j / PP < 2 ? at_u : at_v;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(off[j]), "s"(rsrc), "s"(at) : "m0");
+}
+
+// Four rows of 32 columns (64 bytes) are read at a time from a [32][T] stage: where in its row a row's lie, so that the four fill
+// the 64 banks (T = 64: two rows fill them already).  Without: 24.8 -> 33 us for a product of 26 steps.
+template <int T>
+__device__ __forceinline__ int v_swizzle(int row) {
+    return T == 64 ? (row & 2) << 1 : (row & 3) << 2;
+}
+
+// Of four rows (k) of sixteen elements, lane i of sixteen brings the four at (row i / 4, columns 4 (i % 4) ...) and takes column
+// i of the four rows.
+__device__ __forceinline__ h16x4 read_transposed(const char* p) {
+    typedef __attribute__((ext_vector_type(4))) short s16x4;
+    return __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
 // The fragments of 16 k of a wave's tile, from the stage at `base`: rows m0 ... of U, n0 ... of V
@@ -430,9 +444,20 @@ template <int FM, int FN>
 struct Frags {
     static constexpr int READS = 2 * (FM + FN), PRODUCTS = 3 * FM * FN;
     h16x8 u[2][FM], v[2][FN];  // hi, lo
-    __device__ __forceinline__ void read(const char* base, int plane, int m0, int n0, int half, int lane, int r) {
+    // APPLY: V's stage is [32 k][T], 16 columns of it at a time turned round on the way
+    template <int T, bool APPLY>
+    __device__ __forceinline__ void read(const char* base, int m0, int n0, int half, int lane, int r) {
+        constexpr int plane = T * 64;
         const bool of_u = r < 2 * FM;
         const int f = (of_u ? r : r - 2 * FM) >> 1, pl = r & 1, ch = half * 2 + (lane >> 5);
+        if (APPLY && !of_u) {
+            const int row = half * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);
+            const int chunk = (n0 + f * 32 + (lane & 16)) / 8 + ((lane & 3) >> 1);
+            const char* p = base + (2 + pl) * plane + row * (T * 2) + ((chunk ^ v_swizzle<T>(row)) << 4) + (lane & 1) * 8;
+            const h16x4 a = read_transposed(p), b = read_transposed(p + 4 * (T * 2));
+            v[pl][f] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+            return;
+        }
         const int row = (of_u ? m0 : n0) + f * 32 + (lane & 31), at = row * 64 + ((ch ^ ((row >> 2) & 3)) << 4);
         const h16x8 got = *(const h16x8*)(base + (of_u ? pl : 2 + pl) * plane + at);
         if (of_u) u[pl][f] = got;
@@ -464,9 +489,10 @@ constexpr int gemm_threads() {
     return T == 256 ? 512 : 256;
 }
 
-// Tile T x T of C = U V': four waves of T/2 x T/2, or eight of 128 x 64.  U [M][K], V [N][K], each a hi plane and a lo plane;
-// K % 32 == 0.  Stages of 32 k (64 bytes a row) go to LDS by DMA, chunk c of row r at position c ^ ((r >> 2) & 3): the 16 rows
-// that a fragment read touches at a time then lie in different banks.
+// Tile T x T of C = U V' or U V: four waves of T/2 x T/2, or eight of 128 x 64.  U [M][K], V [N][K] or [K][N], each a hi plane and
+// a lo plane; K % 32 == 0.  Stages of 32 k go to LDS by DMA.  Of a plane with k along its rows a stage holds 64 bytes a row, chunk
+// c of row r at position c ^ ((r >> 2) & 3): the 16 rows that a fragment read touches at a time then lie in different banks.  Of
+// [K][N] it holds 32 rows of T, chunk c of row r at c ^ v_swizzle(r).
 template <int T, int NST>
 __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm_k(const Ops s, int dtype) {
     constexpr int WAVES = gemm_threads<T>() / 64, WN = WAVES / 2;  // waves: 2 x WN
@@ -475,45 +501,50 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
     constexpr int PER = STAGE / 1024 / WAVES;                      // DMA instructions per wave and stage
     constexpr int PP = PER / 4;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
-    // Workgroups go round the eight dies, each with a cache of its own: a die gets a run of them.  Tiles follow one another along
-    // the rows of U, sharing their rows of V, and a slice's tiles lie together.
-    const int each = gridDim.x >> 3, rest = gridDim.x & 7, die = blockIdx.x & 7;
-    const int id = die * each + (die < rest ? die : rest) + ((int)blockIdx.x >> 3);
-    const int group = group_of(s, id);
+    const int group = group_of(s, blockIdx.x);
     const Op q = s.mat[group];  // (a copy: one batch of scalar loads)
+    // Workgroups go round the eight dies, each with a cache of its own: of each group's, a die gets a run.  Tiles follow one
+    // another along the rows of U, sharing their rows of V, and a slice's tiles lie together.
+    const int all = s.first[group + 1] - s.first[group], local = (int)blockIdx.x - s.first[group];
+    const int each = all >> 3, rest = all & 7, die = local & 7;
+    const int id = die * each + (die < rest ? die : rest) + (local >> 3);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
     // (divisions run on vector registers: say that the results are the wave's, or every use of an address loops over lanes)
     const int per = q.tiles * q.cut;
-    const int b = __builtin_amdgcn_readfirstlane((id - s.first[group]) / per);
-    const int in_b = id - s.first[group] - b * per;
+    const int b = __builtin_amdgcn_readfirstlane(id / per);
+    const int in_b = id - b * per;
     const int slice = __builtin_amdgcn_readfirstlane(in_b / q.tiles), tile = in_b - slice * q.tiles;
     char* ws = q.ws + b * q.stride;
     const char *u = ws + (int64_t)q.u * 256, *v = ws + (int64_t)q.v * 256;
     const int M = q.M, N = q.N, K = q.K;
-    const bool sym = q.kind != RESULT && q.dn == q.dt;
     int ti, tj;
-    if (sym) {
-        const int2 t = tile_of(tile, (M + T - 1) / T);
-        ti = t.x;
-        tj = t.y;
-    } else {
+    if (q.apply) {
         const int tm = (M + T - 1) / T;
         tj = __builtin_amdgcn_readfirstlane(tile / tm);
         ti = tile - tj * tm;
+    } else {
+        const int2 t = tile_of(tile, (M + T - 1) / T);
+        ti = t.x;
+        tj = t.y;
     }
     const int i0 = ti * T, j0 = tj * T;
     // ---- staging: a wave's instruction j covers 1 KB of the stage = 16 rows of one plane
-    const unsigned kb = (unsigned)K * 2;
+    const unsigned kb = (unsigned)K * 2, nb = (unsigned)N * 2;
+    const unsigned v_step = q.apply ? 32 * nb : 64;
     unsigned off[PER];
-    const int rsub = lane >> 2, pos = lane & 3;
-    const char* const planes[4] = {scalar(u + (int64_t)i0 * kb), scalar(u + ((int64_t)M + i0) * kb), scalar(v + (int64_t)j0 * kb),
-                                   scalar(v + ((int64_t)N + j0) * kb)};
+    const char* const v0 = v + (q.apply ? (int64_t)j0 * 2 : (int64_t)j0 * kb);
+    const char* const planes[4] = {scalar(u + (int64_t)i0 * kb), scalar(u + ((int64_t)M + i0) * kb), scalar(v0), scalar(v0 + (int64_t)N * kb)};
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const int piece = WAVES * j + wave, pl = piece / (T / 16), row = piece % (T / 16) * 16 + rsub;
-        // rows past the matrix (T = 128 over an odd number of 64s): the last row again, their results are not stored
-        const int lim = pl < 2 ? M - i0 : N - j0;
-        off[j] = (unsigned)(row < lim ? row : lim - 1) * kb + (unsigned)((pos ^ ((row >> 2) & 3)) * 16);
+        const int piece = WAVES * j + wave, pl = piece / (T / 16), at = piece % (T / 16) * 1024 + lane * 16;
+        // rows (columns) past the matrix (T = 128 over an odd number of 64s): the last again, their results are not stored
+        if (pl < 2 || !q.apply) {
+            const int row = at / 64, pos = at % 64 / 16, lim = pl < 2 ? M - i0 : N - j0;
+            off[j] = (unsigned)(row < lim ? row : lim - 1) * kb + (unsigned)((pos ^ ((row >> 2) & 3)) * 16);
+        } else {
+            const int row = at / (T * 2), pos = at % (T * 2) / 16, col = (pos ^ v_swizzle<T>(row)) * 8, lim = N - j0 - 8;
+            off[j] = (unsigned)row * nb + (unsigned)(col < lim ? col : lim) * 2;
+        }
     }
     using Fr = Frags<FM, FN>;
     f32x16 sums[Fr::NACC][FM][FN];
@@ -526,11 +557,14 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
 #pragma unroll
                 for (int r = 0; r < 16; ++r) sums[a][x][y][r] = 0.f;
     const int k0 = slice * q.steps, nk = (K / 32 - k0 < q.steps ? K / 32 - k0 : q.steps);
+    auto issue = [&](char* base, int step, int j) __attribute__((always_inline)) {
+        ortho_issue<WAVES, PP>(base, (unsigned)(k0 + step) * 64, (unsigned)(k0 + step) * v_step, wave, planes, off, j);
+    };
 #pragma unroll
     for (int k = 0; k < NST; ++k)
         if (k < nk) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) ortho_issue<WAVES, PP>(lds + k * STAGE, k0 + k, wave, planes, off, j);
+            for (int j = 0; j < PER; ++j) issue(lds + k * STAGE, k, j);
         }
     // While the matrix instructions of one half of a stage (16 k) run, the other half's fragments are read and DMA is asked for,
     // a piece behind each: eight requests in a row would hold the wave at the address unit (64 bytes a clock for the CU) for as
@@ -539,53 +573,56 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
     // the next half's turn.
     constexpr int HALF = PER / 2;
     const int m0 = wm * (T / 2), n0 = wn * (T / WN);
-    Fr f0, f1;
-    stage_arrived<(NST - 1) * PER>(nk >= NST);
+    auto walk = [&](auto apply) __attribute__((always_inline)) {
+        constexpr bool APPLY = decltype(apply)::value;
+        Fr f0, f1;
+        stage_arrived<(NST - 1) * PER>(nk >= NST);
 #pragma unroll
-    for (int r = 0; r < Fr::READS; ++r) f0.read(lds, PLANE, m0, n0, 0, lane, r);
-    auto step = [&](int k, bool late, bool more) __attribute__((always_inline)) {
-        char *here = lds + k % NST * STAGE, *last = lds + (k + NST - 1) % NST * STAGE, *next = lds + (k + 1) % NST * STAGE;
+        for (int r = 0; r < Fr::READS; ++r) f0.template read<T, APPLY>(lds, m0, n0, 0, lane, r);
+        auto step = [&](int k, bool late, bool more) __attribute__((always_inline)) {
+            char *here = lds + k % NST * STAGE, *last = lds + (k + NST - 1) % NST * STAGE, *next = lds + (k + 1) % NST * STAGE;
 #pragma unroll
-        for (int i = 0; i < Fr::PRODUCTS; ++i) {
-            f0.multiply(sums, i);
+            for (int i = 0; i < Fr::PRODUCTS; ++i) {
+                f0.multiply(sums, i);
 #pragma unroll
-            for (int r = 0; r < Fr::READS; ++r)
-                if (r * Fr::PRODUCTS / (2 * Fr::READS) == i) f1.read(here, PLANE, m0, n0, 1, lane, r);
-            if (late) {
+                for (int r = 0; r < Fr::READS; ++r)
+                    if (r * Fr::PRODUCTS / (2 * Fr::READS) == i) f1.template read<T, APPLY>(here, m0, n0, 1, lane, r);
+                if (late) {
 #pragma unroll
-                for (int j = 0; j < HALF; ++j)
-                    if ((j + 1) * Fr::PRODUCTS / HALF - 1 == i) ortho_issue<WAVES, PP>(last, k0 + k - 1 + NST, wave, planes, off, HALF + j);
+                    for (int j = 0; j < HALF; ++j)
+                        if ((j + 1) * Fr::PRODUCTS / HALF - 1 == i) issue(last, k - 1 + NST, HALF + j);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        stage_arrived<(NST - 2) * PER>(k + NST - 1 < nk);  // stages k + 2 ... k + NST - 1 behind it
+            stage_arrived<(NST - 2) * PER>(k + NST - 1 < nk);  // stages k + 2 ... k + NST - 1 behind it
 #pragma unroll
-        for (int i = 0; i < Fr::PRODUCTS; ++i) {
-            f1.multiply(sums, i);
+            for (int i = 0; i < Fr::PRODUCTS; ++i) {
+                f1.multiply(sums, i);
 #pragma unroll
-            for (int r = 0; r < Fr::READS; ++r)
-                if (r * Fr::PRODUCTS / (2 * Fr::READS) == i) f0.read(next, PLANE, m0, n0, 0, lane, r);
-            if (more) {
+                for (int r = 0; r < Fr::READS; ++r)
+                    if (r * Fr::PRODUCTS / (2 * Fr::READS) == i) f0.template read<T, APPLY>(next, m0, n0, 0, lane, r);
+                if (more) {
 #pragma unroll
-                for (int j = 0; j < HALF; ++j)
-                    if ((j + 1) * Fr::PRODUCTS / HALF - 1 == i) ortho_issue<WAVES, PP>(here, k0 + k + NST, wave, planes, off, j);
+                    for (int j = 0; j < HALF; ++j)
+                        if ((j + 1) * Fr::PRODUCTS / HALF - 1 == i) issue(here, k + NST, j);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    if (nk > 1) step(0, false, NST < nk);
-    int k = 1;
-    for (; k + NST < nk; ++k) step(k, true, true);
-    for (; k + 1 < nk; ++k) step(k, k - 1 + NST < nk, false);
-    {
+        };
+        if (nk > 1) step(0, false, NST < nk);
+        int k = 1;
+        for (; k + NST < nk; ++k) step(k, true, true);
+        for (; k + 1 < nk; ++k) step(k, k - 1 + NST < nk, false);
         const char* here = lds + (nk - 1) % NST * STAGE;
 #pragma unroll
-        for (int r = 0; r < Fr::READS; ++r) f1.read(here, PLANE, m0, n0, 1, lane, r);
+        for (int r = 0; r < Fr::READS; ++r) f1.template read<T, APPLY>(here, m0, n0, 1, lane, r);
 #pragma unroll
         for (int i = 0; i < Fr::PRODUCTS; ++i) f0.multiply(sums, i);
 #pragma unroll
         for (int i = 0; i < Fr::PRODUCTS; ++i) f1.multiply(sums, i);
-    }
+    };
+    if (q.apply) walk(std::true_type{});
+    else walk(std::false_type{});
     f32x16(&acc)[FM][FN] = sums[0];
     if (Fr::NACC == 3) {
 #pragma unroll
@@ -613,7 +650,7 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
         for (int k = 1; k < FM * FN; ++k)
             if (f == k) one = acc[k / FN][k % FN];
         const int i = i0 + wm * (T / 2) + f / FN * 32, j = j0 + wn * (T / WN) + f % FN * 32;
-        if (i < M && j < N) finish(s, q, ws, b, i, j, one, !sym || ti != tj, dtype, t);
+        if (i < M && j < N) finish(s, q, ws, b, i, j, one, !q.apply && ti != tj, dtype, t);
     }
 }
 
@@ -689,7 +726,8 @@ struct Walk {
         auto mul = [&](int u, int v, int to, float gain) {
             q.u = sq(u);
             q.v = sq(v);
-            q.dn = q.dt = sq(to);
+            q.to = sq(to);
+            q.apply = 0;
             q.gain = gain;
             q.M = q.N = q.K = (int)l.mp;
         };
@@ -699,16 +737,16 @@ struct Walk {
         const int last = size == 1 ? 2 : 6;
         if (at == 0) {
             mul(0, 0, A0, SA / (SX * SX));
-            q.u = q.v = (unsigned)(l.xm[cur] / 256);
+            q.u = q.v = (unsigned)(l.x[cur] / 256);
             q.K = (int)l.np;
             q.cut = l.cut;
         } else if (at == last) {
             const bool end = left == size;
             q.kind = end ? RESULT : SCALED;
             q.u = sq(size == 1 ? P0 : Q0);
-            q.v = (unsigned)(l.xt[cur] / 256);
-            q.dn = (unsigned)(l.xm[cur ^ 1] / 256);
-            q.dt = (unsigned)(l.xt[cur ^ 1] / 256);
+            q.v = (unsigned)(l.x[cur] / 256);
+            q.to = (unsigned)(l.x[cur ^ 1] / 256);
+            q.apply = 1;
             q.gain = 1.f / SP;
             q.M = q.K = (int)l.mp;
             q.N = (int)l.np;
@@ -757,6 +795,12 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
         }
         ws += w.l.bytes * mats[k].batch;
     }
+    // long sums first: what starts last should end soon
+    for (int k = 1; k < s.count; ++k)
+        for (int j = k; j > 0 && s.mat[j].steps > s.mat[j - 1].steps; --j) {
+            std::swap(s.mat[j], s.mat[j - 1]);
+            std::swap(batch[j], batch[j - 1]);
+        }
     // one tile size for the launch: the one that takes least, counted as if all its workgroups ran over the longest k
     int T = 64;
     double least = 1e30;
@@ -764,7 +808,7 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
         int64_t wgs = 0, longest = 0;
         for (int k = 0; k < s.count; ++k) {
             const Op& q = s.mat[k];
-            wgs += tiles_of(q.M, q.N, q.kind != RESULT && q.dn == q.dt, t) * q.cut * batch[k];
+            wgs += tiles_of(q.M, q.N, !q.apply, t) * q.cut * batch[k];
             if (q.steps > longest) longest = q.steps;
         }
         const double c = cost_of(t, wgs, 1, longest);
@@ -776,10 +820,11 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
     int64_t blocks = 0;
     for (int k = 0; k < s.count; ++k) {
         Op& q = s.mat[k];
-        q.tiles = (int)tiles_of(q.M, q.N, q.kind != RESULT && q.dn == q.dt, T);
+        q.tiles = (int)tiles_of(q.M, q.N, !q.apply, T);
         s.first[k] = (int)blocks;
         blocks += (int64_t)q.tiles * q.cut * batch[k];
     }
+    s.first[s.count] = (int)blocks;
     if (int rc = T == 256                  ? launch_gemm<256, 2>((unsigned)blocks, s, dtype, st)
                  : T == 64 && blocks > 512 ? launch_gemm<64, 2>((unsigned)blocks, s, dtype, st)   // five a CU fit, and hide more than a longer ring
                  : T == 64                 ? launch_gemm<64, 4>((unsigned)blocks, s, dtype, st)   // (576 tiles of k = 512: 16.7 us against 17.9)
@@ -1091,7 +1136,7 @@ int64_t total_bytes(const gan_matrix* mats, int count) {
     for (int k = 0; k < count; ++k) {
         const gan_matrix& g = mats[k];
         if (g.rows < 1 || g.cols < 1 || g.batch < 0 || g.rows > (1 << 20) || g.cols > (1 << 20) || g.batch > (1 << 30)) return -1;
-        if (g.rows * g.cols > (1LL << 32) || (g.rows < g.cols ? g.rows : g.cols) > 32768) return -1;
+        if (g.rows * g.cols > (1LL << 30) || (g.rows < g.cols ? g.rows : g.cols) > 32768) return -1;
         const int64_t one = lay_of(g.rows, g.cols).bytes;
         if (g.batch && one > (1LL << 60) / g.batch) return -1;
         n += one * g.batch;
@@ -1114,8 +1159,7 @@ int pack(const gan_matrix* mats, int n, char* ws, Mats& s, hipStream_t st) {
         q.buf = g.buf;
         q.ws = ws;
         q.stride = l.bytes;
-        q.nat = g.rows <= g.cols ? l.xm[0] : l.xt[0];
-        q.tra = g.rows <= g.cols ? l.xt[0] : l.xm[0];
+        q.x = l.x[0];
         q.rows = (int)g.rows;
         q.cols = (int)g.cols;
         ws += l.bytes * g.batch;
@@ -1146,7 +1190,7 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, const
     GAN_CHECK_ARG(bounded(steps, rule.a, rule.b, rule.c), "%s: with coefficients %g %g %g a singular value can grow beyond 3.5", what, (double)rule.a,
                   (double)rule.b, (double)rule.c);
     const int64_t need = total_bytes(all, count);
-    GAN_CHECK_ARG(need >= 0, "%s: a matrix has a size that is not supported (1 to 2^20 either way, the smaller at most 32768)", what);
+    GAN_CHECK_ARG(need >= 0, "%s: a matrix has a size that is not supported (1 to 2^20 either way, the smaller at most 32768, 2^30 elements)", what);
     GAN_CHECK_ARG(need == 0 || (ws && bytes >= need), "%s: workspace of %lld bytes wanted, %lld given", what, (long long)need,
                   (long long)(ws ? bytes : 0));
     GAN_CHECK_ARG(((uintptr_t)ws % 256) == 0, "%s: workspace must be 256-byte aligned", what);
