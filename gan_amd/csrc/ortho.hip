@@ -3,8 +3,12 @@
 //   A = X X',  P = a I + b A + c A A,  X <- P X
 // Every product is C = U V' on 16-bit matrix instructions with 32-bit accuracy: a value is held as two fp16 planes
 // (hi + lo, 22 bits, times a power of two that its bound allows: |X|, |A|, |P| have bounds that the coefficients set), and
-// hi hi + hi lo + lo hi are accumulated in fp32.  The dropped lo lo is 2^-24 of the product.  Three fp16 products run at
-// a third of the dense 2.5 PFLOP/s; fp32 matrix instructions stop at 0.16.
+// hi hi + hi lo + lo hi are accumulated in fp32.  The dropped lo lo is 2^-24 of the product.  Three fp16 products cost a third
+// of the fp16 rate, and fp32 matrix instructions run at an eighth of it (1.18 PFLOP/s and 0.154 for large products).
+// Measured: P X of 2048 x 8192 in 166 us = 1.24 PFLOP/s of fp16 (0.41 of fp32 accuracy), A = X X' of it in 116 us (0.94; half
+// of A is computed); five iterations 1294 us, of 512 x 4608 181 us.  Large products are bound by the matrix instructions, those
+// of a few hundred rows by their latency: 8 to 10 us a launch, of which a chain of the products a workgroup adds up, the requests' way
+// through the caches and the end of the workgroup are the larger part.
 // All matrices of a call share the launches (one per product), their tiles side by side in the grid; A and P are symmetric,
 // only the tiles on and above the diagonal are computed and the others mirrored.
 #include <type_traits>
@@ -34,8 +38,13 @@ __device__ __forceinline__ void split(float v, h16& hi, h16& lo) {
     lo = (h16)(v - (float)hi);
 }
 
-// eight values to the two planes
-__device__ __forceinline__ void store_planes(h16* to, int64_t plane, const float (&o)[8]) {
+// A matrix in the workspace: of every 32 columns of a row the hi halves, then the lo halves, 128 bytes together -- a line of the
+// caches, which a product's step of 32 k takes as a whole (with the planes apart it would fetch every line twice).
+__device__ __forceinline__ int64_t hi_at(int64_t row, int col, int64_t ld) { return row * 2 * ld + (col >> 5) * 64 + (col & 31); }
+constexpr int LO = 32;  // the lo half, from the hi half
+
+// eight values, the first in a column that is a multiple of eight
+__device__ __forceinline__ void store_planes(h16* to, const float (&o)[8]) {
     h16x8 hi, lo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -45,7 +54,7 @@ __device__ __forceinline__ void store_planes(h16* to, int64_t plane, const float
         lo[e] = w;
     }
     *(h16x8*)to = hi;
-    *(h16x8*)(to + plane) = lo;
+    *(h16x8*)(to + LO) = lo;
 }
 
 // elements of one partial sum of squares
@@ -61,7 +70,7 @@ struct Mat {
     float* buf;      // momentum (NULL: orthogonalise g itself)
     char* ws;        // workspace of the first
     int64_t stride;
-    int64_t x;       // offset of the planes
+    int64_t x;       // offset of X
     int rows, cols;
 };
 
@@ -78,8 +87,7 @@ struct Mats {
     Mat mat[NOPS];
 };
 
-// Byte offsets in one matrix's workspace: the partial sums, two X ([m][n], hi plane then lo plane), five
-// symmetric m x m, the slices' tiles of a product that is cut.  All multiples of 256.
+// Byte offsets in one matrix's workspace: the partial sums, two X (m x n), five symmetric m x m, the slices' tiles of a product that is cut.  All multiples of 256.
 enum { A0, A1, P0, P1, Q0, SQUARES };
 struct Lay {
     int64_t mp, np, nparts, x[2], sq[SQUARES], join, bytes;
@@ -87,12 +95,12 @@ struct Lay {
 };
 
 // What a product of `tiles` T x T tiles over `steps` steps of 32 k takes, in us, every tile's k in `cut` slices: workgroups run
-// in rounds, 256 (T = 256) or 512 of them at a time, a step of theirs as long as measured (T = 256: 2.8; T = 128: 0.55 alone
-// on a CU, 0.8 each where two share it; T = 64: 0.2 and 0.25), a round begins and ends in 5 to 9 us, and slices are written and
+// in rounds, 256 (T = 256) or 512 of them at a time, a step of theirs as long as measured (T = 256: 2.45; T = 128: 0.42 alone
+// on a CU, 0.62 each where two share it; T = 64: 0.19 and 0.2), a round begins and ends in 5 to 9 us, and slices are written and
 // read again at 5 TB/s by one more launch.
 double cost_of(int T, int64_t tiles, int cut, int64_t steps) {
     const int64_t wgs = tiles * cut, slots = T < 256 && wgs > 256 ? 512 : 256, left = wgs % slots;
-    const double alone = T == 256 ? 2.8 : T == 128 ? 0.55 : 0.2, shared = T == 128 ? 1.6 : 0.5, ends = T == 256 ? 9. : T == 128 ? 7. : 5.;
+    const double alone = T == 256 ? 2.45 : T == 128 ? 0.42 : 0.19, shared = T == 128 ? 1.25 : 0.4, ends = T == 256 ? 9. : T == 128 ? 7. : 5.;
     const double n = (double)ceil_div64(steps, cut);
     return (double)(wgs / slots) * (n * (slots == 512 ? shared : alone) + ends) + (left ? n * (left > 256 ? shared : alone) + ends : 0.) +
            (cut > 1 ? 5. + (double)wgs * T * T * 8e-6 / 5. : 0.);
@@ -103,8 +111,7 @@ int64_t tiles_of(int64_t M, int64_t N, bool sym, int T) {
     return sym ? tm * (tm + 1) / 2 : tm * tn;
 }
 
-// Slices of A = X X' (a long k, few tiles), at least eight steps each.  By the matrix's own shape, so that its bits do not
-// depend on what else is in the call.
+// Slices of A = X X' (a long k, few tiles), at least eight steps each, by the matrix's own shape (the workspace goes by it).
 int cut_of(int64_t mp, int64_t np) {
     int best = 1;
     double least = 1e30;
@@ -225,7 +232,7 @@ __device__ __forceinline__ float scale_of(const double* part, int nparts, float 
     return n < 1e300 ? (float)((double)SX / (n > (double)eps ? n : (double)eps)) : __builtin_nanf("");
 }
 
-// ---- the scaled source as two planes [m][n], padded with zeros (a tall source transposed) ------------------------------
+// ---- the scaled source as m x n, padded with zeros (a tall source transposed) --------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
     __shared__ float tile[64][65];
@@ -258,14 +265,13 @@ __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
     }
     __syncthreads();
     h16* to = (h16*)(ws + q.x);
-    const int64_t plane = (int64_t)rp * cp;
     const bool wide = q.rows <= q.cols;
     for (int k = threadIdx.x; k < 64 * 8; k += 256) {
         const int r = k >> 3, c = (k & 7) * 8;
         float o[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = wide ? tile[r][c + e] : tile[c + e][r];
-        store_planes(to + (wide ? (int64_t)(r0 + r) * cp + c0 + c : (int64_t)(c0 + r) * rp + r0 + c), plane, o);
+        store_planes(to + (wide ? hi_at(r0 + r, c0 + c, cp) : hi_at(c0 + r, r0 + c, rp)), o);
     }
 }
 
@@ -307,11 +313,25 @@ __device__ __forceinline__ float step_of(const Rule& s, int rows, int cols) {
     return s.update == 2 ? s.step * sqrtf(fmaxf(1.f, r / c)) : s.update == 3 ? s.step * 0.2f * sqrtf(fmaxf(r, c)) : s.step;
 }
 
-// Tile t of the tiles on and above the diagonal of n x n, row by row
+// Tile t of the tiles on and above the diagonal of n x n: strips of four tile rows, down the columns of each.  A run of sixteen
+// tiles then reads eight row blocks of the operand, not seventeen as along a row: what a die's cache has to bring in from the
+// memory side, at 8 TB/s over all of them, bounds these products.
 __device__ __forceinline__ int2 tile_of(int t, int n) {
-    int ti = 0;
-    for (int left = n; t >= left; --left, ++ti) t -= left;
-    return make_int2(ti, ti + t);
+    int top = 0, h = n < 4 ? n : 4;
+    for (;;) {
+        const int all = h * (h + 1) / 2 + h * (n - top - h);
+        if (t < all) break;
+        t -= all;
+        top += 4;
+        h = n - top < 4 ? n - top : 4;
+    }
+    int c = 0;
+    for (; c < h; ++c) {  // the triangle on the diagonal
+        if (t <= c) return make_int2(top + t, top + c);
+        t -= c + 1;
+    }
+    c = t / h;
+    return make_int2(top + t - c * h, top + h + c);
 }
 
 // A wave's 32 x 32 block of a product at (i0, j0), as accumulated: lane holds column lane & 31, rows 8 (r / 4) + 4 (lane >> 5) +
@@ -343,15 +363,14 @@ __device__ __forceinline__ void store_result(const Rule& rule, T* to, float (&o)
 
 __device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int b, int i0, int j0, f32x16& acc, bool mirror, int dtype, float* t) {
     const int lane = threadIdx.x & 63;
-    const int64_t plane = (int64_t)q.M * q.N;
     // the values first, where the accumulators hold them: no branch or load stands between the trips through LDS
     if (q.kind == POLY) {  // (A is symmetric: its rows for the columns held here)
-        const h16* A = (const h16*)(ws + (int64_t)q.aux * 256) + (int64_t)(j0 + (lane & 31)) * q.N + i0 + 4 * (lane >> 5);
+        const h16* A = (const h16*)(ws + (int64_t)q.aux * 256) + hi_at(j0 + (lane & 31), i0 + 4 * (lane >> 5), q.N);
         h16x4 ah[4], al[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             ah[r] = *(const h16x4*)(A + 8 * r);
-            al[r] = *(const h16x4*)(A + plane + 8 * r);
+            al[r] = *(const h16x4*)(A + LO + 8 * r);
         }
         const float c = s.rule.c * (SP / (SA * SA)), bb = s.rule.b * (SP / SA), aa = s.rule.a * SP;
         const int on = j0 + (lane & 31) - i0 - 4 * (lane >> 5);  // the row of the diagonal
@@ -396,10 +415,10 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int 
     }
     h16* to = (h16*)(ws + (int64_t)q.to * 256);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) store_planes(to + (int64_t)(i0 + h * 16 + a) * q.N + j0 + c, plane, o[h]);
+    for (int h = 0; h < 2; ++h) store_planes(to + hi_at(i0 + h * 16 + a, j0 + c, q.N), o[h]);
     if (mirror) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) store_planes(to + (int64_t)(j0 + h * 16 + a) * q.N + i0 + c, plane, x[h]);
+        for (int h = 0; h < 2; ++h) store_planes(to + hi_at(j0 + h * 16 + a, i0 + c, q.N), x[h]);
     }
 }
 
@@ -412,24 +431,19 @@ __device__ __forceinline__ const char* scalar(const char* p) {
     return (const char*)(((uint64_t)hi << 32) | lo);
 }
 
-// One LDS-DMA instruction: a wave's instruction j covers 1 KB of plane j / PP of the stage at `base`.  p: the planes' first bytes,
-// at: the stage's bytes from there in U and in V.  Written out, since the compiler would wait for every request on its way in
-// front of any transposing read of LDS (it cannot tell the stages apart); stage_arrived() waits for what is needed.
-template <int WAVES, int PP>
-__device__ __forceinline__ void ortho_issue(char* base, unsigned at_u, unsigned at_v, int wave, const char* const* p, const unsigned* off, int j) {
+// One LDS-DMA instruction: instruction j of the waves covers WAVES pieces of 1 KB of the stage at `base`, T / 8 pieces of U and then
+// T / 8 of V.  u, v: the operands' first bytes, at: the stage's bytes from there.  Written out, since the compiler would wait for
+// every request on its way in front of any transposing read of LDS (it cannot tell the stages apart); stage_arrived() waits for
+// what is needed.
+template <int T, int WAVES>
+__device__ __forceinline__ void ortho_issue(char* base, unsigned at_u, unsigned at_v, int wave, const char* u, const char* v, const unsigned* off, int j) {
     typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
-    const uint64_t from = (uint64_t)p[j / PP];
+    const bool of_u = WAVES * j < T / 8;
+    const uint64_t from = (uint64_t)(of_u ? u : v);
     const u32x4 rsrc = {(unsigned)from, (unsigned)(from >> 32), 0xffffffffu, 0x00020000u};
     const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)(base + (WAVES * j + wave) * 1024);
-    const unsigned at = j / PP < 2 ? at_u : at_v;
+    const unsigned at = of_u ? at_u : at_v;
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(off[j]), "s"(rsrc), "s"(at) : "m0");
-}
-
-// Four rows of 32 columns (64 bytes) are read at a time from a [32][T] stage: where in its row a row's lie, so that the four fill
-// the 64 banks (T = 64: two rows fill them already).  Without: 24.8 -> 33 us for a product of 26 steps.
-template <int T>
-__device__ __forceinline__ int v_swizzle(int row) {
-    return T == 64 ? (row & 2) << 1 : (row & 3) << 2;
 }
 
 // Of four rows (k) of sixteen elements, lane i of sixteen brings the four at (row i / 4, columns 4 (i % 4) ...) and takes column
@@ -447,19 +461,18 @@ struct Frags {
     // APPLY: V's stage is [32 k][T], 16 columns of it at a time turned round on the way
     template <int T, bool APPLY>
     __device__ __forceinline__ void read(const char* base, int m0, int n0, int half, int lane, int r) {
-        constexpr int plane = T * 64;
         const bool of_u = r < 2 * FM;
-        const int f = (of_u ? r : r - 2 * FM) >> 1, pl = r & 1, ch = half * 2 + (lane >> 5);
+        const int f = (of_u ? r : r - 2 * FM) >> 1, pl = r & 1;
         if (APPLY && !of_u) {
             const int row = half * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);
-            const int chunk = (n0 + f * 32 + (lane & 16)) / 8 + ((lane & 3) >> 1);
-            const char* p = base + (2 + pl) * plane + row * (T * 2) + ((chunk ^ v_swizzle<T>(row)) << 4) + (lane & 1) * 8;
-            const h16x4 a = read_transposed(p), b = read_transposed(p + 4 * (T * 2));
+            const int chunk = (n0 / 32 + f) * 8 + pl * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+            const char* p = base + T * 128 + row * (T * 4) + ((chunk ^ ((row & 3) << 2)) << 4) + (lane & 1) * 8;
+            const h16x4 a = read_transposed(p), b = read_transposed(p + 4 * (T * 4));
             v[pl][f] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
             return;
         }
-        const int row = (of_u ? m0 : n0) + f * 32 + (lane & 31), at = row * 64 + ((ch ^ ((row >> 2) & 3)) << 4);
-        const h16x8 got = *(const h16x8*)(base + (of_u ? pl : 2 + pl) * plane + at);
+        const int row = (of_u ? m0 : n0) + f * 32 + (lane & 31), chunk = pl * 4 + half * 2 + (lane >> 5);
+        const h16x8 got = *(const h16x8*)(base + (of_u ? 0 : T * 128) + row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4));
         if (of_u) u[pl][f] = got;
         else v[pl][f] = got;
     }
@@ -484,22 +497,19 @@ __device__ __forceinline__ void stage_arrived(bool full) {
     asm volatile("" ::: "memory");
 }
 
-template <int T>
-constexpr int gemm_threads() {
-    return T == 256 ? 512 : 256;
-}
-
-// Tile T x T of C = U V' or U V: four waves of T/2 x T/2, or eight of 128 x 64.  U [M][K], V [N][K] or [K][N], each a hi plane and
-// a lo plane; K % 32 == 0.  Stages of 32 k go to LDS by DMA.  Of a plane with k along its rows a stage holds 64 bytes a row, chunk
-// c of row r at position c ^ ((r >> 2) & 3): the 16 rows that a fragment read touches at a time then lie in different banks.  Of
-// [K][N] it holds 32 rows of T, chunk c of row r at c ^ v_swizzle(r).
-template <int T, int NST>
-__global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm_k(const Ops s, int dtype) {
-    constexpr int WAVES = gemm_threads<T>() / 64, WN = WAVES / 2;  // waves: 2 x WN
+// Tile T x T of C = U V' or U V: four waves of T/2 x T/2 each, or (T = 256) eight of 128 x 64.  KG = 2: two such sets of four, each
+// with one half of every stage; their sums are added at the end.  That is for grids of a workgroup a CU at most, where a lone
+// wave on its SIMD would have nothing beside it while it waits.
+// U [M][K], V [N][K] or [K][N]; K % 32 == 0.  Stages of 32 k go to LDS by DMA.  Of a matrix with k along its rows a stage holds a
+// line (128 bytes: hi, lo) a row, chunk c of row r at position c ^ ((r >> 1) & 7): the 16 rows that a fragment read touches at a
+// time then lie in different banks.  Of [K][N] it holds 32 rows of T, chunk c of row r at c ^ 4 (r & 3): the four rows of 64
+// bytes that a transposing read touches fill the banks.
+template <int T, int NST, int KG>
+__global__ void __launch_bounds__(T == 256 ? 512 : 256 * KG, T == 64 ? 4 : 2) ortho_gemm_k(const Ops s, int dtype) {
+    constexpr int SET = T == 256 ? 8 : 4, WAVES = SET * KG, WN = SET / 2;  // a set's waves: 2 x WN
     constexpr int FM = T / 64, FN = T / 32 / WN;                   // 32 x 32 fragments of a wave
-    constexpr int PLANE = T * 64, STAGE = 4 * PLANE;               // bytes: U hi, U lo, V hi, V lo
+    constexpr int STAGE = 2 * T * 128;                             // bytes: U, V
     constexpr int PER = STAGE / 1024 / WAVES;                      // DMA instructions per wave and stage
-    constexpr int PP = PER / 4;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int group = group_of(s, blockIdx.x);
     const Op q = s.mat[group];  // (a copy: one batch of scalar loads)
@@ -508,7 +518,8 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
     const int all = s.first[group + 1] - s.first[group], local = (int)blockIdx.x - s.first[group];
     const int each = all >> 3, rest = all & 7, die = local & 7;
     const int id = die * each + (die < rest ? die : rest) + (local >> 3);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), in_set = wave % SET, kg = wave / SET,
+              wm = in_set / WN, wn = in_set % WN;
     // (divisions run on vector registers: say that the results are the wave's, or every use of an address loops over lanes)
     const int per = q.tiles * q.cut;
     const int b = __builtin_amdgcn_readfirstlane(id / per);
@@ -524,26 +535,27 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
         ti = tile - tj * tm;
     } else {
         const int2 t = tile_of(tile, (M + T - 1) / T);
-        ti = t.x;
-        tj = t.y;
+        ti = __builtin_amdgcn_readfirstlane(t.x);
+        tj = __builtin_amdgcn_readfirstlane(t.y);
     }
     const int i0 = ti * T, j0 = tj * T;
-    // ---- staging: a wave's instruction j covers 1 KB of the stage = 16 rows of one plane
-    const unsigned kb = (unsigned)K * 2, nb = (unsigned)N * 2;
-    const unsigned v_step = q.apply ? 32 * nb : 64;
+    // ---- staging: a wave's instruction j covers 1 KB of the stage: eight rows with k along them, or part of one that runs along n
+    const unsigned kb = (unsigned)K * 4, nb = (unsigned)N * 4, v_step = q.apply ? 32 * nb : 128;
     unsigned off[PER];
-    const char* const v0 = v + (q.apply ? (int64_t)j0 * 2 : (int64_t)j0 * kb);
-    const char* const planes[4] = {scalar(u + (int64_t)i0 * kb), scalar(u + ((int64_t)M + i0) * kb), scalar(v0), scalar(v0 + (int64_t)N * kb)};
+    const char* const pu = scalar(u + (int64_t)i0 * kb);
+    const char* const pv = scalar(v + (q.apply ? (int64_t)j0 * 4 : (int64_t)j0 * kb));
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const int piece = WAVES * j + wave, pl = piece / (T / 16), at = piece % (T / 16) * 1024 + lane * 16;
+        const int piece = WAVES * j + wave;
+        const bool of_u = piece < T / 8;
+        const int at = (of_u ? piece : piece - T / 8) * 1024 + lane * 16;
         // rows (columns) past the matrix (T = 128 over an odd number of 64s): the last again, their results are not stored
-        if (pl < 2 || !q.apply) {
-            const int row = at / 64, pos = at % 64 / 16, lim = pl < 2 ? M - i0 : N - j0;
-            off[j] = (unsigned)(row < lim ? row : lim - 1) * kb + (unsigned)((pos ^ ((row >> 2) & 3)) * 16);
+        if (of_u || !q.apply) {
+            const int row = at / 128, pos = at % 128 / 16, lim = of_u ? M - i0 : N - j0;
+            off[j] = (unsigned)(row < lim ? row : lim - 1) * kb + (unsigned)((pos ^ ((row >> 1) & 7)) * 16);
         } else {
-            const int row = at / (T * 2), pos = at % (T * 2) / 16, col = (pos ^ v_swizzle<T>(row)) * 8, lim = N - j0 - 8;
-            off[j] = (unsigned)row * nb + (unsigned)(col < lim ? col : lim) * 2;
+            const int row = at / (T * 4), pos = at % (T * 4) / 16, chunk = pos ^ ((row & 3) << 2), lim = (N - j0) / 4 - 1;
+            off[j] = (unsigned)row * nb + (unsigned)(chunk < lim ? chunk : lim) * 16;
         }
     }
     using Fr = Frags<FM, FN>;
@@ -558,7 +570,7 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
                 for (int r = 0; r < 16; ++r) sums[a][x][y][r] = 0.f;
     const int k0 = slice * q.steps, nk = (K / 32 - k0 < q.steps ? K / 32 - k0 : q.steps);
     auto issue = [&](char* base, int step, int j) __attribute__((always_inline)) {
-        ortho_issue<WAVES, PP>(base, (unsigned)(k0 + step) * 64, (unsigned)(k0 + step) * v_step, wave, planes, off, j);
+        ortho_issue<T, WAVES>(base, (unsigned)(k0 + step) * 128, (unsigned)(k0 + step) * v_step, wave, pu, pv, off, j);
     };
 #pragma unroll
     for (int k = 0; k < NST; ++k)
@@ -576,6 +588,43 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
     auto walk = [&](auto apply) __attribute__((always_inline)) {
         constexpr bool APPLY = decltype(apply)::value;
         Fr f0, f1;
+        if constexpr (KG == 2) {
+            // this set's half of the next stage is read, and the stage after the last asked for, while its half of this one runs
+            auto step = [&](int k, Fr& now, Fr& then, bool more) __attribute__((always_inline)) {
+                stage_arrived<(NST - 2) * PER>(k + NST - 1 < nk);
+#pragma unroll
+                for (int i = 0; i < Fr::PRODUCTS; ++i) {
+                    now.multiply(sums, i);
+#pragma unroll
+                    for (int r = 0; r < Fr::READS; ++r)
+                        if (r * Fr::PRODUCTS / (2 * Fr::READS) == i)
+                            then.template read<T, APPLY>(lds + (k + 1) % NST * STAGE, m0, n0, kg, lane, r);
+                    if (more) {
+#pragma unroll
+                        for (int j = 0; j < PER; ++j)
+                            if ((j + 1) * Fr::PRODUCTS / PER - 1 == i) issue(lds + k % NST * STAGE, k + NST, j);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            stage_arrived<(NST - 1) * PER>(nk >= NST);
+#pragma unroll
+            for (int r = 0; r < Fr::READS; ++r) f0.template read<T, APPLY>(lds, m0, n0, kg, lane, r);
+            int k = 0;
+            for (; k + 1 + NST < nk; k += 2) {
+                step(k, f0, f1, true);
+                step(k + 1, f1, f0, true);
+            }
+            for (; k + 2 < nk; k += 2) {
+                step(k, f0, f1, k + NST < nk);
+                step(k + 1, f1, f0, k + 1 + NST < nk);
+            }
+            if (k + 1 < nk) step(k, f0, f1, k + NST < nk);
+            const Fr& tail = k + 1 < nk ? f1 : f0;
+#pragma unroll
+            for (int i = 0; i < Fr::PRODUCTS; ++i) tail.multiply(sums, i);
+            return;
+        }
         stage_arrived<(NST - 1) * PER>(nk >= NST);
 #pragma unroll
         for (int r = 0; r < Fr::READS; ++r) f0.template read<T, APPLY>(lds, m0, n0, 0, lane, r);
@@ -628,36 +677,59 @@ __global__ void __launch_bounds__(gemm_threads<T>(), T == 64 ? 4 : 2) ortho_gemm
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[0][0][r] = sums[Fr::NACC - 1][0][0][r] + (acc[0][0][r] + sums[Fr::NACC / 2][0][0][r]);
     }
-    if (q.cut > 1) {  // this slice's sums, in the order that join_k reads them
-        float4* out = (float4*)(ws + (int64_t)q.join * 256) + ((int64_t)slice * q.tiles + tile) * (T * T / 4) + wave * (T * T / 4 / WAVES) + lane;
-#pragma unroll
-        for (int x = 0; x < FM; ++x)
-#pragma unroll
-            for (int y = 0; y < FN; ++y)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    out[((x * FN + y) * 4 + r) * 64] = make_float4(acc[x][y][r * 4], acc[x][y][r * 4 + 1], acc[x][y][r * 4 + 2], acc[x][y][r * 4 + 3]);
-        return;
-    }
+    // the blocks that this wave goes on with, in a row: all of the set's, or its set's share once the sets' sums are added
+    constexpr int BLOCKS = FM * FN, KEEP = KG == 1 ? BLOCKS : (BLOCKS + 1) / 2;
+    const int keep = kg * KEEP;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();  // (the stages are read: their LDS is free)
-    float* t = (float*)(lds + wave * TBYTES);
+    if constexpr (KG == 2) {
+        float4* x = (float4*)lds + in_set * BLOCKS * 256 + lane;
+#pragma unroll
+        for (int f = 0; f < BLOCKS; ++f)
+            if (f / KEEP != kg) {  // the other set's
+                const f32x16& o = acc[f / FN][f % FN];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[(f * 4 + r) * 64] = make_float4(o[r * 4], o[r * 4 + 1], o[r * 4 + 2], o[r * 4 + 3]);
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+#pragma unroll
+        for (int f = 0; f < BLOCKS; ++f)
+            if (f / KEEP == kg) {
+                f32x16& o = acc[f / FN][f % FN];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float4 v = x[(f * 4 + r) * 64];
+                    o[r * 4] += v.x;
+                    o[r * 4 + 1] += v.y;
+                    o[r * 4 + 2] += v.z;
+                    o[r * 4 + 3] += v.w;
+                }
+            }
+    }
+    float4* out = (float4*)(ws + (int64_t)q.join * 256) + ((int64_t)slice * q.tiles + tile) * (T * T / 4) + in_set * (T * T / 4 / SET) + lane;
+    float* t = (float*)(lds + (KG == 1 ? 0 : SET * BLOCKS * 4096) + wave * TBYTES);
     // one block after another through the same code: unrolled, its instructions would be fetched for every block anew
 #pragma unroll 1
-    for (int f = 0; f < FM * FN; ++f) {
+    for (int f = keep; f < BLOCKS && f < keep + KEEP; ++f) {
         f32x16 one = acc[0][0];
 #pragma unroll
-        for (int k = 1; k < FM * FN; ++k)
+        for (int k = 1; k < BLOCKS; ++k)
             if (f == k) one = acc[k / FN][k % FN];
         const int i = i0 + wm * (T / 2) + f / FN * 32, j = j0 + wn * (T / WN) + f % FN * 32;
-        if (i < M && j < N) finish(s, q, ws, b, i, j, one, !q.apply && ti != tj, dtype, t);
+        if (q.cut > 1) {  // this slice's sums, in the order that join_k reads them
+#pragma unroll
+            for (int r = 0; r < 4; ++r) out[(f * 4 + r) * 64] = make_float4(one[r * 4], one[r * 4 + 1], one[r * 4 + 2], one[r * 4 + 3]);
+        } else if (i < M && j < N) {
+            finish(s, q, ws, b, i, j, one, !q.apply && ti != tj, dtype, t);
+        }
     }
 }
 
 // The slices of a product that was cut, added in their order; a 32 x 32 block a workgroup of one wave
 template <int T>
 __global__ void __launch_bounds__(64) ortho_join_k(const Ops s, int dtype) {
-    constexpr int WAVES = gemm_threads<T>() / 64, WN = WAVES / 2, FN = T / 32 / WN, BLK = T * T / 1024;  // blocks of a tile
+    constexpr int WAVES = T == 256 ? 8 : 4, WN = WAVES / 2, FN = T / 32 / WN, BLK = T * T / 1024;  // blocks of a tile
     __shared__ __attribute__((aligned(16))) float lds[TBYTES / 4];
     const int group = group_of(s, blockIdx.x);
     const Op q = s.mat[group];
@@ -694,15 +766,15 @@ __global__ void __launch_bounds__(64) ortho_join_k(const Ops s, int dtype) {
     if (i < q.M && j < q.N) finish(s, q, ws, b, i, j, acc, t.x != t.y, dtype, lds);
 }
 
-template <int T, int NST>
+template <int T, int NST, int KG>
 int launch_gemm(unsigned blocks, const Ops& s, int dtype, hipStream_t st) {
-    constexpr int lds = NST * 4 * T * 64;
+    constexpr int lds = NST * 2 * T * 128;
     // more than 64 KB of dynamic LDS needs the attribute (set on every call: it is per device, and cheap)
-    if (lds > 64 * 1024 && hipFuncSetAttribute((const void*)ortho_gemm_k<T, NST>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+    if (lds > 64 * 1024 && hipFuncSetAttribute((const void*)ortho_gemm_k<T, NST, KG>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
         gan_set_error("orthogonalize: cannot reserve %d bytes of LDS", lds);
         return GAN_ERR_LAUNCH;
     }
-    hipLaunchKernelGGL((ortho_gemm_k<T, NST>), dim3(blocks), dim3(gemm_threads<T>()), lds, st, s, dtype);
+    hipLaunchKernelGGL((ortho_gemm_k<T, NST, KG>), dim3(blocks), dim3(T == 256 ? 512 : 256 * KG), lds, st, s, dtype);
     GAN_CHECK_LAUNCH("orthogonalize(product)");
     return GAN_OK;
 }
@@ -825,11 +897,14 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
         blocks += (int64_t)q.tiles * q.cut * batch[k];
     }
     s.first[s.count] = (int)blocks;
-    if (int rc = T == 256                  ? launch_gemm<256, 2>((unsigned)blocks, s, dtype, st)
-                 : T == 64 && blocks > 512 ? launch_gemm<64, 2>((unsigned)blocks, s, dtype, st)   // five a CU fit, and hide more than a longer ring
-                 : T == 64                 ? launch_gemm<64, 4>((unsigned)blocks, s, dtype, st)   // (576 tiles of k = 512: 16.7 us against 17.9)
-                 : blocks > 256            ? launch_gemm<128, 2>((unsigned)blocks, s, dtype, st)  // two a CU; 222 us against 237 with a ring of four
-                                           : launch_gemm<128, 4>((unsigned)blocks, s, dtype, st))  // alone: 131 us against 167 with a ring of two
+    // Where there is a workgroup a CU at most, a long ring of stages and two sets of waves (KG = 2) hide the waits: 116 us against 182
+    // for A = X X' of 2048 x 8192.  Where there are more, those do, and short rings let more of them in: two of T = 128 a CU
+    // (174 us against 184 for P X), five of T = 64 (14.3 us against 15.5 for 576 tiles of k = 512).
+    if (int rc = T == 256                  ? launch_gemm<256, 2, 1>((unsigned)blocks, s, dtype, st)
+                 : T == 128 ? blocks > 256 ? launch_gemm<128, 2, 1>((unsigned)blocks, s, dtype, st)
+                                           : launch_gemm<128, 4, 2>((unsigned)blocks, s, dtype, st)
+                 : blocks > 512            ? launch_gemm<64, 2, 1>((unsigned)blocks, s, dtype, st)
+                                           : launch_gemm<64, 4, 2>((unsigned)blocks, s, dtype, st))
         return rc;
     if (!sliced) return GAN_OK;
     int64_t join = 0;
@@ -1136,7 +1211,7 @@ int64_t total_bytes(const gan_matrix* mats, int count) {
     for (int k = 0; k < count; ++k) {
         const gan_matrix& g = mats[k];
         if (g.rows < 1 || g.cols < 1 || g.batch < 0 || g.rows > (1 << 20) || g.cols > (1 << 20) || g.batch > (1 << 30)) return -1;
-        if (g.rows * g.cols > (1LL << 30) || (g.rows < g.cols ? g.rows : g.cols) > 32768) return -1;
+        if (up64(g.rows) * up64(g.cols) >= (1LL << 30) || (g.rows < g.cols ? g.rows : g.cols) > 32768) return -1;
         const int64_t one = lay_of(g.rows, g.cols).bytes;
         if (g.batch && one > (1LL << 60) / g.batch) return -1;
         n += one * g.batch;
@@ -1186,23 +1261,24 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, const
             hipStream_t st) {
     GAN_CHECK_ARG(count >= 0 && (count == 0 || all), "%s: null list", what);
     GAN_CHECK_ARG(steps >= 1 && steps <= 100, "%s: 1 to 100 steps, got %d", what, steps);
-    GAN_CHECK_ARG(source.eps > 0.f && source.eps < 1e30f, "%s: eps must be positive, got %g", what, (double)source.eps);
+    // (SX / eps has to be a finite fp32)
+    GAN_CHECK_ARG(source.eps >= 1e-30f && source.eps <= 1e30f, "%s: eps must be positive, 1e-30 to 1e30, got %g", what, (double)source.eps);
     GAN_CHECK_ARG(bounded(steps, rule.a, rule.b, rule.c), "%s: with coefficients %g %g %g a singular value can grow beyond 3.5", what, (double)rule.a,
                   (double)rule.b, (double)rule.c);
     const int64_t need = total_bytes(all, count);
-    GAN_CHECK_ARG(need >= 0, "%s: a matrix has a size that is not supported (1 to 2^20 either way, the smaller at most 32768, 2^30 elements)", what);
+    GAN_CHECK_ARG(need >= 0, "%s: a matrix has a size that is not supported (1 to 2^20 either way, the smaller at most 32768, fewer than 2^30 elements when padded to 64s)", what);
     GAN_CHECK_ARG(need == 0 || (ws && bytes >= need), "%s: workspace of %lld bytes wanted, %lld given", what, (long long)need,
                   (long long)(ws ? bytes : 0));
     GAN_CHECK_ARG(((uintptr_t)ws % 256) == 0, "%s: workspace must be 256-byte aligned", what);
+    const bool small = all_small(all, count);
     for (int k = 0; k < count; ++k) {
         const gan_matrix& g = all[k];
         GAN_CHECK_ARG(!g.batch || (g.g && g.out && (!rule.update || g.buf)), "%s: null pointer", what);
         const Lay l = lay_of(g.rows, g.cols);
         const int64_t tiles = l.mp / 64 * (l.np / 64) + 4096;  // (slices stay below that)
-        GAN_CHECK_ARG(g.batch <= MAXGRID / NOPS / (tiles > l.nparts ? tiles : l.nparts), "%s: %lld matrices of %lld x %lld are too many for one call",
+        GAN_CHECK_ARG(g.batch <= (small ? (1 << 22) / NOPS : MAXGRID / NOPS / (tiles > l.nparts ? tiles : l.nparts)), "%s: %lld matrices of %lld x %lld are too many for one call",
                       what, (long long)g.batch, (long long)g.rows, (long long)g.cols);
     }
-    const bool small = all_small(all, count);
     Mats s = {};
     Ops o = {};
     s.from = source;

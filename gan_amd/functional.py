@@ -1018,7 +1018,7 @@ def matrix_workspace(mats, device) -> Tuple[Optional[Tensor], int]:
     n = _lib.load().gan_orthogonalize_workspace(ctypes.addressof(mats), len(mats))
     if n < 0:
         sizes = sorted({(m.rows, m.cols) for m in mats}, key=max)
-        raise _lib.GanAmdError(f"orthogonalize: matrices of 1 to 2^20 rows and columns, the smaller side at most 32768, 2^30 elements; got up to {sizes[-1]}")
+        raise _lib.GanAmdError(f"orthogonalize: matrices of 1 to 2^20 rows and columns, the smaller side at most 32768, fewer than 2^30 elements; got up to {sizes[-1]}")
     return (torch.empty((n,), dtype=torch.uint8, device=device) if n else None), n
 
 
