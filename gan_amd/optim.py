@@ -159,7 +159,7 @@ def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentum_buffer
         raise _lib.GanAmdError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momentum_buffers)} momentum buffers")
     if adjust_lr_fn not in _SCALINGS:
         raise _lib.GanAmdError(f"muon_step: adjust_lr_fn must be None, 'original', 'match_rms_adamw' or 'none', got {adjust_lr_fn!r}")
-    held, mats, seen = [], [], set()
+    held, mats, spans = [], [], []
     for p, g, m in zip(params, grads, momentum_buffers):
         if p.dim() < 2:
             raise _lib.GanAmdError(f"muon_step: parameters of two or more dimensions, got shape {tuple(p.shape)}")
@@ -175,13 +175,16 @@ def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentum_buffer
             continue
         g = g.contiguous()
         held.append(g)
-        for t in (p, m):
-            if t.data_ptr() in seen:
-                raise _lib.GanAmdError("muon_step: a parameter or momentum buffer is given twice")
-            seen.add(t.data_ptr())
+        spans += [(t.data_ptr(), t.data_ptr() + t.numel() * 4, written) for t, written in ((p, True), (m, True), (g, False))]
         mats.append((g.data_ptr(), m.data_ptr(), p.data_ptr(), *_as_matrix(p.shape), 1))
-    if any(g.data_ptr() in seen for g in held):
-        raise _lib.GanAmdError("muon_step: a gradient lies where a parameter or momentum buffer does")
+    reads, writes = 0, 0  # where what lies below ends
+    for start, end, written in sorted(spans):
+        if start < writes or (written and start < reads):
+            raise _lib.GanAmdError("muon_step: a parameter or momentum buffer is given twice, or overlaps another or a gradient")
+        if written:
+            writes = max(writes, end)
+        else:
+            reads = max(reads, end)
     require_gpu(*params[:1])
     if not mats:
         return

@@ -23,9 +23,9 @@ def dev():
     return torch.device("cuda:0")
 
 
-def definition(g, steps=5, coefficients=COEFFS, eps=1e-7):
+def definition(g, steps=5, coefficients=COEFFS, eps=1e-7, on="cpu"):
     a, b, c = coefficients
-    x = g.detach().double().cpu()
+    x = g.detach().double().to(on)
     x = x / torch.linalg.matrix_norm(x).clamp_min(eps)[..., None, None]
     tall = x.shape[-2] > x.shape[-1]
     if tall:
@@ -68,6 +68,44 @@ def test_against_the_definition(dev, m, n):
         got = GF.orthogonalize(bf)
         assert got.dtype == torch.bfloat16
         assert rel_err(got, definition(bf)) < lim + 2.0**-8, kind
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1990, 33000), (2048, 8192), (1030, 4100), (3, 1000, 1777), (9, 260, 2000), (20000, 3, 5), (100000, 40)])
+def test_large_ones(dev, shape):
+    """Sizes at which the larger tiles run, whole and with a part of one at the end, with their sums cut in slices and not; many
+    matrices at once, and very long ones.  (The reference runs on the device, in 64 bits.)"""
+    from gan_amd import functional as GF
+
+    torch.manual_seed(5)
+    g = torch.randn(shape, device=dev)
+    if shape[-1] > 5:
+        g += 4 * torch.randn(*shape[:-1], 2, device=dev) @ torch.randn(*shape[:-2], 2, shape[-1], device=dev)
+    want = definition(g, on=dev)
+    lim = 1e-4 if shape[-1] > 5 else 6e-4
+    assert rel_err(GF.orthogonalize(g), want) < lim
+    del want
+    g = g.bfloat16()
+    assert rel_err(GF.orthogonalize(g), definition(g, on=dev)) < lim + 2.0**-8
+
+
+@pytest.mark.gpu
+def test_two_calls_at_once(dev):
+    """Calls on two streams, neither waiting for the other, leave the bits of calls one after another."""
+    from gan_amd import functional as GF
+
+    xs = [make(300, 2300, dev, seed=1), make(512, 900, dev, seed=2)]
+    want = [GF.orthogonalize(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for k, (x, st) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(st):
+                got[k].append(GF.orthogonalize(x))
+    torch.cuda.synchronize()
+    for w, all_of in zip(want, got):
+        assert all(torch.equal(w, y) for y in all_of)
 
 
 @pytest.mark.gpu
@@ -409,7 +447,7 @@ def test_refusals():
     ):
         with pytest.raises(_lib.GanAmdError):
             call()
-    x = x.detach()
+    x, flat = x.detach(), torch.randn(64)
     for args, kw in (
         (([x], [x.clone()], [x.clone()]), {}),  # not on a ROCm device
         (([x], [], [x]), {}),
@@ -421,6 +459,8 @@ def test_refusals():
         (([x], [x], [x.clone()]), {}),
         (([x], [x.clone()], [x]), {}),
         (([x], [x.clone()], [x.clone()]), dict(adjust_lr_fn="other")),
+        (([flat[:32].view(4, 8), flat[31:63].view(4, 8)], [x.clone(), x.clone()], [x.clone(), x.clone()]), {}),
+        (([flat[:32].view(4, 8)], [flat[31:63].view(4, 8)], [x.clone()]), {}),
     ):
         with pytest.raises(_lib.GanAmdError):
             muon_step(*args, lr=0.1, **kw)
@@ -443,12 +483,13 @@ def test_refusals():
     assert need > 0
     assert run(ok, steps=0) != 0 and run(ok, steps=101) != 0
     assert run(ok, eps=0.0) != 0 and run(ok, eps=float("nan")) != 0
+    assert run(ok, eps=1e-31) != 0 and run(ok, eps=1e31) != 0
     assert run(ok, coeffs=(10.0, 0.0, 0.0)) != 0 and run(ok, coeffs=(float("nan"), 0.0, 0.0)) != 0
     assert run(ok, dtype=2) != 0
     assert run(ok, ws=None) != 0 and run(ok, nbytes=need - 1) != 0 and run(ok, ws=p + 16) != 0
     assert run(mats((None, None, p, 4, 8, 1))) != 0 and run(mats((p, None, None, 4, 8, 1))) != 0
     assert run(mats((p, p, p, 4, 8, 1))) != 0  # a momentum buffer without a step
-    for rows, cols, batch in ((0, 8, 1), (4, -1, 1), (4, 8, -1), (1 << 21, 8, 1), (40000, 40000, 1), (4, 8, 1 << 31)):
+    for rows, cols, batch in ((0, 8, 1), (4, -1, 1), (4, 8, -1), (1 << 21, 8, 1), (40000, 40000, 1), (1 << 20, 1024, 1), (4, 8, 1 << 31)):
         bad = mats((p, None, p, rows, cols, batch))
         assert lib.gan_orthogonalize_workspace(ctypes.addressof(bad), 1) < 0 and run(bad) != 0
     assert run(mats((p, None, p, 4, 8, 0))) == 0  # nothing to do
