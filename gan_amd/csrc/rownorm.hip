@@ -167,7 +167,7 @@ struct RowArgs {
     const void *x, *g, *v;
     const float *w, *b, *cw, *cb;
     void *y, *y2;      // forward: y.  backward: gx.  second: gg, gxx
-    float2* stats;     // (m, r) of each row
+    float2* stats;     // (m, r) of each row (forward: may be NULL)
     float2* vstats;    // second: (mean v, mean(v t)) of each row, for the column kernel (may be NULL)
     float* part;       // column partials [blocks][ncol][D], or NULL
     float* join;       // long rows: partial sums [rows][pieces][NSUM]
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(block_of<TPR>()) ln_fwd_k(const RowArgs a) {
         row_sum<1, TPR>(q, lds, flip);
         x.settle();
         const float r = rsqrtf(q[0] * inv + a.eps);
-        if (lane == 0) a.stats[row] = make_float2(m, r);
+        if (a.stats && lane == 0) a.stats[row] = make_float2(m, r);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             float wk[V], bk[V];
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(TPB) ln_long_apply_k(const RowArgs a) {
         }
         row_sum<1, TPB>(q, lds, flip);
         const float r = rsqrtf(q[0] * inv + a.eps);
-        if (p == 0 && lane == 0) a.stats[row] = make_float2(m, r);
+        if (a.stats && p == 0 && lane == 0) a.stats[row] = make_float2(m, r);
         float b[LK][V];
         load_cols<V, LK, TPB>(a.b ? a.b + (int64_t)p * a.piece : nullptr, 0.f, b, lane, n);
 #pragma unroll
@@ -857,7 +857,7 @@ extern "C" int gan_layernorm_fwd(const void* x, const float* w, const float* b, 
     GAN_CHECK_ARG(!bad_shape(rows, D, dtype), "layernorm_fwd: bad shape or dtype (%lld rows of %lld, dtype %d)", (long long)rows, (long long)D, dtype);
     GAN_CHECK_ARG(eps >= 0.f, "layernorm_fwd: eps must not be negative");
     if (rows == 0) return GAN_OK;
-    GAN_CHECK_ARG(x && y && stats, "layernorm_fwd: null pointer");
+    GAN_CHECK_ARG(x && y, "layernorm_fwd: null pointer");
     GAN_CHECK_ARG(((uintptr_t)stats % 8) == 0, "layernorm_fwd: stats must be 8-byte aligned");
     const Plan p = plan_of(rows, D, dtype, 0, false);
     if (int rc = check_common("layernorm_fwd", rows, D, dtype, ws, ws_floats, p)) return rc;

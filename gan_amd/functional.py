@@ -30,7 +30,7 @@ from typing import Dict, Optional, Tuple
 import torch
 import torch.nn.functional as F
 from torch import Tensor
-from torch.autograd import Function as _TorchFunction
+from torch.autograd import Function as _TorchFunction, forward_ad
 
 from . import _lib
 from ._lib import check, dtype_code, on_device, ptr, require_gpu, stream_of
@@ -2605,12 +2605,12 @@ def _launch(family: str, tensors, tag, fn, *args) -> None:
         check(status, fn.__name__)
 
 
-def raw_layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], d: int, eps: float):
-    """(y, stats (rows, 2)) of contiguous x, normalised over its last d elements."""
+def raw_layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], d: int, eps: float, keep: bool = True):
+    """(y, stats (rows, 2), or None unless `keep`) of contiguous x, normalised over its last d elements."""
     rows, code = x.numel() // d, dtype_code(x)
     y = torch.empty_like(x)
     n = _layer_norm_ws(rows, d, code, 0, False)
-    stats = x.new_empty((rows, 2), dtype=torch.float32)
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if keep else None
     ws = x.new_empty((n,), dtype=torch.float32) if n else None
     _launch("layernorm", (x, y), (rows, d), _lib.load().gan_layernorm_fwd, ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(stats), rows, d, eps, code,
             ptr(ws), n)
@@ -2760,7 +2760,11 @@ def layer_norm(x: Tensor, normalized_shape, weight: Optional[Tensor] = None, bia
     dtype_code(x)
     require_gpu(x)
     d = math.prod(shape)
-    if weight is not None and weight.is_leaf and weight.requires_grad and torch.is_grad_enabled():
+    if not (torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))):
+        # sampling and evaluation: the launch alone (a dual tensor of forward-mode AD is left to the Function, which refuses it)
+        if x.is_contiguous() and forward_ad._current_level < 0:
+            return raw_layer_norm(x, _plain_f32(weight), _plain_f32(bias), d, eps, False)[0]
+    elif weight is not None and weight.is_leaf and weight.requires_grad:
         weight = weight.view_as(weight)  # (see _wanted)
     if x.is_contiguous():
         return LayerNormFn.apply(x, weight, bias, d, eps)

@@ -340,7 +340,7 @@ int gan_space_to_depth(const void* x, void* out, int N, int H, int W, int C, int
 
 /* ---- layer norm over the rows of a dense (rows, D) matrix: forward, backward, second order ---------------------
  * With m, r = (mean, 1 / sqrt(biased variance + eps)) of a row, t = (x - m) r and P(u) = u - mean(u) - t mean(u t):
- * gan_layernorm_fwd : y = t * w + b; stats [rows][2] = (m, r), kept for the other two.
+ * gan_layernorm_fwd : y = t * w + b; stats [rows][2] = (m, r), kept for the other two (NULL: not wanted).
  * gan_layernorm_bwd : gx = r P(g w); gwb [2][D] = (sum over rows of g t, of g).  Either may be NULL (skipped).
  * gan_layernorm_bwd2: the gradients of <v, gx> + <cw, gwb[0]> + <cb, gwb[1]> with respect to g (gg), x (gxx) and w (gww [D]);
  *                     any output may be NULL, cw and cb may be NULL (no such cotangent).

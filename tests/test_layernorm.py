@@ -297,6 +297,26 @@ def test_same_bits_other_stream_and_graph(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,d", [(1, 1), (5, 24), (3, 700), (4, 5000), (2, 40000)])
+def test_without_gradients(dev, rows, d, dt):
+    """Where nothing asks for a gradient the same bits come back and nothing is kept."""
+    from gan_amd import functional as GF
+
+    torch.manual_seed(rows + d)
+    x = torch.randn(rows, d, device=dev).to(dt)
+    w, b = torch.randn(d, device=dev, requires_grad=True), torch.randn(d, device=dev, requires_grad=True)
+    want = GF.layer_norm(x, d, w, b)
+    assert want.requires_grad
+    with torch.no_grad():
+        got = GF.layer_norm(x, d, w, b)
+    assert not got.requires_grad and torch.equal(got, want)
+    assert torch.equal(GF.layer_norm(x, d, w.detach(), b.detach()), want)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError):
+        GF.layer_norm(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), d, w.detach())
+
+
+@pytest.mark.gpu
 def test_third_order_is_refused(dev):
     from gan_amd import functional as GF
 
