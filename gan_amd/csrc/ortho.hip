@@ -34,6 +34,7 @@ constexpr float SP = 16.f;       // |P| and products of two of them <= 4000
 __host__ __device__ inline int64_t up64(int64_t v) { return (v + PAD - 1) / PAD * PAD; }
 
 __device__ __forceinline__ void split(float v, h16& hi, h16& lo) {
+    asm("" : "+v"(v));  // (an fp32 value: a product fused into one of the conversions and rounded in front of the other gives halves that do not fit)
     hi = (h16)v;
     lo = (h16)(v - (float)hi);
 }
@@ -376,7 +377,7 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int 
         const int on = j0 + (lane & 31) - i0 - 4 * (lane >> 5);  // the row of the diagonal
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            acc[r] = acc[r] * c + bb * ((float)ah[r >> 2][r & 3] + (float)al[r >> 2][r & 3]) + (on == 8 * (r >> 2) + (r & 3) ? aa : 0.f);
+            acc[r] = fmaf((float)ah[r >> 2][r & 3], bb, fmaf((float)al[r >> 2][r & 3], bb, acc[r] * c)) + (on == 8 * (r >> 2) + (r & 3) ? aa : 0.f);
     } else {
         const float gain = q.kind == SCALED ? q.gain : 1.f / (SP * SX);
 #pragma unroll
@@ -924,12 +925,18 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
 }
 
 // ---- matrices that fit into LDS: one workgroup of sixteen waves each does everything, in one launch ---------------------------
-// Of X two copies are wanted, [m][n] for A = X X' and [n][m] for P X; the first one's place holds A and then P in between.  A
-// product's results wait in registers (two 32 x 32 blocks a wave) until everyone has read the operands that they replace.
-// Rows are 8 elements longer than they are, which spreads any sixteen of them over the banks.  The launches of the general
-// path cost about 5 us each, seventeen of them for five steps; a product of 128 x 128 matrices takes 2 us here.
+// X lies there once, as [n][m]: P X reads it along the rows, A = X X' through transposing reads; A, then P, lie behind it, their
+// blocks on and below the diagonal only (what lies above is read transposed).  A row is made of 128-byte lines, of 32 elements
+// the hi and then the lo halves, and 16 bytes more: sixteen rows at one place, and four rows four apart over 64 bytes, then lie
+// in different banks; neighbouring rows lie four apart (slot_of), so that a transposing read takes them in their order.  A
+// product's results wait in registers (one or two 32 x 32 blocks a wave) until everyone has read the operands that they replace.
+// The vector instructions around the products (halves, addresses) take as long as the products, and all of it is fetched cold
+// once: little code, and addresses of one number a lane and constants.  Five iterations: 16 x 144 18 us, 128 x 128 39 us (a step
+// 6.6 us, of which A, A A and P X take 1.3 + 1.5 + 1.8), 64 x 512 41 us where the launches of the general path (5 to 8 us each) took
+// 100; 512 matrices of 64 x 512 102 us (320).
 constexpr int SMALL_LDS = 160 * 1024 - 512;
-constexpr int SMALL_ELEMS = 20;  // source elements a thread
+constexpr int SMALL_BLOCKS = 32;                   // of 32 x 32, of X: two a wave
+constexpr int SMALL_QUADS = SMALL_BLOCKS * 256 / 1024;  // a thread's groups of four source elements
 
 struct SmallMat {
     const void* g;
@@ -945,32 +952,118 @@ struct Smalls {
 
 __host__ __device__ inline int up32(int v) { return (v + 31) & ~31; }
 
-bool is_small(const gan_matrix& g) {
-    const int64_t m = g.rows < g.cols ? g.rows : g.cols, n = g.rows < g.cols ? g.cols : g.rows;
-    if (n > 4096) return false;
-    const int64_t mp = up32((int)m), np = up32((int)n);
-    return (mp * (np + 8) + np * (mp + 8)) * 4 <= SMALL_LDS && g.rows * g.cols <= SMALL_ELEMS * 1024 && mp * np <= 32 * 1024;
+int small_bytes(int64_t rows, int64_t cols) {
+    const int m = up32((int)(rows < cols ? rows : cols)), n = up32((int)(rows < cols ? cols : rows));
+    return (m + n) * (m * 4 + 16);
 }
 
-// blocks wave, wave + 16 of a bm x bn grid of 32 x 32 blocks: acc += U V' over k, rows of U and V `lu` and `lv` elements long
-__device__ __forceinline__ void small_product(f32x16 (&acc)[2], const h16* u, int lu, int pu, const h16* v, int lv, int pv, int bm, int bn, int k) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+bool is_small(const gan_matrix& g) {
+    if (g.rows > 1024 || g.cols > 1024) return false;
+    return up32((int)g.rows) * up32((int)g.cols) <= SMALL_BLOCKS * 1024 && small_bytes(g.rows, g.cols) <= SMALL_LDS;
+}
+
+// Where row `row` lies: of sixteen rows 4 a + b at place 4 b + a.
+__device__ __forceinline__ int slot_of(int row) { return (row & ~15) | (row & 3) << 2 | ((row >> 2) & 3); }
+
+// A matrix in LDS at byte `base` (a number, not a pointer: every address is then known to lie in LDS), and the lane's places in it
+struct SmallView {
+    unsigned base, pitch, row, col;
+    __device__ __forceinline__ SmallView(unsigned b, int mp, int lane)
+        : base(b), pitch(mp * 4 + 16), row(slot_of(lane & 31) * pitch + (lane >> 5) * 16),
+          col(((lane >> 5) * 2 + (lane & 12)) * pitch + ((lane >> 4) & 1) * 32 + (lane & 3) * 8) {}
+    template <typename V>
+    static __device__ __forceinline__ __attribute__((address_space(3))) V& value(unsigned at) {
+        return *(__attribute__((address_space(3))) V*)(uintptr_t)at;
+    }
+    // the 16 elements from column 16 kk of rows 32 blk ...: a lane row lane & 31 and eight of them
+    __device__ __forceinline__ h16x8 along(int blk, int kk, int pl) const {
+        return value<h16x8>(base + blk * 32 * pitch + kk / 2 * 128 + row + kk % 2 * 32 + pl * 64);
+    }
+    // the same of the transpose: places 0 4 8 12, 1 5 9 13 of the sixteen rows from 16 kk (lanes from 32 on: 2 ..., 3 ...)
+    __device__ __forceinline__ h16x8 across(int blk, int kk, int pl) const {
+        typedef __attribute__((ext_vector_type(4))) short s16x4;
+        const unsigned p = base + kk * 16 * pitch + blk * 128 + col;
+        const h16x4 a = __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(&value<s16x4>(p + pl * 64))),
+                    b = __builtin_bit_cast(h16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(&value<s16x4>(p + pitch + pl * 64)));
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+    // four values from column `col` (a multiple of four) on, of row `at`
+    __device__ __forceinline__ void store(unsigned at, int col, const float (&v)[4]) const {
+        h16x4 hi, lo;
 #pragma unroll
-    for (int z = 0; z < 2; ++z) {
-        const int blk = wave + 16 * z;
-        if (blk >= bm * bn) break;
-        const int bi = blk % bm, bj = blk / bm;
-        const h16 *pu_ = u + (bi * 32 + (lane & 31)) * lu + (lane >> 5) * 8, *pv_ = v + (bj * 32 + (lane & 31)) * lv + (lane >> 5) * 8;
+        for (int e = 0; e < 4; ++e) {
+            h16 x, y;
+            split(v[e], x, y);
+            hi[e] = x;
+            lo[e] = y;
+        }
+        const unsigned to = at + (col >> 5) * 128 + (col & 31) * 2;
+        value<h16x4>(to) = hi;
+        value<h16x4>(to + 64) = lo;
+    }
+    // block (bi, bj) of a product, as accumulated: stored transposed
+    __device__ __forceinline__ void store(int bi, int bj, const f32x16& a, float gain) const {
+        const unsigned to = base + bj * 32 * pitch + bi * 128 + place();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[z][r] = 0.f;
-        for (int kk = 0; kk < k; kk += 16) {
-            const h16x8 uh = *(const h16x8*)(pu_ + kk), ul = *(const h16x8*)(pu_ + pu + kk);
-            const h16x8 vh = *(const h16x8*)(pv_ + kk), vl = *(const h16x8*)(pv_ + pv + kk);
-            acc[z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, vl, acc[z], 0, 0, 0);
-            acc[z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ul, vh, acc[z], 0, 0, 0);
-            acc[z] = __builtin_amdgcn_mfma_f32_32x32x16_f16(uh, vh, acc[z], 0, 0, 0);
+        for (int r = 0; r < 4; ++r) {
+            const float v[4] = {gain * a[r * 4], gain * a[r * 4 + 1], gain * a[r * 4 + 2], gain * a[r * 4 + 3]};
+            store(to, 8 * r, v);
         }
     }
+    // of that block: the lane's column, its first row
+    __device__ __forceinline__ unsigned place() const { return row - (threadIdx.x & 32) / 4; }
+};
+
+// A wave's products over the k from 32 from to 32 end: a block of rows `ub` of U by `vb` of V, or by U's own (B = 0), or by two
+// blocks of V, vb and vb + 1 (B = 2).  TU, TV: k runs down the columns.  The next 16 are read while one is multiplied, with no
+// branch in between (behind one, a wait would be for all reads).  A single block has an accumulator for hi hi and one for the
+// others.
+template <bool TU, bool TV, int B>
+__device__ __forceinline__ void small_part(f32x16 (&acc)[2], const SmallView& U, int ub, const SmallView& V, int vb, int from, int end) {
+    if (from >= end) return;
+    struct Pieces {
+        h16x8 u[2], v[2], w[2];
+    } f[2];
+    auto read = [&](Pieces& p, int kk) __attribute__((always_inline)) {
+#pragma unroll
+        for (int pl = 0; pl < 2; ++pl) {
+            p.u[pl] = TU ? U.across(ub, kk, pl) : U.along(ub, kk, pl);
+            if (B) p.v[pl] = TV ? V.across(vb, kk, pl) : V.along(vb, kk, pl);
+            if (B == 2) p.w[pl] = V.along(vb + 1, kk, pl);
+        }
+    };
+    auto multiply = [&](const Pieces& p) __attribute__((always_inline)) {
+        const h16x8(&u)[2] = p.u, (&v)[2] = B ? p.v : p.u, (&w)[2] = p.w;
+        if (B == 2) {
+            acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[0], v[1], acc[0], 0, 0, 0);
+            acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[0], w[1], acc[1], 0, 0, 0);
+            acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[1], v[0], acc[0], 0, 0, 0);
+            acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[1], w[0], acc[1], 0, 0, 0);
+            acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[0], v[0], acc[0], 0, 0, 0);
+            acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[0], w[0], acc[1], 0, 0, 0);
+        } else {
+            acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[0], v[1], acc[1], 0, 0, 0);
+            acc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[0], v[0], acc[0], 0, 0, 0);
+            acc[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u[1], v[0], acc[1], 0, 0, 0);
+        }
+    };
+    read(f[0], 2 * from);
+    int k = from;
+#pragma unroll 1
+    for (; k + 1 < end; ++k) {
+        read(f[1], 2 * k + 1);
+        multiply(f[0]);
+        read(f[0], 2 * k + 2);
+        multiply(f[1]);
+    }
+    read(f[1], 2 * k + 1);
+    multiply(f[0]);
+    multiply(f[1]);
+}
+
+__device__ __forceinline__ void clear(f32x16 (&acc)[2]) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[0][r] = acc[1][r] = 0.f;
 }
 
 template <typename T>
@@ -982,170 +1075,177 @@ __global__ void __launch_bounds__(1024) ortho_small_k(const Smalls s, const Sour
     const int rows = q.rows, cols = q.cols, size = rows * cols;
     const int64_t b = (int)blockIdx.x - s.first[group];
     const bool wide = rows <= cols;
-    const int mp = up32(wide ? rows : cols), np = up32(wide ? cols : rows), lm = np + 8, lt = mp + 8, la = mp + 8;
-    const int pm = mp * lm, pt = np * lt, pa = mp * la;  // from hi to lo plane
-    h16 *xm = (h16*)lds, *xt = xm + 2 * pm, *sq = xm;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // ---- source: momentum, norm, planes
+    const int m = wide ? rows : cols, n = wide ? cols : rows, mp = up32(m), np = up32(n);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    SmallView X((unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds, mp, lane), Q(X.base + np * X.pitch, mp, lane);
+    // ---- source: momentum, norm, planes.  A thread has groups of four elements i ... i + 3 of a column j of X, neighbours in
+    // memory beside each other's; zeros past the matrix.
     const T* g = (const T*)q.g + b * size;
     float* buf = q.buf ? q.buf + b * size : nullptr;
-    float val[SMALL_ELEMS];
+    auto element = [](auto* of, unsigned i) __attribute__((always_inline)) -> auto& {  // (32 bits of offset: one instruction less or four each)
+        return *(decltype(of))((const char*)of + i * (unsigned)sizeof(*of));
+    };
+    const int fast = wide ? np : mp / 4, quads = mp * np / 4, slow0 = tid / fast, fast0 = tid - slow0 * fast, dslow = 1024 / fast,
+              dfast = 1024 - dslow * fast;
+    auto each = [&](auto&& f) __attribute__((always_inline)) {
+        int a = slow0, c = fast0;
 #pragma unroll
-    for (int k = 0; k < SMALL_ELEMS; ++k) {
-        const int i = k * 1024 + tid;
-        val[k] = i < size ? (float)g[i] : 0.f;
-    }
+        for (int k = 0; k < SMALL_QUADS; ++k) {
+            if (k * 1024 >= quads) break;
+            f(k, wide ? c : a, 4 * (wide ? a : c));
+            c += dfast;
+            a += dslow;
+            if (c >= fast) {
+                c -= fast;
+                ++a;
+            }
+        }
+    };
+    const unsigned di = wide ? cols : 1, dj = wide ? 1 : cols;
+    float val[SMALL_QUADS][4];
+    // (what is outside: the first element instead, cleared afterwards, so that no load stands behind a branch)
+    each([&](int k, int j, int i) __attribute__((always_inline)) {
+        const unsigned at = i * di + j * dj;
+        const int in = j < n ? m - i : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) val[k][e] = (float)element(g, e < in ? at + e * di : 0u);
+    });
     if (buf) {
-        float m[SMALL_ELEMS];
+        float old[SMALL_QUADS][4];
+        each([&](int k, int j, int i) __attribute__((always_inline)) {
+            const unsigned at = i * di + j * dj;
+            const int in = j < n ? m - i : 0;
 #pragma unroll
-        for (int k = 0; k < SMALL_ELEMS; ++k) {
-            const int i = k * 1024 + tid;
-            m[k] = i < size ? buf[i] : 0.f;
-        }
+            for (int e = 0; e < 4; ++e) old[k][e] = element(buf, e < in ? at + e * di : 0u);
+        });
+        each([&](int k, int j, int i) __attribute__((always_inline)) {
+            const unsigned at = i * di + j * dj;
+            const int in = j < n ? m - i : 0;
 #pragma unroll
-        for (int k = 0; k < SMALL_ELEMS; ++k) {
-            const int i = k * 1024 + tid;
-            m[k] = fmaf(h.mu, m[k], (1.f - h.mu) * val[k]);
-            val[k] = update_of(h, val[k], m[k]);
-            if (i < size) buf[i] = m[k];
-        }
+            for (int e = 0; e < 4; ++e) {
+                const float u = fmaf(h.mu, old[k][e], (1.f - h.mu) * val[k][e]);
+                val[k][e] = update_of(h, val[k][e], u);
+                if (e < in) element(buf, at + e * di) = u;
+            }
+        });
     }
-    for (int i = tid; i < (2 * pm + 2 * pt) / 8; i += 1024) ((uint4*)lds)[i] = make_uint4(0u, 0u, 0u, 0u);
     double sum = 0.;
+    each([&](int k, int j, int i) __attribute__((always_inline)) {
+        const int in = j < n ? m - i : 0;
 #pragma unroll
-    for (int k = 0; k < SMALL_ELEMS; ++k) sum += (double)val[k] * (double)val[k];
+        for (int e = 0; e < 4; ++e) {
+            val[k][e] = e < in ? val[k][e] : 0.f;
+            sum = fma((double)val[k][e], (double)val[k][e], sum);
+        }
+    });
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
     if (lane == 0) red[wave] = sum;
     __syncthreads();
     sum = 0.;
 #pragma unroll
     for (int w = 0; w < 16; ++w) sum += red[w];
-    const double n = sqrt(sum);
-    const float scale = n < 1e300 ? (float)((double)SX / (n > (double)h.eps ? n : (double)h.eps)) : __builtin_nanf("");
+    const double norm = sqrt(sum);
+    const float scale = norm < 1e300 ? (float)((double)SX / (norm > (double)h.eps ? norm : (double)h.eps)) : __builtin_nanf("");
+    each([&](int k, int j, int i) __attribute__((always_inline)) {
+        float v[4];
 #pragma unroll
-    for (int k = 0; k < SMALL_ELEMS; ++k) {
-        const int e = k * 1024 + tid;
-        if (e < size) {
-            const int r = e / cols, c = e - r * cols, i = wide ? r : c, j = wide ? c : r;
-            h16 hi, lo;
-            split(val[k] * scale, hi, lo);
-            xm[i * lm + j] = xt[j * lt + i] = hi;
-            xm[pm + i * lm + j] = xt[pt + j * lt + i] = lo;
-        }
-    }
+        for (int e = 0; e < 4; ++e) v[e] = scale * val[k][e];
+        if (k * 1024 + tid < quads) X.store(X.base + slot_of(j) * X.pitch, i, v);
+    });
     __syncthreads();
-    // ---- iterations; lane holds column lane & 31, rows 8 r + 4 (lane >> 5) ... + 3 of a block
+    // ---- iterations; lane holds column lane & 31, rows 8 r + 4 (lane >> 5) ... + 3 of a block, which is stored transposed
     const int bm = mp / 32, bn = np / 32;
+    int si = wave, sj = 0;  // of the blocks (si <= sj) of a symmetric product
+    while (si > sj) si -= ++sj;
+    const bool square = sj < bm;
+    // Of P X two blocks with the same rows of P a wave where there are more of them than waves.  (Where they are not needed, pairs read
+    // less of LDS but leave waves idle that hide what the others wait for: 128 x 128 3990 clocks alone, 4530 in pairs.)
+    const bool pairs = bm * bn > 16;
+    const int ai = wave % bm, aj = wave / bm * (pairs ? 2 : 1);
+    const bool apply = aj < bn, two = pairs && aj + 1 < bn;
     f32x16 acc[2];
+#pragma unroll 1
     for (int step = 0; step < s.steps; ++step) {
-        small_product(acc, xm, lm, pm, xm, lm, pm, bm, bm, np);
+        // (sums of these are not kept from one step to the next: there are no registers for them)
+        asm volatile("" : "+v"(X.row), "+v"(X.col), "+v"(Q.row), "+v"(Q.col));
+        if (square) {
+            clear(acc);
+            if (si == sj) small_part<true, true, 0>(acc, X, si, X, sj, 0, bn);
+            else small_part<true, true, 1>(acc, X, si, X, sj, 0, bn);
+            acc[0] += acc[1];
+            Q.store(si, sj, acc[0], SA / (SX * SX));
+        }
         __syncthreads();
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            const int blk = wave + 16 * z;
-            if (blk >= bm * bm) break;
-            h16* to = sq + (blk / bm * 32 + (lane & 31)) * la + blk % bm * 32 + 4 * (lane >> 5);  // (symmetric: stored transposed)
+        if (square) {
+            clear(acc);
+            const int below = si + 1, above = sj + 1, end = bm;
+            if (si == sj) {
+                small_part<false, false, 0>(acc, Q, si, Q, sj, 0, below);
+                small_part<true, true, 0>(acc, Q, si, Q, sj, below, end);
+            } else {
+                small_part<false, false, 1>(acc, Q, si, Q, sj, 0, below);
+                small_part<true, false, 1>(acc, Q, si, Q, sj, below, above);
+                small_part<true, true, 1>(acc, Q, si, Q, sj, above, end);
+            }
+            acc[0] += acc[1];
+            const unsigned A = Q.base + sj * 32 * Q.pitch + si * 128 + Q.place();
+            const float cc = o.c * (SP / (SA * SA)), bb = o.b * (SP / SA);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                h16x4 hi, lo;
+                const h16x4 ah = Q.value<h16x4>(A + 16 * r), al = Q.value<h16x4>(A + 16 * r + 64);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    h16 x, y;
-                    split(acc[z][r * 4 + e] * (SA / (SX * SX)), x, y);
-                    hi[e] = x;
-                    lo[e] = y;
-                }
-                *(h16x4*)(to + 8 * r) = hi;
-                *(h16x4*)(to + pa + 8 * r) = lo;
+                for (int e = 0; e < 4; ++e) acc[0][r * 4 + e] = fmaf((float)ah[e], bb, fmaf((float)al[e], bb, acc[0][r * 4 + e] * cc));
+            }
+            if (si == sj) {
+                const int on = (lane & 31) - 4 * (lane >> 5);  // the row of the diagonal
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[0][r] += on == 8 * (r >> 2) + (r & 3) ? o.a * SP : 0.f;
             }
         }
         __syncthreads();
-        small_product(acc, sq, la, pa, sq, la, pa, bm, bm, mp);
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            const int blk = wave + 16 * z;
-            if (blk >= bm * bm) break;
-            const int i0 = blk % bm * 32 + 4 * (lane >> 5), j = blk / bm * 32 + (lane & 31);
-            const h16* from = sq + j * la + i0;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const h16x4 ah = *(const h16x4*)(from + 8 * r), al = *(const h16x4*)(from + pa + 8 * r);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    acc[z][r * 4 + e] = acc[z][r * 4 + e] * (o.c * (SP / (SA * SA))) + o.b * (((float)ah[e] + (float)al[e]) * (SP / SA)) +
-                                        (i0 + 8 * r + e == j ? o.a * SP : 0.f);
+        if (square) Q.store(si, sj, acc[0], 1.f);
+        __syncthreads();
+        if (apply) {
+            clear(acc);
+            const int below = ai + 1, end = bm;
+            if (two) {
+                small_part<false, false, 2>(acc, Q, ai, X, aj, 0, below);
+                small_part<true, false, 2>(acc, Q, ai, X, aj, below, end);
+            } else {
+                small_part<false, false, 1>(acc, Q, ai, X, aj, 0, below);
+                small_part<true, false, 1>(acc, Q, ai, X, aj, below, end);
+                acc[0] += acc[1];
             }
         }
-        __syncthreads();
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            const int blk = wave + 16 * z;
-            if (blk >= bm * bm) break;
-            h16* to = sq + (blk / bm * 32 + (lane & 31)) * la + blk % bm * 32 + 4 * (lane >> 5);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                h16x4 hi, lo;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    h16 x, y;
-                    split(acc[z][r * 4 + e], x, y);
-                    hi[e] = x;
-                    lo[e] = y;
-                }
-                *(h16x4*)(to + 8 * r) = hi;
-                *(h16x4*)(to + pa + 8 * r) = lo;
-            }
-        }
-        __syncthreads();
-        small_product(acc, sq, la, pa, xt, lt, pt, bm, bn, mp);
         if (step + 1 == s.steps) break;
         __syncthreads();
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            const int blk = wave + 16 * z;
-            if (blk >= bm * bn) break;
-            const int i0 = blk % bm * 32 + 4 * (lane >> 5), j = blk / bm * 32 + (lane & 31);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                h16x4 hi, lo;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    h16 x, y;
-                    split(acc[z][r * 4 + e] * (1.f / SP), x, y);
-                    hi[e] = x;
-                    lo[e] = y;
-                    xm[(i0 + 8 * r + e) * lm + j] = x;
-                    xm[pm + (i0 + 8 * r + e) * lm + j] = y;
-                }
-                *(h16x4*)(xt + j * lt + i0 + 8 * r) = hi;
-                *(h16x4*)(xt + pt + j * lt + i0 + 8 * r) = lo;
-            }
+        if (apply) {
+            X.store(ai, aj, acc[0], 1.f / SP);
+            if (two) X.store(ai, aj + 1, acc[1], 1.f / SP);
         }
         __syncthreads();
     }
+    if (!apply) return;
     const float shaped = o.update ? step_of(o, rows, cols) : 0.f;
+    T* out = (T*)q.out + b * size;
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
-        const int blk = wave + 16 * z;
-        if (blk >= bm * bn) break;
-        const int i0 = blk % bm * 32 + 4 * (lane >> 5), j = blk / bm * 32 + (lane & 31);
+        if (z && !two) break;
+        const int i0 = ai * 32 + 4 * (lane >> 5), j = (aj + z) * 32 + (lane & 31), in = j < n ? m - i0 : 0;
+        const unsigned at = i0 * di + j * dj;
         float old[16];
         if (o.update) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int i = i0 + 8 * (r >> 2) + (r & 3), row = wide ? i : j, col = wide ? j : i;
-                old[r] = row < rows && col < cols ? ((const float*)q.out)[b * size + row * cols + col] : 0.f;
+                const int e = 8 * (r >> 2) + (r & 3);
+                old[r] = (float)element(out, e < in ? at + e * di : 0u);
             }
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int i = i0 + 8 * (r >> 2) + (r & 3), row = wide ? i : j, col = wide ? j : i;
-            if (row < rows && col < cols) {
-                const float x = acc[z][r] * (1.f / (SP * SX));
-                const int64_t at = b * size + row * cols + col;
-                if (o.update) ((float*)q.out)[at] = fmaf(-shaped, x, o.decay * old[r]);
-                else ((T*)q.out)[at] = (T)x;
-            }
+            const int e = 8 * (r >> 2) + (r & 3);
+            const float x = acc[z][r] * (1.f / (SP * SX));
+            if (e < in) element(out, at + e * di) = (T)(o.update ? fmaf(-shaped, x, o.decay * old[r]) : x);
         }
     }
 }
@@ -1161,8 +1261,7 @@ int run_small(const gan_matrix* mats, int n, int steps, const Source& h, const R
         s.mat[k] = SmallMat{g.g, g.buf, g.out, (int)g.rows, (int)g.cols};
         s.first[k] = blocks;
         blocks += (int)g.batch;
-        const int m = up32((int)(g.rows < g.cols ? g.rows : g.cols)), w = up32((int)(g.rows < g.cols ? g.cols : g.rows));
-        const int need = (m * (w + 8) + w * (m + 8)) * 4;
+        const int need = small_bytes(g.rows, g.cols);
         lds = need > lds ? need : lds;
     }
     // more than 64 KB of dynamic LDS needs the attribute (set on every call: it is per device, and cheap)

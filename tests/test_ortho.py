@@ -49,7 +49,7 @@ def make(m, n, dev, seed=0, dt=torch.float32, kind="gauss"):
     return x.to(dt).to(dev)
 
 
-SIZES = [(1, 1), (1, 7), (9, 1), (2, 3), (16, 144), (144, 16), (63, 65), (64, 64), (65, 200), (200, 129), (128, 128), (130, 1000), (777, 300), (512, 1300), (257, 2304)]
+SIZES = [(1, 1), (1, 7), (9, 1), (2, 3), (16, 144), (144, 16), (63, 65), (64, 64), (65, 200), (200, 129), (128, 128), (130, 1000), (777, 300), (512, 1300), (257, 2304), (64, 512), (1024, 20), (97, 128), (128, 160), (33, 500), (96, 310)]
 
 
 @pytest.mark.gpu
