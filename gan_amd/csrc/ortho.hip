@@ -95,16 +95,17 @@ struct Lay {
     int cut;
 };
 
-// What a product of `tiles` T x T tiles over `steps` steps of 32 k takes, in us, every tile's k in `cut` slices: workgroups run
-// in rounds, 256 (T = 256) or 512 of them at a time, a step of theirs as long as measured (T = 256: 2.45; T = 128: 0.42 alone
-// on a CU, 0.62 each where two share it; T = 64: 0.19 and 0.2), a round begins and ends in 5 to 9 us, and slices are written and
-// read again at 5 TB/s by one more launch.
+// What a product of `tiles` T x T tiles over `steps` steps of 32 k takes, in us, every tile's k in `cut` slices: a CU holds one, two
+// or five workgroups (T = 256, 128, 64) at a time, a step of all of them takes as long as measured (2.45; 0.42 alone, 0.62 each where
+// two share the CU; 0.19 and 0.2), a round begins and ends in 5 to 9 us, and slices are written and read again at 5 TB/s by one
+// more launch.
 double cost_of(int T, int64_t tiles, int cut, int64_t steps) {
-    const int64_t wgs = tiles * cut, slots = T < 256 && wgs > 256 ? 512 : 256, left = wgs % slots;
-    const double alone = T == 256 ? 2.45 : T == 128 ? 0.42 : 0.19, shared = T == 128 ? 1.25 : 0.4, ends = T == 256 ? 9. : T == 128 ? 7. : 5.;
+    const int hold = T == 256 ? 1 : T == 128 ? 2 : 5;
+    const double alone = T == 256 ? 2.45 : T == 128 ? 0.42 : 0.19, each = T == 128 ? 0.62 : 0.2, ends = T == 64 ? 5. : 9.;
+    const int64_t wgs = tiles * cut, on_cu = ceil_div64(wgs % (256 * hold), 256);
     const double n = (double)ceil_div64(steps, cut);
-    return (double)(wgs / slots) * (n * (slots == 512 ? shared : alone) + ends) + (left ? n * (left > 256 ? shared : alone) + ends : 0.) +
-           (cut > 1 ? 5. + (double)wgs * T * T * 8e-6 / 5. : 0.);
+    auto round = [&](int64_t p) { return p ? n * (p == 1 ? alone : (double)p * each) + ends : 0.; };
+    return (double)(wgs / (256 * hold)) * round(hold) + round(on_cu) + (cut > 1 ? 5. + (double)wgs * T * T * 8e-6 / 5. : 0.);
 }
 
 int64_t tiles_of(int64_t M, int64_t N, bool sym, int T) {
