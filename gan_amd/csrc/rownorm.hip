@@ -231,33 +231,47 @@ __global__ void __launch_bounds__(block_of<TPR>()) ln_fwd_k(const RowArgs a) {
     }
 }
 
-// Column sums of the row groups of one workgroup, added one group after another, then written as its partial row.
+// Column sums of the row groups of one workgroup: of a wave's groups by exchange between lanes, of the waves through LDS in their
+// order, then written as the workgroup's partial row.  (One group after another through LDS: 12 us of the 38 that the pass over
+// 131072 x 128 bf16 takes; like this 2.)
 template <int NC, int V, int K, int TPR>
-__device__ __forceinline__ void write_partials(float (&acc)[NC][K][V], float* part, int lane, int grp, int D) {
-    constexpr int G = block_of<TPR>() / TPR;
-    extern __shared__ float cols[];  // [NC][D] for G > 1
+__device__ __forceinline__ void write_partials(float (&acc)[NC][K][V], float* part, int lane, int D) {
+    constexpr int G = block_of<TPR>() / TPR, W = TPB / 64, DP = K * TPR * V;
     float* out = part + (int64_t)blockIdx.x * NC * D;
-    for (int gi = 0; gi < G; ++gi) {
-        if (grp == gi) {
+    if constexpr (G == 1) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const int c = (lane + k * TPR) * V + e;
-                    if (c < D) {
+                    if (c < D) out[(int64_t)j * D + c] = acc[j][k][e];
+                }
+    } else {
+        __shared__ __attribute__((aligned(16))) float cols[W][NC][DP];
+        const int wave = threadIdx.x >> 6;
 #pragma unroll
-                        for (int j = 0; j < NC; ++j) {
-                            const float s = G > 1 && gi > 0 ? cols[j * D + c] + acc[j][k][e] : acc[j][k][e];
-                            if (gi == G - 1)
-                                out[(int64_t)j * D + c] = s;
-                            else
-                                cols[j * D + c] = s;
-                        }
-                    }
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+#pragma unroll
+                    for (int off = TPR; off < 64; off *= 2) acc[j][k][e] += __shfl_xor(acc[j][k][e], off);
+                if ((threadIdx.x & 63) < TPR) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) cols[wave][j][(lane + k * TPR) * V + e] = acc[j][k][e];
                 }
             }
+        __syncthreads();
+        for (int i = threadIdx.x; i < NC * DP; i += TPB) {
+            const int j = i / DP, c = i % DP;
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) s += cols[w][j][c];
+            if (c < D) out[(int64_t)j * D + c] = s;
         }
-        if (G > 1) __syncthreads();
     }
 }
 
@@ -393,7 +407,7 @@ __global__ void __launch_bounds__(block_of<TPR>()) ln_bwd_k(const RowArgs a) {
             g.store((T*)a.y + row * D, lane, D);
         }
     }
-    if constexpr (COLS == 1) write_partials<2, V, K, TPR>(acc, a.part, lane, grp, D);
+    if constexpr (COLS == 1) write_partials<2, V, K, TPR>(acc, a.part, lane, D);
 }
 
 // ---- second order ------------------------------------------------------------------------------------------------
@@ -491,7 +505,7 @@ __global__ void __launch_bounds__(block_of<TPR>()) ln_bwd2_k(const RowArgs a) {
         if (a.y) v.store((T*)a.y + row * D, lane, D);
         if (a.y2) x.store((T*)a.y2 + row * D, lane, D);
     }
-    if constexpr (COLS == 1) write_partials<1, V, K, TPR>(acc, a.part, lane, grp, D);
+    if constexpr (COLS == 1) write_partials<1, V, K, TPR>(acc, a.part, lane, D);
 }
 
 // ---- long rows: pieces of a row sum, then join and write -----------------------------------------------------------
@@ -650,18 +664,26 @@ __global__ void __launch_bounds__(TPB) ln_long_apply_k(const RowArgs a) {
 // The first `split` columns go to out0, the others to out1 (either may be NULL).
 __global__ void __launch_bounds__(1024) fold_cols_k(const float* __restrict__ part, int n, int64_t width, float* __restrict__ out0,
                                                     float* __restrict__ out1, int64_t split) {
-    __shared__ float red[64][17];
+    __shared__ float red[16][17];
+    constexpr int AHEAD = 8;  // rows requested at a time
     const int c = threadIdx.x & 15, sl = threadIdx.x >> 4;
-    const int64_t col = (int64_t)blockIdx.x * 16 + c;
+    const int64_t col = (int64_t)blockIdx.x * 16 + c, in = col < width ? col : 0;
     float s = 0.f;
-    if (col < width)
-        for (int p = sl; p < n; p += 64) s += part[(int64_t)p * width + col];
-    red[sl][c] = s;
+    for (int p = sl; p < n; p += 64 * AHEAD) {
+        float v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) v[k] = part[(int64_t)(p + 64 * k < n ? p + 64 * k : p) * width + in];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) s += p + 64 * k < n ? v[k] : 0.f;
+    }
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if ((threadIdx.x & 63) < 16) red[threadIdx.x >> 6][c] = s;
     __syncthreads();
     if (sl == 0 && col < width) {
         float t = 0.f;
 #pragma unroll
-        for (int k = 0; k < 64; ++k) t += red[k][c];
+        for (int k = 0; k < 16; ++k) t += red[k][c];
         if (col < split) {
             if (out0) out0[col] = t;
         } else if (out1) {
@@ -681,7 +703,8 @@ struct Plan {
     int64_t floats;  // workspace
 };
 
-constexpr int MAXB = 1024;  // four workgroups of 256 threads a CU
+// Four workgroups of 256 threads a CU; forward, with fewer registers, eight (65536 x 512 bf16: 23.8 us against 26.5).
+constexpr int MAXB = 1024;
 
 // pass 0 forward, 1 backward, 2 second.  cols: column sums wanted.
 Plan plan_of(int64_t rows, int64_t D, int dtype, int pass, bool cols) {
@@ -702,12 +725,13 @@ Plan plan_of(int64_t rows, int64_t D, int dtype, int pass, bool cols) {
     if (p.tpr) {
         const int g = p.tpr >= TPB ? 1 : TPB / p.tpr;
         const int64_t need = ceil_div64(rows, g);
-        p.blocks = (int)(need < MAXB ? need : MAXB);
+        const int64_t many = pass == 0 ? 2 * MAXB : MAXB;
+        p.blocks = (int)(need < many ? need : many);
         if (cols && pass > 0 && p.tpr <= 512) {
             // A partial row of ncol D floats per workgroup is written and read again, next to at least three tensor rows of D
             // elements that a row costs anyway: few enough workgroups keep that under a sixth.  Where so few are left that
             // they would not fill the chip, a kernel down the columns reads the tensors a second time instead.
-            const int64_t most = rows / (dtype == GAN_F32 ? 8 : 16);
+            const int64_t most = rows / ((dtype == GAN_F32 ? 8 : 16) / (pass == 2 && p.tpr <= 256 ? 2 : 1));
             if (most >= 64) {
                 p.fused = true;
                 if (p.blocks > most) p.blocks = (int)most;
@@ -736,15 +760,14 @@ Plan plan_of(int64_t rows, int64_t D, int dtype, int pass, bool cols) {
 template <typename T, int PASS, int COLS, int TPR, int K>
 void launch_row(int blocks, const RowArgs& a, hipStream_t st) {
     constexpr int BLK = block_of<TPR>();
-    const size_t lds = COLS == 1 && TPR < TPB ? sizeof(float) * (PASS == 2 ? 1 : 2) * (size_t)a.D : 0;
     if constexpr (PASS == 0)
         hipLaunchKernelGGL((ln_fwd_k<T, TPR, K>), dim3(blocks), dim3(BLK), 0, st, a);
     else if constexpr (PASS == 1)
-        hipLaunchKernelGGL((ln_bwd_k<T, TPR, K, COLS>), dim3(blocks), dim3(BLK), lds, st, a);
+        hipLaunchKernelGGL((ln_bwd_k<T, TPR, K, COLS>), dim3(blocks), dim3(BLK), 0, st, a);
     else if (a.cw || a.cb)
-        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS, true>), dim3(blocks), dim3(BLK), lds, st, a);
+        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS, true>), dim3(blocks), dim3(BLK), 0, st, a);
     else
-        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS, false>), dim3(blocks), dim3(BLK), lds, st, a);
+        hipLaunchKernelGGL((ln_bwd2_k<T, TPR, K, COLS, false>), dim3(blocks), dim3(BLK), 0, st, a);
 }
 
 template <typename T, int PASS, int COLS>
