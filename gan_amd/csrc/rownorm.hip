@@ -9,12 +9,23 @@
 //             gww = sum_rows g r P(v)
 // All three move a few bytes per flop: HBM bounds them.  Each row is read once and kept in registers, 16 bytes a lane and
 // load, between its statistics and its results; a row belongs to TPR threads (16 and more) with one or two
-// such vectors each (up to 1024 and four in the widest), so that short rows need no LDS and registers leave room for many waves.  Longer rows are cut into pieces
-// that first sum and then, in a second launch, join the sums and write.
+// such vectors each (up to 1024 and four in the widest), so that short rows need no LDS and registers leave room for many waves.
+// Longer rows are cut into pieces that first sum and then, in a second launch, join the sums and write.
 // Column sums: where a workgroup walks over many rows, its threads keep their columns' sums in registers and write one
 // partial row per workgroup (fold_cols_k adds those in a fixed order: no atomics, the same bits on every run); where there
-// are few rows for that, a second kernel goes down the columns.
+// are few rows for that, a second kernel (backward: more workgroups of the same) goes down the columns.
 // Sums and statistics are fp32 throughout; bf16 results are rounded once, on the store.
+// Measured, launches alone, of 5.0 TB/s that a copy reaches (in brackets the bytes' time at that rate):
+//                          forward        backward, x only   and the column sums   second, all three
+//   65536 x 512 bf16       25 us (26.7)   35 (40)            41                    84 (67)
+//   16384 x 512 bf16       7.7 (6.7)      11 (10)            17                    23 (17)
+//   131072 x 128 bf16      12.6 (13.4)    18 (20)            24                    34 (33)
+//   4099 x 1001 fp32       7.7 (6.5)      12 (10)            21                    23 (16)
+//   8192 x 2048 bf16       14 (13.4)      20 (20)            37                    44 (33)
+//   2000 x 8000 fp32       32 (25)        39 (38)            62                    84 (64)
+//   64 x 32768 bf16        9.6 (1.7)      14.6 (2.5)         14.6                  20 (4.2)
+// The column sums of wide rows are what is left: few workgroups (their partial rows cost bytes) that each wait for row after row;
+// asking for the next row ahead, or for two at a time, gained nothing (the wait also covers the stores in between).
 #include "common.h"
 
 namespace {
@@ -729,8 +740,9 @@ Plan plan_of(int64_t rows, int64_t D, int dtype, int pass, bool cols) {
         p.blocks = (int)(need < many ? need : many);
         if (cols && pass > 0 && p.tpr <= 512) {
             // A partial row of ncol D floats per workgroup is written and read again, next to at least three tensor rows of D
-            // elements that a row costs anyway: few enough workgroups keep that under a sixth.  Where so few are left that
-            // they would not fill the chip, a kernel down the columns reads the tensors a second time instead.
+            // elements that a row costs anyway: few enough workgroups keep that under a sixth (second order, with one partial row
+            // against five tensors: twice as many, 8192 x 2048 bf16 54 -> 45 us; rows of 512 threads lose by it, 84 -> 90).  Where so
+            // few are left that they would not fill the chip, a kernel down the columns reads the tensors a second time instead.
             const int64_t most = rows / ((dtype == GAN_F32 ? 8 : 16) / (pass == 2 && p.tpr <= 256 ? 2 : 1));
             if (most >= 64) {
                 p.fused = true;
