@@ -196,6 +196,23 @@ def test_muon_step(dev, nesterov, wd, scaling):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(64, 512), (1024, 20), (96, 288)], [(300, 520), (40, 64, 3, 3)] + [(12, 5, 3, 3)] * 40 + [(129, 128), (700, 90)]])
+def test_muon_step_of_large_and_small(dev, shapes):
+    """Lists that fit into LDS matrix by matrix, and that do not: a long one in several groups, small ones among the others."""
+    from gan_amd.optim import muon_step
+
+    gen = torch.Generator(device="cpu").manual_seed(3)
+    p, g, buf = ([torch.randn(s, generator=gen).to(dev) for s in shapes] for _ in range(3))
+    want = [step_ref(*t, 0.5, 0.9, True, 0.01, "original") for t in zip(p, g, buf)]
+    before = [t.clone() for t in p]
+    muon_step(p, g, buf, lr=0.5, momentum=0.9, weight_decay=0.01)
+    for a, b, m, (wp, wb) in zip(p, before, buf, want):
+        assert rel_err(m, wb) < 1e-6
+        upd, upd_w = a.double().cpu() - b.double().cpu(), wp - b.double().cpu()  # (the bound of test_muon_step)
+        assert float((upd - upd_w).norm()) <= 6e-4 * float(upd_w.norm()) + 2.0**-23 * float(b.norm())
+
+
+@pytest.mark.gpu
 def test_same_bits_other_stream_and_graph(dev):
     from gan_amd import functional as GF
     from gan_amd.optim import muon_step
