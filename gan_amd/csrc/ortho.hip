@@ -278,22 +278,22 @@ __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
 }
 
 // ---- products ----------------------------------------------------------------------------------------------------------
-enum Kind { SCALED, POLY, RESULT };
+enum Kind { SCALED, POLY, CHAIN, RESULT };  // gain U V'; c U V' + b aux + a I; c U V' + b aux + a aux2; the call's result
 
 // C = U V' (or U V) of one group of equal matrices
 struct Op {
     char* ws;          // of the group's first matrix
     int64_t stride;
     void* out;         // RESULT
-    unsigned u, v;     // operands, result, POLY's A, slices: in 256 bytes from ws
-    unsigned to, aux, join;
+    unsigned u, v;     // operands, result, POLY's and CHAIN's further terms, slices: in 256 bytes from ws
+    unsigned to, aux, aux2, join;
     int M, N, K;       // padded
     int apply;         // C = U V with V [K][N] as it lies, not transposed; else C is symmetric: tiles on and above the diagonal
     int rows, cols;    // of the source
     int tiles;         // per matrix
     int cut, steps;    // slices of k, steps of 32 k in each but the last
     int kind;
-    float gain;        // SCALED: result = gain * accumulator
+    float gain;        // of the product; P and what CHAIN adds have the scale SP, POLY's A has SA
 };
 
 // the polynomial, and what becomes of the result
@@ -366,19 +366,34 @@ __device__ __forceinline__ void store_result(const Rule& rule, T* to, float (&o)
 __device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int b, int i0, int j0, f32x16& acc, bool mirror, int dtype, float* t) {
     const int lane = threadIdx.x & 63;
     // the values first, where the accumulators hold them: no branch or load stands between the trips through LDS
-    if (q.kind == POLY) {  // (A is symmetric: its rows for the columns held here)
-        const h16* A = (const h16*)(ws + (int64_t)q.aux * 256) + hi_at(j0 + (lane & 31), i0 + 4 * (lane >> 5), q.N);
-        h16x4 ah[4], al[4];
+    if (q.kind == POLY || q.kind == CHAIN) {  // (what is added is symmetric: its rows for the columns held here)
+        const int64_t at = hi_at(j0 + (lane & 31), i0 + 4 * (lane >> 5), q.N);
+        const h16* A = (const h16*)(ws + (int64_t)q.aux * 256) + at;
+        h16x4 ah[4], al[4], ph[4], pl[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             ah[r] = *(const h16x4*)(A + 8 * r);
             al[r] = *(const h16x4*)(A + LO + 8 * r);
         }
-        const float c = s.rule.c * (SP / (SA * SA)), bb = s.rule.b * (SP / SA), aa = s.rule.a * SP;
-        const int on = j0 + (lane & 31) - i0 - 4 * (lane >> 5);  // the row of the diagonal
+        if (q.kind == CHAIN) {
+            const h16* P = (const h16*)(ws + (int64_t)q.aux2 * 256) + at;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            acc[r] = fmaf((float)ah[r >> 2][r & 3], bb, fmaf((float)al[r >> 2][r & 3], bb, acc[r] * c)) + (on == 8 * (r >> 2) + (r & 3) ? aa : 0.f);
+            for (int r = 0; r < 4; ++r) {
+                ph[r] = *(const h16x4*)(P + 8 * r);
+                pl[r] = *(const h16x4*)(P + LO + 8 * r);
+            }
+        }
+        const float c = s.rule.c * q.gain, bb = s.rule.b * (q.kind == POLY ? SP / SA : 1.f);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] = fmaf((float)ah[r >> 2][r & 3], bb, fmaf((float)al[r >> 2][r & 3], bb, acc[r] * c));
+        if (q.kind == CHAIN) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] = fmaf((float)ph[r >> 2][r & 3], s.rule.a, fmaf((float)pl[r >> 2][r & 3], s.rule.a, acc[r]));
+        } else if (i0 == j0) {
+            const int on = (lane & 31) - 4 * (lane >> 5);  // the row of the diagonal
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] += on == 8 * (r >> 2) + (r & 3) ? s.rule.a * SP : 0.f;
+        }
     } else {
         const float gain = q.kind == SCALED ? q.gain : 1.f / (SP * SX);
 #pragma unroll
@@ -784,58 +799,63 @@ int launch_gemm(unsigned blocks, const Ops& s, int dtype, hipStream_t st) {
 // What a matrix does in the launches, one after another: stages of one or two iterations, each from A = X X' anew.
 //   one:  P = poly(A);                                                     X <- P X
 //   two:  P = poly(A), T = P A, A2 = P T (= X2 X2'), P2 = poly(A2), Q = P2 P;  X <- Q X
+//   two, side by side:  P = poly(A) | T = P A, S = P P | A2 = T P, B = T S (= A2 P) | Q = a P + b B + c A2 B;  X <- Q X
 // Two iterations at a time replace a product with X and one into it by three m x m ones: 6 m^2 n + 2 m^3 against
 // 3 m^2 n + 5 m^3, which pays from n = 2 m on.  Not more at a time: an error of A, 2^-22 of its largest singular value, weighs
 // the more on the smallest ones the longer the iteration runs on A alone (error against 64 bits, 512 x 4608 with a spectrum that
 // falls like 1 / i: 1.9e-6 step by step, 3.1e-6 like this, 7.8e-6 in stages of two and three, 1.7e-4 in one).  The first
 // stage is a single iteration: the small values are smallest there.
+// Side by side is a product more and a launch less: taken where two products of each matrix leave no CU with more than one tile,
+// the launch then being as long as one (512 x 4608: 195 -> 184 us, 704 x 1500 187 -> 178; 1000 x 4000, which has more tiles, gains nothing).
 int stage_of(const Lay& l, int left, int steps) { return l.np >= 2 * l.mp && left < steps && left >= 2 ? 2 : 1; }
 
 struct Walk {
     Lay l;
-    int left, size, at, cur;  // iterations left, this stage's size, the next product within it, the X that holds the iterate
-    void next(Op& q, int steps) {
+    bool beside;              // two iterations: side by side
+    int left, size, at, cur;  // iterations left, this stage's size, the next launch within it, the X that holds the iterate
+    // one or two products
+    int next(Op* q, int steps) {
         if (at == 0) size = stage_of(l, left, steps);
+        int n = 0;
         auto sq = [&](int k) { return (unsigned)(l.sq[k] / 256); };
-        auto mul = [&](int u, int v, int to, float gain) {
-            q.u = sq(u);
-            q.v = sq(v);
-            q.to = sq(to);
-            q.apply = 0;
-            q.gain = gain;
-            q.M = q.N = q.K = (int)l.mp;
+        auto mul = [&](int u, int v, int to, float gain, int kind = SCALED, int aux = 0, int aux2 = 0) {
+            Op& o = q[n++];
+            o.u = sq(u);
+            o.v = sq(v);
+            o.to = sq(to);
+            o.aux = sq(aux);
+            o.aux2 = sq(aux2);
+            o.apply = 0;
+            o.gain = gain;
+            o.kind = kind;
+            o.cut = 1;
+            o.M = o.N = o.K = (int)l.mp;
         };
-        q.kind = SCALED;
-        q.cut = 1;
-        q.aux = 0;
-        const int last = size == 1 ? 2 : 6;
+        const float poly = SP / (SA * SA);
+        const int last = size == 1 ? 2 : beside ? 5 : 6;
         if (at == 0) {
             mul(0, 0, A0, SA / (SX * SX));
-            q.u = q.v = (unsigned)(l.x[cur] / 256);
-            q.K = (int)l.np;
-            q.cut = l.cut;
+            q->u = q->v = (unsigned)(l.x[cur] / 256);
+            q->K = (int)l.np;
+            q->cut = l.cut;
         } else if (at == last) {
-            const bool end = left == size;
-            q.kind = end ? RESULT : SCALED;
-            q.u = sq(size == 1 ? P0 : Q0);
-            q.v = (unsigned)(l.x[cur] / 256);
-            q.to = (unsigned)(l.x[cur ^ 1] / 256);
-            q.apply = 1;
-            q.gain = 1.f / SP;
-            q.M = q.K = (int)l.mp;
-            q.N = (int)l.np;
+            mul(size == 1 ? P0 : Q0, 0, 0, 1.f / SP, left == size ? RESULT : SCALED);
+            q->v = (unsigned)(l.x[cur] / 256);
+            q->to = (unsigned)(l.x[cur ^ 1] / 256);
+            q->apply = 1;
+            q->N = (int)l.np;
         } else if (at == 1) {
-            mul(A0, A0, P0, 0.f);
-            q.kind = POLY;
-            q.aux = sq(A0);
+            mul(A0, A0, P0, poly, POLY, A0);
         } else if (at == 2) {
             mul(P0, A0, Q0, 1.f / SP);
+            if (beside) mul(P0, P0, P1, 1.f / SP);
         } else if (at == 3) {
             mul(P0, Q0, A1, 1.f / SP);
+            if (beside) mul(Q0, P1, A0, 1.f / SA);
+        } else if (beside) {
+            mul(A1, A0, Q0, 1.f / SA, CHAIN, A0, P0);
         } else if (at == 4) {
-            mul(A1, A1, P1, 0.f);
-            q.kind = POLY;
-            q.aux = sq(A1);
+            mul(A1, A1, P1, poly, POLY, A1);
         } else {
             mul(P1, P0, Q0, 1.f / SP);
         }
@@ -844,6 +864,7 @@ struct Walk {
             cur ^= 1;
             at = 0;
         }
+        return n;
     }
 };
 
@@ -854,7 +875,7 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
     int64_t batch[NOPS];
     for (int k = 0; k < n; ++k) {
         Walk& w = walks[k];
-        if (w.left) {
+        for (int left = w.left ? w.next(s.mat + s.count, steps) : 0; left > 0; --left) {
             batch[s.count] = mats[k].batch;
             Op& q = s.mat[s.count++];
             q.ws = ws;
@@ -863,7 +884,6 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
             q.rows = (int)mats[k].rows;
             q.cols = (int)mats[k].cols;
             q.join = (unsigned)(w.l.join / 256);
-            w.next(q, steps);
             q.steps = (int)ceil_div64(q.K / 32, q.cut);
             sliced |= q.cut > 1;
         }
@@ -1402,7 +1422,12 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, const
         int rc = dtype == GAN_F32 ? pack<float>(some, n, at, s, st) : pack<bf16>(some, n, at, s, st);
         if (rc) return rc;
         Walk walks[NOPS];
-        for (int k = 0; k < n; ++k) walks[k] = Walk{lay_of(some[k].rows, some[k].cols), steps, 1, 0, 0};
+        int64_t tiles = 0;
+        for (int k = 0; k < n; ++k) {
+            walks[k] = Walk{lay_of(some[k].rows, some[k].cols), false, steps, 1, 0, 0};
+            tiles += tiles_of(walks[k].l.mp, walks[k].l.mp, true, 64) * some[k].batch;
+        }
+        for (int k = 0; k < n; ++k) walks[k].beside = 2 * n <= NOPS && 2 * tiles <= 256;
         for (bool more = true; more;) {
             if ((rc = products(some, walks, n, steps, o, at, dtype, st))) return rc;
             more = false;
