@@ -105,7 +105,7 @@ double cost_of(int T, int64_t tiles, int cut, int64_t steps) {
     const int64_t wgs = tiles * cut, on_cu = ceil_div64(wgs % (256 * hold), 256);
     const double n = (double)ceil_div64(steps, cut);
     auto round = [&](int64_t p) { return p ? n * (p == 1 ? alone : (double)p * each) + ends : 0.; };
-    return (double)(wgs / (256 * hold)) * round(hold) + round(on_cu) + (cut > 1 ? 5. + (double)wgs * T * T * 8e-6 / 5. : 0.);
+    return (double)(wgs / (256 * hold)) * round(hold) + round(on_cu) + (cut > 1 ? 4. + (double)wgs * T * T * 8e-6 / 5. : 0.);
 }
 
 int64_t tiles_of(int64_t M, int64_t N, bool sym, int T) {
@@ -113,26 +113,26 @@ int64_t tiles_of(int64_t M, int64_t N, bool sym, int T) {
     return sym ? tm * (tm + 1) / 2 : tm * tn;
 }
 
-// Slices of A = X X' (a long k, few tiles), at least eight steps each, by the matrix's own shape (the workspace goes by it).
-int cut_of(int64_t mp, int64_t np) {
+// Slices of A = X X' (a long k, few tiles), at least eight steps each, by the group alone (the workspace goes by it).
+int cut_of(int64_t mp, int64_t np, int64_t batch) {
     int best = 1;
     double least = 1e30;
     for (int T = 64; T <= 256; T *= 2) {
         const int64_t tiles = tiles_of(mp, mp, true, T), steps = np / 32;
-        int64_t cut = 256 / tiles;
-        if (cut > steps / 8) cut = steps / 8;
-        if (cut < 1) cut = 1;
-        const double c = cost_of(T, tiles, (int)cut, steps);
-        if (c < least) {
-            least = c;
-            best = (int)cut;
+        for (int64_t cut = 1; cut == 1 || (cut <= 256 / tiles && cut <= steps / 8); ++cut) {
+            const double c = cost_of(T, tiles * batch, (int)cut, steps);
+            if (c < least) {
+                least = c;
+                best = (int)cut;
+            }
         }
     }
     const int64_t steps = np / 32, each = ceil_div64(steps, best);
     return (int)ceil_div64(steps, each);
 }
 
-Lay lay_of(int64_t rows, int64_t cols) {
+Lay lay_of(const gan_matrix& g) {
+    const int64_t rows = g.rows, cols = g.cols;
     Lay l;
     l.mp = up64(rows < cols ? rows : cols);
     l.np = up64(rows < cols ? cols : rows);
@@ -148,7 +148,7 @@ Lay lay_of(int64_t rows, int64_t cols) {
         at += sq;
     }
     l.join = at;
-    l.cut = cut_of(l.mp, l.np);
+    l.cut = cut_of(l.mp, l.np, g.batch);
     const int64_t t = (l.mp + 255) / 256 * 4;  // in whole tiles of the largest size
     if (l.cut > 1) at += l.cut * t * (t + 4) / 2 * 4096 * 4;
     l.bytes = at;
@@ -1332,7 +1332,7 @@ int64_t total_bytes(const gan_matrix* mats, int count) {
         const gan_matrix& g = mats[k];
         if (g.rows < 1 || g.cols < 1 || g.batch < 0 || g.rows > (1 << 20) || g.cols > (1 << 20) || g.batch > (1 << 30)) return -1;
         if (up64(g.rows) * up64(g.cols) >= (1LL << 30) || (g.rows < g.cols ? g.rows : g.cols) > 32768) return -1;
-        const int64_t one = lay_of(g.rows, g.cols).bytes;
+        const int64_t one = lay_of(g).bytes;
         if (g.batch && one > (1LL << 60) / g.batch) return -1;
         n += one * g.batch;
         if (n > (1LL << 60)) return -1;
@@ -1348,7 +1348,7 @@ int pack(const gan_matrix* mats, int n, char* ws, Mats& s, hipStream_t st) {
     s.count = n;
     for (int k = 0; k < n; ++k) {
         const gan_matrix& g = mats[k];
-        const Lay l = lay_of(g.rows, g.cols);
+        const Lay l = lay_of(g);
         Mat& q = s.mat[k];
         q.g = g.g;
         q.buf = g.buf;
@@ -1394,7 +1394,7 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, const
     for (int k = 0; k < count; ++k) {
         const gan_matrix& g = all[k];
         GAN_CHECK_ARG(!g.batch || (g.g && g.out && (!rule.update || g.buf)), "%s: null pointer", what);
-        const Lay l = lay_of(g.rows, g.cols);
+        const Lay l = lay_of(g);
         const int64_t tiles = l.mp / 64 * (l.np / 64) + 4096;  // (slices stay below that)
         GAN_CHECK_ARG(g.batch <= (small ? (1 << 22) / NOPS : MAXGRID / NOPS / (tiles > l.nparts ? tiles : l.nparts)), "%s: %lld matrices of %lld x %lld are too many for one call",
                       what, (long long)g.batch, (long long)g.rows, (long long)g.cols);
@@ -1412,7 +1412,7 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, const
             const gan_matrix& g = all[from++];
             if (!g.batch) continue;
             some[n++] = g;
-            if (!small) used += lay_of(g.rows, g.cols).bytes * g.batch;
+            if (!small) used += lay_of(g).bytes * g.batch;
         }
         if (!n) break;
         if (small) {
@@ -1424,7 +1424,7 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, const
         Walk walks[NOPS];
         int64_t tiles = 0;
         for (int k = 0; k < n; ++k) {
-            walks[k] = Walk{lay_of(some[k].rows, some[k].cols), false, steps, 1, 0, 0};
+            walks[k] = Walk{lay_of(some[k]), false, steps, 1, 0, 0};
             tiles += tiles_of(walks[k].l.mp, walks[k].l.mp, true, 64) * some[k].batch;
         }
         for (int k = 0; k < n; ++k) walks[k].beside = 2 * n <= NOPS && 2 * tiles <= 256;
