@@ -921,13 +921,15 @@ int products(const gan_matrix* mats, Walk* walks, int n, int steps, Ops& s, char
     s.first[s.count] = (int)blocks;
     // Where there is a workgroup a CU at most, a long ring of stages and two sets of waves (KG = 2) hide the waits: 116 us against 182
     // for A = X X' of 2048 x 8192.  Where there are more, those do, and short rings let more of them in: two of T = 128 a CU
-    // (174 us against 184 for P X), five of T = 64 (14.3 us against 15.5 for 576 tiles of k = 512).
-    if (int rc = T == 256                  ? launch_gemm<256, 2, 1>((unsigned)blocks, s, dtype, st)
-                 : T == 128 ? blocks > 256 ? launch_gemm<128, 2, 1>((unsigned)blocks, s, dtype, st)
-                                           : launch_gemm<128, 4, 2>((unsigned)blocks, s, dtype, st)
-                 : blocks > 512            ? launch_gemm<64, 2, 1>((unsigned)blocks, s, dtype, st)
-                                           : launch_gemm<64, 4, 2>((unsigned)blocks, s, dtype, st))
-        return rc;
+    // (174 us against 184 for P X), five of T = 64 (14.3 us against 15.5 for 576 tiles of k = 512); up to two a CU of T = 64 keep the
+    // long ring (five iterations of 1500 x 1500, 300 tiles: 405 us against 423 with two sets of waves and 480 with short rings).
+    int rc;
+    const unsigned grid = (unsigned)blocks;
+    if (T == 256) rc = launch_gemm<256, 2, 1>(grid, s, dtype, st);
+    else if (T == 128) rc = blocks > 256 ? launch_gemm<128, 2, 1>(grid, s, dtype, st) : launch_gemm<128, 4, 2>(grid, s, dtype, st);
+    else if (blocks > 512) rc = launch_gemm<64, 2, 1>(grid, s, dtype, st);
+    else rc = blocks > 256 ? launch_gemm<64, 4, 1>(grid, s, dtype, st) : launch_gemm<64, 4, 2>(grid, s, dtype, st);
+    if (rc) return rc;
     if (!sliced) return GAN_OK;
     int64_t join = 0;
     int m = 0;
