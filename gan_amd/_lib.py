@@ -173,8 +173,10 @@ def stream_of(t: Tensor):
 
 
 _HERE_ALREADY = contextlib.nullcontext()
+# (what torch.cuda.current_device() returns once there are tensors on a device)
+current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def on_device(t: Tensor):
     """Context in which t's device is the current one (launches go to the current device's context)."""
-    return _HERE_ALREADY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE_ALREADY if t.device.index == current_device() else torch.cuda.device(t.device)

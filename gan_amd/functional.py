@@ -2594,13 +2594,17 @@ def _layer_norm_ws(rows: int, d: int, code: int, order: int, columns: bool) -> i
 
 def _launch(family: str, tensors, tag, fn, *args) -> None:
     """A call of the library on tensors[0]'s device and stream, measured where a profile is set.  (Called without a profile some
-    hundred times per iteration from the engine's threads: no closures.)"""
+    hundred times per iteration from the engine's threads: no closures and no context.)"""
     t = tensors[0]
-    with on_device(t):
-        if _PROFILE is None:
-            status = fn(*args, stream_of(t))
-        else:
-            status = _PROFILE.launch(family, 0, _nbytes(*tensors), lambda: fn(*args, stream_of(t)), tag)
+    index = t.device.index
+    if _PROFILE is None and index == _lib.current_device():
+        status = fn(*args, _lib._raw_stream(index))
+    else:
+        with on_device(t):
+            if _PROFILE is None:
+                status = fn(*args, stream_of(t))
+            else:
+                status = _PROFILE.launch(family, 0, _nbytes(*tensors), lambda: fn(*args, stream_of(t)), tag)
     if status:
         check(status, fn.__name__)
 
@@ -2610,10 +2614,10 @@ def raw_layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], 
     rows, code = x.numel() // d, dtype_code(x)
     y = torch.empty_like(x)
     n = _layer_norm_ws(rows, d, code, 0, False)
-    stats = x.new_empty((rows, 2), dtype=torch.float32) if keep else None
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if keep else None
     ws = x.new_empty((n,), dtype=torch.float32) if n else None
-    _launch("layernorm", (x, y), (rows, d), _lib.load().gan_layernorm_fwd, ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(stats), rows, d, eps, code,
-            ptr(ws), n)
+    _launch("layernorm", (x, y), (rows, d), _lib.load().gan_layernorm_fwd, x.data_ptr(), ptr(weight), ptr(bias), y.data_ptr(), ptr(stats), rows, d,
+            eps, code, ptr(ws), n)
     return y, stats
 
 
@@ -2626,8 +2630,8 @@ def raw_layer_norm_bwd(g: Tensor, x: Tensor, weight: Optional[Tensor], stats: Te
     gwb = x.new_empty((2, d), dtype=torch.float32) if need_cols else None
     n = _layer_norm_ws(rows, d, code, 1, need_cols)
     ws = x.new_empty((n,), dtype=torch.float32) if n else None
-    _launch("layernorm_bwd", (x, g, gx), (rows, d), _lib.load().gan_layernorm_bwd, ptr(g), ptr(x), ptr(weight), ptr(stats), ptr(gx), ptr(gwb), rows, d,
-            code, ptr(ws), n)
+    _launch("layernorm_bwd", (x, g, gx), (rows, d), _lib.load().gan_layernorm_bwd, g.data_ptr(), x.data_ptr(), ptr(weight), stats.data_ptr(), ptr(gx),
+            ptr(gwb), rows, d, code, ptr(ws), n)
     return gx, gwb
 
 
@@ -2654,14 +2658,15 @@ def _plain_f32(t: Optional[Tensor]) -> Optional[Tensor]:
 
 def _shaped(g: Tensor, shape, dtype) -> Tensor:
     """A (d,) fp32 gradient as its parameter is."""
-    g = g if len(shape) == 1 else g.view(shape)
-    return g if dtype == torch.float32 else g.to(dtype)
+    if len(shape) != 1:
+        g = g.view(shape)
+    return g if dtype is torch.float32 else g.to(dtype)
 
 
 def _wanted(ctx, edge: int) -> bool:
-    """Will the engine run what takes the gradient of the `edge`-th tensor argument (see _need)?  Asked of parameters only, which
-    `layer_norm` hands over as views: whether torch.autograd.grad() wants a leaf can only be asked by way of an exception,
-    and raising one costs 15 us, three times what the view does."""
+    """Will the engine run what takes the gradient of the `edge`-th tensor argument (see _need)?  Asked under create_graph only, a
+    penalty's first pass: elsewhere a parameter that requires a gradient nearly always gets one, and asking about a leaf that
+    torch.autograd.grad() was given ends in an exception, 15 us."""
     if not _PRUNE_UNWANTED:
         return True
     fn = ctx.next_functions[edge][0]
@@ -2689,16 +2694,14 @@ class LayerNormFn(_TorchFunction):
     def backward(ctx, g):
         x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        # Under torch.autograd.grad(out, x, create_graph=True), a penalty's first pass, the parameters' sums would be thrown away.
-        # (The bias's comes with the weight's: one question to the engine for both.)
-        if need_w:
-            need_w = need_b = _wanted(ctx, 1)
-            need_b = need_b and ctx.needs_input_grad[2]
-        elif need_b:
-            need_b = _wanted(ctx, 1 if weight is None else 2)
         if torch.is_grad_enabled():
-            if g.is_leaf and g.requires_grad:
-                g = g.view_as(g)  # (see _wanted)
+            # Under torch.autograd.grad(out, x, create_graph=True), a penalty's first pass, the parameters' sums would be thrown
+            # away.  (The bias's comes with the weight's: one question to the engine for both.)
+            if need_w:
+                need_w = _wanted(ctx, 1)
+                need_b = need_b and need_w
+            elif need_b:
+                need_b = _wanted(ctx, 1 if weight is None else 2)
             gx, gw, gb = LayerNormBwdFn.apply(g, x, weight, stats, ctx.d, (need_x, need_w, need_b))
         else:
             gx, gwb = raw_layer_norm_bwd(g if g.dtype == x.dtype and g.is_contiguous() else g.to(x.dtype).contiguous(), x, _plain_f32(weight), stats,
@@ -2733,8 +2736,7 @@ class LayerNormBwdFn(_TorchFunction):
         elif v.dtype != gc.dtype or not v.is_contiguous():
             v = v.to(gc.dtype).contiguous()
         need = ctx.needs_input_grad
-        gg, gxx, gww = raw_layer_norm_bwd2(v, _plain_f32(cw), _plain_f32(cb), gc, x, _plain_f32(weight), stats, ctx.d, need[0], need[1],
-                                           need[2] and _wanted(ctx, 2))
+        gg, gxx, gww = raw_layer_norm_bwd2(v, _plain_f32(cw), _plain_f32(cb), gc, x, _plain_f32(weight), stats, ctx.d, *need[:3])
         if gg is not None and gg.dtype != ctx.g_dtype:
             gg = gg.to(ctx.g_dtype)
         return gg, gxx, (None if gww is None else _shaped(gww, weight.shape, weight.dtype)), None, None, None
@@ -2751,21 +2753,21 @@ def layer_norm(x: Tensor, normalized_shape, weight: Optional[Tensor] = None, bia
         raise _lib.GanAmdError(f"layer_norm: normalized_shape must be positive sizes, got {shape}")
     if x.shape[-len(shape):] != shape:
         raise _lib.GanAmdError(f"layer_norm: the trailing sizes of {tuple(x.shape)} are not normalized_shape {shape}")
+    grads = x.requires_grad
     if weight is not None:
         _check_affine("weight", weight, x, shape)
+        grads = grads or weight.requires_grad
     if bias is not None:
         _check_affine("bias", bias, x, shape)
+        grads = grads or bias.requires_grad
     if not eps >= 0.0:
         raise _lib.GanAmdError(f"layer_norm: eps must not be negative, got {eps}")
     dtype_code(x)
     require_gpu(x)
     d = math.prod(shape)
-    if not (torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad))):
-        # sampling and evaluation: the launch alone (a dual tensor of forward-mode AD is left to the Function, which refuses it)
-        if x.is_contiguous() and forward_ad._current_level < 0:
-            return raw_layer_norm(x, _plain_f32(weight), _plain_f32(bias), d, eps, False)[0]
-    elif weight is not None and weight.is_leaf and weight.requires_grad:
-        weight = weight.view_as(weight)  # (see _wanted)
+    # sampling and evaluation: the launch alone (a dual tensor of forward-mode AD is left to the Function, which refuses it)
+    if not (grads and torch.is_grad_enabled()) and forward_ad._current_level < 0 and x.is_contiguous():
+        return raw_layer_norm(x, _plain_f32(weight), _plain_f32(bias), d, eps, False)[0]
     if x.is_contiguous():
         return LayerNormFn.apply(x, weight, bias, d, eps)
     if x.dim() == 4 and len(shape) == 3 and x.is_contiguous(memory_format=CL):
