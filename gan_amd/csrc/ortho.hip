@@ -6,7 +6,8 @@
 // hi hi + hi lo + lo hi are accumulated in fp32.  The dropped lo lo is 2^-24 of the product.  Three fp16 products cost a third
 // of the fp16 rate, and fp32 matrix instructions run at an eighth of it (1.18 PFLOP/s and 0.154 for large products).
 // Measured: P X of 2048 x 8192 in 166 us = 1.24 PFLOP/s of fp16 (0.41 of fp32 accuracy), A = X X' of it in 116 us (0.94; half
-// of A is computed), A A in 37 (0.74: 136 tiles for 256 CUs); five iterations 1300 us, of 512 x 4608 182 us.  Large products are
+// of A is computed), A A in 37 (0.74: 136 tiles for 256 CUs); five iterations 1290 to 1460 us by the clock that
+// the card holds, of 512 x 4608 181 to 190.  Large products are
 // bound by the matrix instructions, those of a few hundred rows by their latency: 8 to 10 us a launch, 3 of them matrix
 // instructions, the others the way of the first requests through the caches and the end of the workgroup.
 // All matrices of a call share the launches (one per product), their tiles side by side in the grid; A and P are symmetric,
