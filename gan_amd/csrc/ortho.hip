@@ -114,6 +114,16 @@ int64_t tiles_of(int64_t M, int64_t N, bool sym, int T) {
     return sym ? tm * (tm + 1) / 2 : tm * tn;
 }
 
+// The same with the best tile, C of M x N over K (cut: as it stands).
+double least_cost(int64_t M, int64_t N, int64_t K, bool sym, int64_t batch, int cut) {
+    double least = 1e30;
+    for (int T = 64; T <= 256; T *= 2) {
+        const double c = cost_of(T, tiles_of(M, N, sym, T) * batch, cut, K / 32);
+        if (c < least) least = c;
+    }
+    return least;
+}
+
 // Slices of A = X X' (a long k, few tiles), at least eight steps each, by the group alone (the workspace goes by it).
 int cut_of(int64_t mp, int64_t np, int64_t batch) {
     int best = 1;
@@ -802,21 +812,31 @@ int launch_gemm(unsigned blocks, const Ops& s, int dtype, hipStream_t st) {
 //   two:  P = poly(A), T = P A, A2 = P T (= X2 X2'), P2 = poly(A2), Q = P2 P;  X <- Q X
 //   two, side by side:  P = poly(A) | T = P A, S = P P | A2 = T P, B = T S (= A2 P) | Q = a P + b B + c A2 B;  X <- Q X
 // Two iterations at a time replace a product with X and one into it by three m x m ones: 6 m^2 n + 2 m^3 against
-// 3 m^2 n + 5 m^3, which pays from n = 2 m on.  Not more at a time: an error of A, 2^-22 of its largest singular value, weighs
+// 3 m^2 n + 5 m^3, which can pay from n = 2 m on.  Not more at a time: an error of A, 2^-22 of its largest singular value, weighs
 // the more on the smallest ones the longer the iteration runs on A alone (error against 64 bits, 512 x 4608 with a spectrum that
 // falls like 1 / i: 1.9e-6 step by step, 3.1e-6 like this, 7.8e-6 in stages of two and three, 1.7e-4 in one).  The first
 // stage is a single iteration: the small values are smallest there.
 // Side by side is a product more and a launch less: taken where two products of each matrix leave no CU with more than one tile,
 // the launch then being as long as one (512 x 4608: 195 -> 184 us, 704 x 1500 187 -> 178; 1000 x 4000, which has more tiles, gains nothing).
-int stage_of(const Lay& l, int left, int steps) { return l.np >= 2 * l.mp && left < steps && left >= 2 ? 2 : 1; }
+// They have to gain a launch's time by the cost rule, else step by step it is, the more accurate way (100 x 2000: 1.3e-6 in 112 us
+// against 3.3e-6 in 110; 300 x 700: 0.7e-6 in 122 against 1.8e-6 in 121; 512 x 4608: 1.2e-6 in 193 us, taken are 1.6e-6 in 175).
+// Where several sizes share the launches all go the same way as far as they can: a discriminator's step takes 393 us, 485 with some of
+// its matrices step by step.
+bool two_at_a_time(const Lay& l, int64_t batch, bool beside, bool shared) {
+    if (l.np < 2 * l.mp) return false;
+    if (shared) return true;
+    const double gram = least_cost(l.mp, l.mp, l.np, true, batch, l.cut), apply = least_cost(l.mp, l.np, l.mp, false, batch, 1),
+                 square = least_cost(l.mp, l.mp, l.mp, true, batch, 1);
+    return gram + apply - (beside ? 2 : 3) * square >= 6.;
+}
 
 struct Walk {
     Lay l;
-    bool beside;              // two iterations: side by side
+    bool pairs, beside;       // two iterations at a time; side by side
     int left, size, at, cur;  // iterations left, this stage's size, the next launch within it, the X that holds the iterate
     // one or two products
     int next(Op* q, int steps) {
-        if (at == 0) size = stage_of(l, left, steps);
+        if (at == 0) size = pairs && left < steps && left >= 2 ? 2 : 1;
         int n = 0;
         auto sq = [&](int k) { return (unsigned)(l.sq[k] / 256); };
         auto mul = [&](int u, int v, int to, float gain, int kind = SCALED, int aux = 0, int aux2 = 0) {
@@ -1427,10 +1447,13 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, const
         Walk walks[NOPS];
         int64_t tiles = 0;
         for (int k = 0; k < n; ++k) {
-            walks[k] = Walk{lay_of(some[k]), false, steps, 1, 0, 0};
+            walks[k] = Walk{lay_of(some[k]), false, false, steps, 1, 0, 0};
             tiles += tiles_of(walks[k].l.mp, walks[k].l.mp, true, 64) * some[k].batch;
         }
-        for (int k = 0; k < n; ++k) walks[k].beside = 2 * n <= NOPS && 2 * tiles <= 256;
+        for (int k = 0; k < n; ++k) {
+            walks[k].beside = 2 * n <= NOPS && 2 * tiles <= 256;
+            walks[k].pairs = two_at_a_time(walks[k].l, some[k].batch, walks[k].beside, n > 1);
+        }
         for (bool more = true; more;) {
             if ((rc = products(some, walks, n, steps, o, at, dtype, st))) return rc;
             more = false;

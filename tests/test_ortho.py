@@ -71,7 +71,7 @@ def test_against_the_definition(dev, m, n):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", [(1990, 33000), (2048, 8192), (1030, 4100), (3, 1000, 1777), (9, 260, 2000), (20000, 3, 5), (100000, 40)])
+@pytest.mark.parametrize("shape", [(1990, 33000), (2048, 8192), (1030, 4100), (500, 4610), (3, 1000, 1777), (9, 260, 2000), (20000, 3, 5), (100000, 40)])
 def test_large_ones(dev, shape):
     """Sizes at which the larger tiles run, whole and with a part of one at the end, with their sums cut in slices and not; many
     matrices at once, and very long ones.  (The reference runs on the device, in 64 bits.)"""
