@@ -2696,12 +2696,9 @@ class LayerNormFn(_TorchFunction):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         if torch.is_grad_enabled():
             # Under torch.autograd.grad(out, x, create_graph=True), a penalty's first pass, the parameters' sums would be thrown
-            # away.  (The bias's comes with the weight's: one question to the engine for both.)
-            if need_w:
-                need_w = _wanted(ctx, 1)
-                need_b = need_b and need_w
-            elif need_b:
-                need_b = _wanted(ctx, 1 if weight is None else 2)
+            # away.  Either may be asked for without the other; where the weight's is, the bias's comes with it, wanted or not.
+            need_w = need_w and _wanted(ctx, 1)
+            need_b = need_b and (need_w or _wanted(ctx, 1 if weight is None else 2))
             gx, gw, gb = LayerNormBwdFn.apply(g, x, weight, stats, ctx.d, (need_x, need_w, need_b))
         else:
             gx, gwb = raw_layer_norm_bwd(g if g.dtype == x.dtype and g.is_contiguous() else g.to(x.dtype).contiguous(), x, _plain_f32(weight), stats,

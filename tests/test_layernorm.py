@@ -368,3 +368,91 @@ def test_refusals():
     assert lib.gan_layernorm_bwd(p, p, p, p, p, p, 0, 8, 0, p, 1 << 20, None) != 0
     assert lib.gan_layernorm_bwd2(None, p, p, p, p, p, p, p, p, p, 4, 8, 0, p, 1 << 20, None) != 0
     assert lib.gan_layernorm_bwd2(p, p, p, p, p, p, p, p, p, p, 4, 8, 0, p + 4, 1 << 20, None) != 0
+
+
+def plain_launches(monkeypatch):
+    """The three launches as their formulas on the CPU: what lies between them and the engine is then what is tested."""
+    from gan_amd import functional as GF
+
+    def t_of(x, stats, d):
+        x, stats = x.detach().reshape(-1, d).double(), stats.double()
+        return (x - stats[:, :1]) * stats[:, 1:]
+
+    def fwd(x, weight, bias, d, eps, keep=True):
+        u = x.detach().reshape(-1, d).double()
+        m = u.mean(1, keepdim=True)
+        stats = torch.cat([m, ((u - m).square().mean(1, keepdim=True) + eps).rsqrt()], 1)
+        y = (u - m) * stats[:, 1:]
+        y = y if weight is None else y * weight.detach().reshape(d).double()
+        y = y if bias is None else y + bias.detach().reshape(d).double()
+        return y.to(x.dtype).view(x.shape), stats.float()
+
+    def bwd(g, x, weight, stats, d, need_x, need_cols):
+        t, u, r = t_of(x, stats, d), g.detach().reshape(-1, d).double(), stats[:, 1:].double()
+        h = u if weight is None else u * weight.detach().reshape(d).double()
+        gx = (r * proj(h, t)).to(x.dtype).view(x.shape) if need_x else None
+        return gx, torch.stack([(u * t).sum(0), u.sum(0)]).float() if need_cols else None
+
+    def bwd2(v, cw, cb, g, x, weight, stats, d, need_g, need_x, need_w):
+        flat = [s.detach().reshape(-1, d) for s in (x, g, v)]
+        one = torch.ones(d, dtype=torch.float64)
+        w = one if weight is None else weight.detach().reshape(d)
+        ref = Ref(*flat, w, one, *(None if s is None else s.detach().reshape(d) for s in (cw, cb)))
+        gg, gxx = (getattr(ref, k).to(x.dtype).view(x.shape) if need else None for k, need in (("gg", need_g), ("gxx", need_x)))
+        return gg, gxx, ref.gww.float() if need_w else None
+
+    monkeypatch.setattr(GF, "raw_layer_norm", fwd)
+    monkeypatch.setattr(GF, "raw_layer_norm_bwd", bwd)
+    monkeypatch.setattr(GF, "raw_layer_norm_bwd2", bwd2)
+
+
+def check_gradients_asked_for_alone(norm, dev, has_weight):
+    """Under create_graph, any of the gradients without the others (whose tensors require one all the same)."""
+    rows, d = 12, 40
+    x0, g0, v, w0, b0, cw, cb = make(rows, d, torch.float32, dev)
+    one, zero = torch.ones_like(w0), torch.zeros_like(w0)
+    for asked in ("x", "w", "b", "xw", "xb", "wb", "xwb"):
+        if "w" in asked and not has_weight:
+            continue
+        leaf = dict(zip("xgwb", (t.clone().requires_grad_() for t in (x0, g0, w0, b0))))
+        w = leaf["w"] if has_weight else None
+        ref = Ref(x0, g0, v if "x" in asked else torch.zeros_like(v), w0 if has_weight else one, b0, cw if "w" in asked else zero, cb if "b" in asked else zero)
+        got = dict(zip(asked, torch.autograd.grad(norm(leaf["x"], w, leaf["b"]), [leaf[k] for k in asked], leaf["g"], create_graph=True)))
+        for k in asked:
+            near(got[k], Ref(x0, g0, v, w0 if has_weight else one, b0), "g" + k, rows)
+        (gg,) = torch.autograd.grad([got[k] for k in asked], leaf["g"], [{"x": v, "w": cw, "b": cb}[k] for k in asked])
+        near(gg, ref, "gg")
+    # handed to backward() by name
+    x, w, b = (t.clone().requires_grad_() for t in (x0, w0, b0))
+    norm(x, w if has_weight else None, b).backward(g0, inputs=[b], create_graph=True)
+    near(b.grad.detach(), Ref(x0, g0, v, w0 if has_weight else one, b0), "gb", rows)
+    assert x.grad is None and w.grad is None
+    b.grad = None  # (else it and its graph hold each other)
+    # a bias computed from what the gradient is taken of
+    c = b0.clone().requires_grad_()
+    y = norm(x, w if has_weight else None, 0.5 * c)
+    (gc,) = torch.autograd.grad([y, c], c, [g0, torch.ones_like(c)], create_graph=True)
+    near((gc.detach() - 1) * 2, Ref(x0, g0, v, w0, b0), "gb", rows + N)  # (1 is added and taken off: another rounding of 1 + |gb|)
+
+
+@pytest.mark.parametrize("has_weight", [True, False])
+def test_gradients_asked_for_alone(monkeypatch, has_weight):
+    from gan_amd import functional as GF
+
+    plain_launches(monkeypatch)
+    check_gradients_asked_for_alone(lambda x, w, b: GF.LayerNormFn.apply(x, w, b, 40, 1e-5), torch.device("cpu"), has_weight)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("has_weight", [True, False])
+def test_gradients_asked_for_alone_on_the_device(dev, has_weight):
+    from gan_amd import functional as GF
+
+    check_gradients_asked_for_alone(lambda x, w, b: GF.layer_norm(x, 40, w, b), dev, has_weight)
+
+    def samples(x, w, b):  # whole samples of a channels-last activation
+        x = x.view(12, 2, 5, 4).permute(0, 3, 1, 2)
+        w, b = (None if t is None else t.view(2, 5, 4).permute(2, 0, 1) for t in (w, b))
+        return GF.layer_norm(x, (4, 2, 5), w, b).permute(0, 2, 3, 1).reshape(12, 40)
+
+    check_gradients_asked_for_alone(samples, dev, has_weight)
