@@ -2657,10 +2657,13 @@ def _plain_f32(t: Optional[Tensor]) -> Optional[Tensor]:
 
 
 def _shaped(g: Tensor, shape, dtype) -> Tensor:
-    """A (d,) fp32 gradient as its parameter is."""
+    """A (d,) fp32 gradient as its parameter is.  (Outside create_graph a view made here could not be changed in place by what
+    asks for a gradient itself: .data is the same memory as a tensor of its own.)"""
+    if dtype is not torch.float32:
+        g = g.to(dtype)
     if len(shape) != 1:
         g = g.view(shape)
-    return g if dtype is torch.float32 else g.to(dtype)
+    return g if torch.is_grad_enabled() else g.data
 
 
 def _wanted(ctx, edge: int) -> bool:
@@ -2720,7 +2723,8 @@ class LayerNormBwdFn(_TorchFunction):
         ctx.save_for_backward(gc, x, weight, stats)
         ctx.d, ctx.g_dtype = d, g.dtype
         ctx.set_materialize_grads(False)
-        return gx, (gwb[0] if need[1] else None), (gwb[1] if need[2] else None)
+        # (.data: two tensors in one allocation; two views of one tensor could not be changed in place)
+        return gx, (gwb[0].data if need[1] else None), (gwb[1].data if need[2] else None)
 
     @staticmethod
     @torch.autograd.function.once_differentiable

@@ -390,7 +390,7 @@ def plain_launches(monkeypatch):
     def bwd(g, x, weight, stats, d, need_x, need_cols):
         t, u, r = t_of(x, stats, d), g.detach().reshape(-1, d).double(), stats[:, 1:].double()
         h = u if weight is None else u * weight.detach().reshape(d).double()
-        gx = (r * proj(h, t)).to(x.dtype).view(x.shape) if need_x else None
+        gx = torch.empty_like(x).copy_((r * proj(h, t)).view(x.shape)) if need_x else None
         return gx, torch.stack([(u * t).sum(0), u.sum(0)]).float() if need_cols else None
 
     def bwd2(v, cw, cb, g, x, weight, stats, d, need_g, need_x, need_w):
@@ -398,7 +398,7 @@ def plain_launches(monkeypatch):
         one = torch.ones(d, dtype=torch.float64)
         w = one if weight is None else weight.detach().reshape(d)
         ref = Ref(*flat, w, one, *(None if s is None else s.detach().reshape(d) for s in (cw, cb)))
-        gg, gxx = (getattr(ref, k).to(x.dtype).view(x.shape) if need else None for k, need in (("gg", need_g), ("gxx", need_x)))
+        gg, gxx = (torch.empty_like(x).copy_(getattr(ref, k).view(x.shape)) if need else None for k, need in (("gg", need_g), ("gxx", need_x)))
         return gg, gxx, ref.gww.float() if need_w else None
 
     monkeypatch.setattr(GF, "raw_layer_norm", fwd)
@@ -456,3 +456,47 @@ def test_gradients_asked_for_alone_on_the_device(dev, has_weight):
         return GF.layer_norm(x, (4, 2, 5), w, b).permute(0, 2, 3, 1).reshape(12, 40)
 
     check_gradients_asked_for_alone(samples, dev, has_weight)
+
+
+def check_gradients_changed_in_place(norm, dev):
+    """The gradients are tensors of their own, as F.layer_norm's are: each may be scaled or clipped where it lies."""
+    rows, d = 6, 40
+    x0, g0, _, w0, b0, cw, cb = make(rows, d, torch.float32, dev)
+    ref = Ref(x0, g0, torch.zeros_like(x0), w0, b0, 2 * cw, 3 * cb)
+    x, g, w, b = (t.clone().requires_grad_() for t in (x0, g0, w0, b0))
+    gw, gb = torch.autograd.grad(norm(x, w, b), (w, b), g, create_graph=True)
+    gw.mul_(2), gb.mul_(3)
+    near(gw.detach() / 2, ref, "gw", rows)
+    near(gb.detach() / 3, ref, "gb", rows)
+    near(torch.autograd.grad((gw, gb), g, (cw, cb))[0], ref, "gg")
+    # those of a first and of a second backward without create_graph, by a factor that asks for a gradient itself
+    factor = torch.full((), 2.0, device=dev, requires_grad=True)
+    first = torch.autograd.grad(norm(x, w, b), (x, w, b), g0)
+    (gx,) = torch.autograd.grad(norm(x, w, b), x, g, create_graph=True)
+    for grad in (*first, *torch.autograd.grad(gx, (x, g, w), g0)):
+        want = 2 * grad
+        grad.mul_(factor)
+        assert torch.equal(grad, want) and grad.requires_grad
+
+
+def test_gradients_changed_in_place(monkeypatch):
+    from gan_amd import functional as GF
+
+    plain_launches(monkeypatch)
+    dev = torch.device("cpu")
+    check_gradients_changed_in_place(lambda x, w, b: GF.LayerNormFn.apply(x, w, b, 40, 1e-5), dev)
+    shape = (4, 10)  # parameters of more than one dimension
+    x, w, b = (t.requires_grad_() for t in (torch.randn(3, *shape), torch.randn(shape), torch.randn(shape)))
+    factor = torch.full((), 2.0, requires_grad=True)
+    for create_graph in (True, False):
+        for grad in torch.autograd.grad(GF.LayerNormFn.apply(x, w, b, 40, 1e-5), (w, b), torch.randn(3, *shape), create_graph=create_graph):
+            want = 2 * grad.detach()
+            grad.mul_(factor)
+            assert torch.equal(grad, want) and grad.shape == shape
+
+
+@pytest.mark.gpu
+def test_gradients_changed_in_place_on_the_device(dev):
+    from gan_amd import functional as GF
+
+    check_gradients_changed_in_place(lambda x, w, b: GF.layer_norm(x, 40, w, b), dev)
