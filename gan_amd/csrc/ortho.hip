@@ -27,7 +27,8 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 constexpr int PAD = 64;          // matrices are padded with zeros to multiples of this
 constexpr int MAXPARTS = 512;    // partial sums of squares of a matrix
 constexpr int NOPS = 32;         // matrices of one launch (their descriptions are kernel arguments: at most 4 KB)
-constexpr int64_t MAXGRID = 1LL << 31;
+// Workgroups of a launch stay below these (work items are counted in 32 bits: 256 in a workgroup of the general path, 1024 in LDS)
+constexpr int64_t MAXBLOCKS = 1LL << 24, MAXSMALL = 1LL << 22;
 constexpr float SX = 16384.f;    // |X| <= 3.9: fp16 ends at 65504
 constexpr float SA = 4096.f;     // |A| <= 15.9
 constexpr float SP = 16.f;       // |P| and products of two of them <= 4000
@@ -164,6 +165,13 @@ Lay lay_of(const gan_matrix& g) {
     if (l.cut > 1) at += l.cut * t * (t + 4) / 2 * 4096 * 4;
     l.bytes = at;
     return l;
+}
+
+// The most workgroups that one of these matrices takes in a launch: a product's tiles of 64, or, where sums are cut in slices, up to
+// 4096 tiles of slices and 1024 / T^2 of a tile's blocks for the launch that joins them.
+int64_t blocks_of(const Lay& l) {
+    const int64_t t = l.mp / 64, tiles = t * (l.np / 64);
+    return (tiles > l.nparts ? tiles : l.nparts) + (l.cut > 1 ? 4096 + 2 * (t + 3) * (t + 7) : 0);
 }
 
 // the group that workgroup `id` works on (first[] ascends)
@@ -1352,18 +1360,19 @@ bool bounded(int steps, float a, float b, float c) {
 
 int64_t total_bytes(const gan_matrix* mats, int count) {
     int64_t n = 0;
-    bool small = true;
+    bool small = true, fit = true;
     for (int k = 0; k < count; ++k) {
         const gan_matrix& g = mats[k];
-        if (g.rows < 1 || g.cols < 1 || g.batch < 0 || g.rows > (1 << 20) || g.cols > (1 << 20) || g.batch > (1 << 30)) return -1;
+        if (g.rows < 1 || g.cols < 1 || g.batch < 0 || g.rows > (1 << 20) || g.cols > (1 << 20) || g.batch >= MAXSMALL) return -1;
         if (up64(g.rows) * up64(g.cols) >= (1LL << 30) || (g.rows < g.cols ? g.rows : g.cols) > 32768) return -1;
-        const int64_t one = lay_of(g).bytes;
-        if (g.batch && one > (1LL << 60) / g.batch) return -1;
-        n += one * g.batch;
+        const Lay l = lay_of(g);
+        if (g.batch && l.bytes > (1LL << 60) / g.batch) return -1;
+        n += l.bytes * g.batch;
         if (n > (1LL << 60)) return -1;
         small = small && is_small(g);
+        fit = fit && g.batch * blocks_of(l) < MAXBLOCKS;
     }
-    return small ? 0 : n;  // (all of them in LDS)
+    return small ? 0 : fit ? n : -1;  // (small: all of them in LDS)
 }
 
 // The two launches in front of the products: momentum and norms, planes.
@@ -1411,19 +1420,12 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, const
     GAN_CHECK_ARG(bounded(steps, rule.a, rule.b, rule.c), "%s: with coefficients %g %g %g a singular value can grow beyond 3.5", what, (double)rule.a,
                   (double)rule.b, (double)rule.c);
     const int64_t need = total_bytes(all, count);
-    GAN_CHECK_ARG(need >= 0, "%s: a matrix has a size that is not supported (1 to 2^20 either way, the smaller at most 32768, fewer than 2^30 elements when padded to 64s)", what);
+    GAN_CHECK_ARG(need >= 0, "%s: a matrix has a size that is not supported (1 to 2^20 either way, the smaller at most 32768, fewer than 2^30 elements when padded to 64s, fewer than 2^22 of them in a batch, in 2^23 blocks of 64 x 64)", what);
     GAN_CHECK_ARG(need == 0 || (ws && bytes >= need), "%s: workspace of %lld bytes wanted, %lld given", what, (long long)need,
                   (long long)(ws ? bytes : 0));
     GAN_CHECK_ARG(((uintptr_t)ws % 256) == 0, "%s: workspace must be 256-byte aligned", what);
     const bool small = all_small(all, count);
-    for (int k = 0; k < count; ++k) {
-        const gan_matrix& g = all[k];
-        GAN_CHECK_ARG(!g.batch || (g.g && g.out && (!rule.update || g.buf)), "%s: null pointer", what);
-        const Lay l = lay_of(g);
-        const int64_t tiles = l.mp / 64 * (l.np / 64) + 4096;  // (slices stay below that)
-        GAN_CHECK_ARG(g.batch <= (small ? (1 << 22) / NOPS : MAXGRID / NOPS / (tiles > l.nparts ? tiles : l.nparts)), "%s: %lld matrices of %lld x %lld are too many for one call",
-                      what, (long long)g.batch, (long long)g.rows, (long long)g.cols);
-    }
+    for (int k = 0; k < count; ++k) GAN_CHECK_ARG(!all[k].batch || (all[k].g && all[k].out && (!rule.update || all[k].buf)), "%s: null pointer", what);
     Mats s = {};
     Ops o = {};
     s.from = source;
@@ -1432,12 +1434,15 @@ int run_all(const char* what, const gan_matrix* all, int count, int steps, const
     char* at = ws;
     for (int from = 0; from < count;) {
         int n = 0;
-        int64_t used = 0;
-        while (from < count && n < NOPS) {
-            const gan_matrix& g = all[from++];
+        int64_t used = 0, blocks = 0;
+        for (; from < count && n < NOPS; ++from) {
+            const gan_matrix& g = all[from];
             if (!g.batch) continue;
+            const Lay l = lay_of(g);
+            blocks += g.batch * (small ? 1 : blocks_of(l));
+            if (n && blocks >= (small ? MAXSMALL : MAXBLOCKS)) break;  // (the next launches')
             some[n++] = g;
-            if (!small) used += lay_of(g).bytes * g.batch;
+            if (!small) used += l.bytes * g.batch;
         }
         if (!n) break;
         if (small) {

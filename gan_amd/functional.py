@@ -1017,8 +1017,9 @@ def matrix_workspace(mats, device) -> Tuple[Optional[Tensor], int]:
     """(workspace of gan_orthogonalize / gan_muon_step for an array of _lib.Matrix, its bytes)."""
     n = _lib.load().gan_orthogonalize_workspace(ctypes.addressof(mats), len(mats))
     if n < 0:
-        sizes = sorted({(m.rows, m.cols) for m in mats}, key=max)
-        raise _lib.GanAmdError(f"orthogonalize: matrices of 1 to 2^20 rows and columns, the smaller side at most 32768, fewer than 2^30 elements; got up to {sizes[-1]}")
+        sizes = sorted({(m.batch, m.rows, m.cols) for m in mats}, key=lambda s: (max(s[1:]), s[0]))
+        raise _lib.GanAmdError("orthogonalize: matrices of 1 to 2^20 rows and columns, the smaller side at most 32768, fewer than 2^30 elements, "
+                               f"fewer than 2^22 of them (2^23 blocks of 64 x 64) in a batch; got up to {' x '.join(map(str, sizes[-1]))}")
     return (torch.empty((n,), dtype=torch.uint8, device=device) if n else None), n
 
 

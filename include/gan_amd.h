@@ -454,8 +454,9 @@ int gan_adam_step_ranges(float* p, const float* g, float* m, float* v, const int
  *                    out = (1 - lr weight_decay) out - lr s X(u) with s = 1 (scaling 0), sqrt(max(1, rows / cols)) (1) or
  *                    0.2 sqrt(max(rows, cols)) (2).
  * No two of g, buf and out may overlap.  Coefficients with which a singular value can grow beyond 3.5 are refused.
- * 1 <= rows, cols <= 2^20, the smaller at most 32768, fewer than 2^30 elements (both sides rounded up to 64s), 1 <= steps <= 100,
- * 1e-30 <= eps <= 1e30.
+ * 1 <= rows, cols <= 2^20, the smaller at most 32768, fewer than 2^30 elements (both sides rounded up to 64s); a batch of fewer than
+ * 2^22 matrices and, unless every matrix of the call fits into a compute unit's LDS (32768 elements and some), 2^23 blocks of 64 x 64;
+ * 1 <= steps <= 100, 1e-30 <= eps <= 1e30.
  * workspace: gan_orthogonalize_workspace bytes, 256-byte aligned; negative: a size that is refused. */
 typedef struct gan_matrix {
     const void* g;

@@ -544,3 +544,57 @@ def test_narrow_matrices_in_a_list(dev):
                 x = a * x + (b * gram + c * (gram @ gram)) @ x
             ratios.append(rel_err(-got, want) / rel_err(x, want))
     assert sum(ratios) / len(ratios) < 1.0, ratios
+
+
+def test_limits_of_a_batch():
+    """What the calls refuse, the workspace query says by a negative number; what it gives a size for, they take."""
+    import ctypes
+
+    from gan_amd import _lib
+
+    lib = _lib.load()
+
+    def need(*sizes):
+        m = (_lib.Matrix * len(sizes))(*((4096, None, 4096, *s) for s in sizes))
+        return lib.gan_orthogonalize_workspace(ctypes.addressof(m), len(m)), lib.gan_orthogonalize(ctypes.addressof(m), len(m), 5, *COEFFS, 1e-7, 0, None, 0, None)
+
+    assert need((8, 8, 1 << 22)) == (-1, need((8, 8, 1 << 22))[1]) and need((8, 8, 1 << 22))[1] != 0
+    assert need((200, 200, 1 << 20))[0] < 0 and need((200, 200, 1 << 20))[1] != 0  # (16 blocks each)
+    assert need((200, 200, 1), (8, 8, 1 << 22))[0] < 0
+    for sizes in (((200, 200, (1 << 19) - 1),), ((64, 64, (1 << 22) - 1), (200, 200, 1)), ((1 << 20, 64, 511),), ((32768, 32704, 32),), ((64, 4096, 300),), ((640, 40960, 400),)):
+        assert need(*sizes)[0] > 0 and need(*sizes)[1] != 0  # (no workspace given)
+        assert b"workspace" in lib.gan_amd_last_error()
+    m = (_lib.Matrix * 2)((4096, None, 4096, 8, 8, (1 << 22) - 1), (4096, None, 4096, 200, 100, 3))
+    assert lib.gan_orthogonalize_workspace(ctypes.addressof(m), 1) == 0  # in LDS
+    assert lib.gan_orthogonalize_workspace(ctypes.addressof(m), 2) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(200000, 8, 8), (20000, 70, 65)])
+def test_large_batches(dev, shape):
+    from gan_amd import functional as GF
+
+    torch.manual_seed(3)
+    g = torch.randn(shape, device=dev)
+    got, want = GF.orthogonalize(g).double(), torch.cat([definition(t, on=dev) for t in g.split(50000)])
+    # (the bound of a square Gaussian matrix; one in so many lies further off than a factor of 30, each is held to its own)
+    assert float(((got - want).norm(dim=(1, 2)) / want.norm(dim=(1, 2))).max()) < 6e-4
+
+
+@pytest.mark.gpu
+def test_lists_beyond_one_launch(dev):
+    """Two batches that a launch does not hold together."""
+    import ctypes
+
+    from gan_amd import _lib
+
+    torch.manual_seed(4)
+    g = [torch.randn(2200000, 2, 3, device=dev), torch.randn(2100000, 3, 1, device=dev)]
+    out = [torch.empty_like(t) for t in g]
+    m = (_lib.Matrix * 2)(*((t.data_ptr(), None, o.data_ptr(), t.shape[1], t.shape[2], t.shape[0]) for t, o in zip(g, out)))
+    lib = _lib.load()
+    assert lib.gan_orthogonalize_workspace(ctypes.addressof(m), 2) == 0
+    assert lib.gan_orthogonalize(ctypes.addressof(m), 2, 5, *COEFFS, 1e-7, 0, None, 0, _lib.stream_of(g[0])) == 0
+    for t, o in zip(g, out):
+        want = torch.cat([definition(part, on=dev) for part in t.split(50000)])
+        assert float(((o.double() - want).norm(dim=(1, 2)) / want.norm(dim=(1, 2))).max()) < 6e-4
