@@ -189,8 +189,10 @@ def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentum_buffer
     if not mats:
         return
     _muon_launch((_lib.Matrix * len(mats))(*mats), params[0], lr, momentum, nesterov, weight_decay, adjust_lr_fn, steps, coefficients, eps)
-    # written through raw pointers: cached GEMM images of the old values would still match their keys
+    # written through raw pointers: cached GEMM images of the old values would still match their keys, and a backward that has saved
+    # one of these tensors has to see that it changed
     GF.invalidate_packed(params)
+    torch.autograd.graph.increment_version([*params, *momentum_buffers])
 
 
 def _muon_launch(mats, like: Tensor, lr, momentum, nesterov, weight_decay, adjust_lr_fn, steps, coefficients, eps) -> None:

@@ -598,3 +598,24 @@ def test_lists_beyond_one_launch(dev):
     for t, o in zip(g, out):
         want = torch.cat([definition(part, on=dev) for part in t.split(50000)])
         assert float(((o.double() - want).norm(dim=(1, 2)) / want.norm(dim=(1, 2))).max()) < 6e-4
+
+
+@pytest.mark.gpu
+def test_muon_step_is_seen_by_a_backward_that_waits(dev):
+    """A parameter changed between a forward and its backward: autograd refuses, as for any other change in place."""
+    from gan_amd.optim import muon_step
+
+    p = torch.randn(12, 20, device=dev, requires_grad=True)
+    buf = torch.zeros(12, 20, device=dev)
+    g = torch.randn(12, 20, device=dev)
+    x = torch.randn(5, 12, device=dev, requires_grad=True)
+    y = (x @ p).sum()
+    versions = p._version, buf._version, g._version
+    muon_step([p], [g], [buf], lr=0.1)
+    assert (p._version, buf._version, g._version) == (versions[0] + 1, versions[1] + 1, versions[2])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():  # (tensors without a version)
+        q = torch.randn(12, 20, device=dev)
+        muon_step([q], [g], [torch.zeros_like(q)], lr=0.1)
+    assert torch.isfinite(q).all()
