@@ -1023,6 +1023,11 @@ def matrix_workspace(mats, device) -> Tuple[Optional[Tensor], int]:
     return (torch.empty((n,), dtype=torch.uint8, device=device) if n else None), n
 
 
+def has_tangent(*tensors: Tensor) -> bool:
+    """Is one of them a dual tensor of forward-mode AD?  (Raw pointers would leave its tangent behind without a word.)"""
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def ortho_flops(rows: int, cols: int, steps: int) -> float:
     """Operations of the products as they run: three 16-bit ones for each, the symmetric ones by half."""
     m, n = min(rows, cols), max(rows, cols)
@@ -1035,13 +1040,15 @@ def orthogonalize(x: Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: 
     tall x is worked on as its transpose).  With the default coefficients and five steps the singular values end between
     0.7 and 1.2.  Each matrix of a batch is one of its own.  Products carry 22 bits of every factor and fp32 sums, for
     bfloat16 too (whose result is rounded once); zeros stay zeros, and a matrix with a value that is not finite comes back as
-    NaN.  An update rule, not a layer: there is no derivative, x must not require one."""
+    NaN.  An update rule, not a layer: there is no derivative, x must not require one or carry a tangent."""
     if x.dim() < 2:
         raise _lib.GanAmdError(f"orthogonalize: expected (..., m, n), got shape {tuple(x.shape)}")
     a, b, c = (float(v) for v in coefficients)
     code = dtype_code(x)
     if x.requires_grad and torch.is_grad_enabled():
         raise _lib.GanAmdError("orthogonalize has no derivative: detach x or call it under torch.no_grad()")
+    if has_tangent(x):
+        raise _lib.GanAmdError("orthogonalize has no derivative: x carries a tangent of forward-mode AD, pass its primal")
     require_gpu(x)
     x = x.detach().contiguous()
     out = torch.empty_like(x)

@@ -159,6 +159,8 @@ def muon_step(params: Sequence[Tensor], grads: Sequence[Tensor], momentum_buffer
         raise _lib.GanAmdError(f"muon_step: {len(params)} parameters, {len(grads)} gradients, {len(momentum_buffers)} momentum buffers")
     if adjust_lr_fn not in _SCALINGS:
         raise _lib.GanAmdError(f"muon_step: adjust_lr_fn must be None, 'original', 'match_rms_adamw' or 'none', got {adjust_lr_fn!r}")
+    if GF.has_tangent(*params, *grads, *momentum_buffers):
+        raise _lib.GanAmdError("muon_step has no derivative: a tensor carries a tangent of forward-mode AD, pass its primal")
     held, mats, spans = [], [], []
     for p, g, m in zip(params, grads, momentum_buffers):
         if p.dim() < 2:

@@ -619,3 +619,26 @@ def test_muon_step_is_seen_by_a_backward_that_waits(dev):
         q = torch.randn(12, 20, device=dev)
         muon_step([q], [g], [torch.zeros_like(q)], lr=0.1)
     assert torch.isfinite(q).all()
+
+
+def test_dual_tensors_are_refused():
+    """A tangent would be dropped without a word: both say that there is no derivative."""
+    from torch.autograd import forward_ad
+
+    from gan_amd import _lib
+    from gan_amd import functional as GF
+    from gan_amd.optim import muon_step
+
+    with forward_ad.dual_level():
+        x = torch.randn(4, 8)
+        dual = forward_ad.make_dual(x.clone(), torch.ones_like(x))
+        with pytest.raises(_lib.GanAmdError, match="no derivative"):
+            GF.orthogonalize(dual)
+        with torch.no_grad(), pytest.raises(_lib.GanAmdError, match="no derivative"):
+            GF.orthogonalize(dual)
+        for args in (([dual], [x], [x.clone()]), ([x], [dual], [x.clone()]), ([x], [x.clone()], [dual])):
+            with pytest.raises(_lib.GanAmdError, match="no derivative"):
+                muon_step(*args, lr=0.1)
+        with pytest.raises(_lib.GanAmdError) as plain:
+            GF.orthogonalize(x)
+        assert "derivative" not in str(plain.value)  # (not on a ROCm device)
