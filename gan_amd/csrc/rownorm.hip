@@ -769,6 +769,9 @@ Plan plan_of(int64_t rows, int64_t D, int dtype, int pass, bool cols) {
     return p;
 }
 
+// (work items of a launch are counted in 32 bits, 256 in a workgroup)
+bool too_many(int64_t rows, const Plan& p) { return !p.tpr && rows * p.pieces >= (1LL << 24); }
+
 template <typename T, int PASS, int COLS, int TPR, int K>
 void launch_row(int blocks, const RowArgs& a, hipStream_t st) {
     constexpr int BLK = block_of<TPR>();
@@ -869,7 +872,7 @@ int run_pass(const Plan& p, RowArgs a, float* gw, float* gb, float* ws, hipStrea
 }
 
 int check_common(const char* what, int64_t rows, int64_t D, int dtype, float* ws, int64_t ws_floats, const Plan& p) {
-    GAN_CHECK_ARG(rows < (1LL << 31) && (p.tpr || rows * p.pieces < (1LL << 31)), "%s: too many rows", what);
+    GAN_CHECK_ARG(!too_many(rows, p), "%s: too many rows", what);
     GAN_CHECK_ARG(p.floats == 0 || (ws && ws_floats >= p.floats), "%s: workspace of %lld floats wanted, %lld given", what, (long long)p.floats,
                   (long long)(ws ? ws_floats : 0));
     GAN_CHECK_ARG(((uintptr_t)ws % 16) == 0, "%s: workspace must be 16-byte aligned", what);
@@ -877,14 +880,15 @@ int check_common(const char* what, int64_t rows, int64_t D, int dtype, float* ws
 }
 
 bool bad_shape(int64_t rows, int64_t D, int dtype) {
-    return rows < 0 || D <= 0 || D > (1 << 30) || (dtype != GAN_F32 && dtype != GAN_BF16);
+    return rows < 0 || rows >= (1LL << 31) || D <= 0 || D > (1 << 30) || (dtype != GAN_F32 && dtype != GAN_BF16);
 }
 
 }  // namespace
 
 extern "C" int64_t gan_layernorm_workspace(int64_t rows, int64_t D, int dtype, int pass, int columns) {
     if (bad_shape(rows, D, dtype) || pass < 0 || pass > 2) return -1;
-    return rows ? plan_of(rows, D, dtype, pass, columns != 0).floats : 0;
+    const Plan p = plan_of(rows ? rows : 1, D, dtype, pass, columns != 0);
+    return !rows ? 0 : too_many(rows, p) ? -1 : p.floats;
 }
 
 extern "C" int gan_layernorm_fwd(const void* x, const float* w, const float* b, void* y, float* stats, int64_t rows, int64_t D, float eps,

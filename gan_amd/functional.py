@@ -2596,7 +2596,7 @@ def layer_norm2d(x: Tensor, weight: Tensor, bias: Tensor, slope: float = 1.0, ep
 def _layer_norm_ws(rows: int, d: int, code: int, order: int, columns: bool) -> int:
     n = _lib.load().gan_layernorm_workspace(rows, d, code, order, int(columns))
     if n < 0:
-        raise _lib.GanAmdError(f"layer_norm: {rows} rows of {d} elements are not supported")
+        raise _lib.GanAmdError(f"layer_norm: {rows} rows of {d} elements are not supported (fewer than 2^31 rows of up to 2^30)")
     return n
 
 
@@ -2620,8 +2620,8 @@ def _launch(family: str, tensors, tag, fn, *args) -> None:
 def raw_layer_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], d: int, eps: float, keep: bool = True):
     """(y, stats (rows, 2), or None unless `keep`) of contiguous x, normalised over its last d elements."""
     rows, code = x.numel() // d, dtype_code(x)
-    y = torch.empty_like(x)
     n = _layer_norm_ws(rows, d, code, 0, False)
+    y = torch.empty_like(x)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if keep else None
     ws = x.new_empty((n,), dtype=torch.float32) if n else None
     _launch("layernorm", (x, y), (rows, d), _lib.load().gan_layernorm_fwd, x.data_ptr(), ptr(weight), ptr(bias), y.data_ptr(), ptr(stats), rows, d,

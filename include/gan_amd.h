@@ -346,7 +346,7 @@ int gan_space_to_depth(const void* x, void* out, int N, int H, int W, int C, int
  *                     any output may be NULL, cw and cb may be NULL (no such cotangent).
  * w NULL: ones; b NULL: zeros.  w, b, cw, cb, stats, gwb, gww are fp32; x, y, g, v, gx, gg, gxx of `dtype`, aligned to their
  * element only (any D); no output may overlap an input.  Column sums are added in an order that depends on the shape alone.
- * 1 <= D <= 2^30.
+ * 1 <= D <= 2^30, fewer than 2^31 rows and (rows of more than 4096 vectors of 16 bytes, 2048 in second order) 2^24 pieces of 16 KB.
  * workspace: gan_layernorm_workspace floats (pass 0 forward, 1 backward, 2 second; columns: gwb / gww wanted), 16-byte
  * aligned, may be NULL where that is 0; negative: the shape is refused. */
 int64_t gan_layernorm_workspace(int64_t rows, int64_t D, int dtype, int pass, int columns);

@@ -500,3 +500,19 @@ def test_gradients_changed_in_place_on_the_device(dev):
     from gan_amd import functional as GF
 
     check_gradients_changed_in_place(lambda x, w, b: GF.layer_norm(x, 40, w, b), dev)
+
+
+def test_workspace_query_refuses_what_the_calls_refuse():
+    from gan_amd import _lib
+
+    lib = _lib.load()
+    p = 4096  # never read
+    for rows, d, dtype in ((1 << 31, 8, 1), (1 << 62, 8, 1), (1 << 25, 1 << 15, 0), (64, 1 << 30, 0), (128, 1 << 30, 1), (1, (1 << 30) + 1, 0)):
+        for order in range(3):
+            assert lib.gan_layernorm_workspace(rows, d, dtype, order, 1) < 0, (rows, d, order)
+        assert lib.gan_layernorm_fwd(p, p, p, p, p, rows, d, 1e-5, dtype, p, 1 << 62, None) != 0
+        assert lib.gan_layernorm_bwd(p, p, p, p, p, p, rows, d, dtype, p, 1 << 62, None) != 0
+        assert lib.gan_layernorm_bwd2(p, p, p, p, p, p, p, p, p, p, rows, d, dtype, p, 1 << 62, None) != 0
+    for rows, d, dtype in (((1 << 31) - 1, 8, 1), (63, 1 << 30, 0), (1, 1 << 30, 0), (4096, 1 << 15, 0)):
+        for order in range(3):
+            assert lib.gan_layernorm_workspace(rows, d, dtype, order, 1) >= 0, (rows, d, order)
