@@ -349,8 +349,11 @@ __device__ __forceinline__ void col_sums(const RowArgs& a, float* __restrict__ o
 }
 
 template <typename T, int PASS>
-__global__ void __launch_bounds__(TPB) ln_cols_k(const RowArgs a, float* __restrict__ out, int64_t chunk) {
-    col_sums<T, PASS, TPB>(a, out, chunk, blockIdx.x, blockIdx.y);
+__global__ void __launch_bounds__(TPB) ln_cols_k(const RowArgs a, float* __restrict__ out, int64_t chunk, int tiles) {
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {  // (once, up to COL_TILES of them)
+        if (tile != (int)blockIdx.x) __syncthreads();
+        col_sums<T, PASS, TPB>(a, out, chunk, tile, blockIdx.y);
+    }
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------
@@ -716,6 +719,8 @@ struct Plan {
 
 // Four workgroups of 256 threads a CU; forward, with fewer registers, eight (65536 x 512 bf16: 23.8 us against 26.5).
 constexpr int MAXB = 1024;
+// Tiles of columns side by side in a launch (work items are counted in 32 bits: 2^24 workgroups of 256, fp32 rows of 2^30, are one too many)
+constexpr int COL_TILES = 1 << 23;
 
 // pass 0 forward, 1 backward, 2 second.  cols: column sums wanted.
 Plan plan_of(int64_t rows, int64_t D, int dtype, int pass, bool cols) {
@@ -859,8 +864,9 @@ int run_pass(const Plan& p, RowArgs a, float* gw, float* gb, float* ws, hipStrea
     }
     if constexpr (PASS > 0) {
         if (!summed) {
-            const dim3 grid((unsigned)ceil_div64(D, 16 * VecOf<T>::V), (unsigned)p.chunks);
-            hipLaunchKernelGGL((ln_cols_k<T, PASS>), grid, dim3(TPB), 0, st, a, sums, p.chunk);
+            const int tiles = (int)ceil_div64(D, 16 * VecOf<T>::V);
+            const dim3 grid((unsigned)(tiles < COL_TILES ? tiles : COL_TILES), (unsigned)p.chunks);
+            hipLaunchKernelGGL((ln_cols_k<T, PASS>), grid, dim3(TPB), 0, st, a, sums, p.chunk, tiles);
             GAN_CHECK_LAUNCH("layernorm(columns)");
         }
         if (cols && p.chunks > 1) {

@@ -516,3 +516,39 @@ def test_workspace_query_refuses_what_the_calls_refuse():
     for rows, d, dtype in (((1 << 31) - 1, 8, 1), (63, 1 << 30, 0), (1, 1 << 30, 0), (4096, 1 << 15, 0)):
         for order in range(3):
             assert lib.gan_layernorm_workspace(rows, d, dtype, order, 1) >= 0, (rows, d, order)
+
+
+@pytest.mark.gpu
+def test_the_longest_row(dev):
+    """2^30 elements, a tail of 2^30 - 3, in fp32: the most tiles of columns and pieces of a row.  Sums go over 2^18 pieces here,
+    1024 one after another in a thread: 1100 roundings, at most three such sums in a value, 4096 roundings asked."""
+    from gan_amd import functional as GF
+
+    for d in ((1 << 30) - 3, 1 << 30):
+        torch.manual_seed(7)
+        x = torch.randn(1, d, device=dev).add_(0.5).requires_grad_()
+        w = torch.randn(d, device=dev).requires_grad_()
+        b = torch.zeros(d, device=dev).requires_grad_()
+        g = torch.randn(1, d, device=dev)
+        y = GF.layer_norm(x, d, w, b)
+        gx, gw, gb = torch.autograd.grad(y, (x, w, b), g)
+        parts = [slice(k, min(k + (1 << 27), d)) for k in range(0, d, 1 << 27)]
+        x, w, g, y, gx = (t.detach().view(-1) for t in (x, w, g, y, gx))
+        mean = sum(x[p].double().sum() for p in parts) / d
+        size = sum(x[p].double().abs().sum() for p in parts) / d
+        r = (sum((x[p].double() - mean).square().sum() for p in parts) / d + 1e-5).rsqrt()
+        hm = sum((g[p].double() * w[p].double()).sum() for p in parts) / d
+        ht = sum((g[p].double() * w[p].double() * (x[p].double() - mean) * r).sum() for p in parts) / d
+        ha = sum((g[p].double() * w[p].double()).abs().sum() for p in parts) / d
+        for p in (parts[0], parts[-1]):
+            t = (x[p].double() - mean) * r
+            ta = t.abs() + (size + x[p].double().abs()) * r
+            h = g[p].double() * w[p].double()
+            lim = 4096 * U
+            assert ((y[p].double() - t * w[p].double()).abs() <= lim * ta * w[p].double().abs() + 1e-37).all()
+            assert ((gw[p].double() - g[p].double() * t).abs() <= lim * g[p].double().abs() * ta + 1e-37).all()
+            assert torch.equal(gb[p], g[p])
+            # (|mean(h t)| <= mean |h| * max |t| and |t| < 8 here)
+            assert ((gx[p].double() - r * (h - hm - t * ht)).abs() <= lim * r * (h.abs() + ha + 8 * ta * ha)).all()
+        del x, w, b, g, y, gx, gw, gb, t, ta, h
+        torch.cuda.empty_cache()
