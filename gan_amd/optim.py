@@ -210,7 +210,8 @@ def _muon_launch(mats, like: Tensor, lr, momentum, nesterov, weight_decay, adjus
 
 class FlatMuon(torch.optim.Optimizer):
     """muon_step over a FlatArena for the matrices of a network, Adam for the rest of it (biases, norm scales, and whatever is a
-    vector in a matrix's shape: one row or one column), in place on the arenas.
+    vector in a matrix's shape: one row or one column), in place on the arenas.  Where every parameter is two-dimensional, which
+    is what torch.optim.Muon takes, all of them are matrices, as there, those of one row or column too.
 
     * two `param_groups`: the matrices (`lr`, `weight_decay`, `momentum`, `nesterov`, `ns_coefficients`, `eps`, `ns_steps`,
       `adjust_lr_fn`: torch.optim.Muon's names and update rule, its products in 22 bits instead of bfloat16's 8) and the rest
@@ -229,7 +230,8 @@ class FlatMuon(torch.optim.Optimizer):
         if adjust_lr_fn not in _SCALINGS:
             raise ValueError(f"FlatMuon: adjust_lr_fn must be None, 'original', 'match_rms_adamw' or 'none', got {adjust_lr_fn!r}")
         self.arena = arena
-        self._matrix = [p.dim() >= 2 and min(_as_matrix(p.shape)) > 1 for p in arena.params]
+        least = 1 if all(p.dim() == 2 for p in arena.params) else 2  # (what torch.optim.Muon takes goes all the same way, as there)
+        self._matrix = [p.dim() >= 2 and min(_as_matrix(p.shape)) >= least for p in arena.params]
         matrices = [p for p, m in zip(arena.params, self._matrix) if m]
         rest = [p for p, m in zip(arena.params, self._matrix) if not m]
         groups = []
@@ -317,7 +319,9 @@ class FlatMuon(torch.optim.Optimizer):
 
 def make_optimizer(name: str, module: nn.Module, lr: float, kwargs: Dict, *, capturable: bool = False) -> torch.optim.Optimizer:
     """The optimizer `name` (a torch.optim class name, train_celeba.py:75) for `module`'s parameters.  Adam / AdamW with
-    only betas / eps / weight_decay set run as FlatAdam on a ROCm device, Muon as FlatMuon; everything else is torch's own class
+    only betas / eps / weight_decay set run as FlatAdam on a ROCm device, Muon as FlatMuon (matrices, convolutions among them, by their
+    orthogonalised momentum; biases, norm scales and, beside such, matrices of one row or column by Adam at `adam_lr`, which is the
+    matrices' `lr` unless given, ten times and more of what Adam usually gets); everything else is torch's own class
     (with capturable=True where it exists and the step is going to be captured in a HIP graph)."""
     params = list(module.parameters())
     on_gpu = bool(params) and all(p.is_cuda and p.dtype == torch.float32 for p in params)

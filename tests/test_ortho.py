@@ -642,3 +642,34 @@ def test_dual_tensors_are_refused():
         with pytest.raises(_lib.GanAmdError) as plain:
             GF.orthogonalize(x)
         assert "derivative" not in str(plain.value)  # (not on a ROCm device)
+
+
+@pytest.mark.gpu
+def test_modules_that_torch_muon_takes(dev):
+    """Two-dimensional parameters only: every one of them goes by the rule of torch.optim.Muon, a head of one row too.  (torch's
+    class runs on the CPU, its products in bfloat16: five steps of three roundings of 2^-8, a few times that after their
+    amplification; a quarter of the update is asked.  Adam's update of a row of 30 would be 5 times the rule's.)"""
+    from torch import nn
+
+    from gan_amd.optim import make_optimizer
+
+    torch.manual_seed(2)
+    net = nn.Sequential(nn.Linear(20, 30, bias=False), nn.Linear(30, 1, bias=False), nn.Linear(1, 6, bias=False)).to(dev)
+    twin = [nn.Parameter(p.detach().cpu().clone()) for p in net.parameters()]
+    opt = make_optimizer("Muon", net, 0.05, {"weight_decay": 0.02, "momentum": 0.8})
+    stock = torch.optim.Muon(twin, lr=0.05, weight_decay=0.02, momentum=0.8)
+    assert len(opt.param_groups) == 1 and all(set(opt.state[p]) == {"momentum_buffer"} for p in net.parameters())
+    ref = [p.detach().double().clone() for p in twin]
+    m = [torch.zeros_like(r) for r in ref]
+    for _ in range(3):
+        for i, (p, q) in enumerate(zip(net.parameters(), twin)):
+            q.grad = torch.randn(q.shape)
+            p.grad = q.grad.to(dev)
+        before = [p.detach().clone() for p in twin]
+        opt.step(), stock.step()
+        for i, (p, q) in enumerate(zip(net.parameters(), twin)):
+            old = ref[i]
+            ref[i], m[i] = step_ref(old, q.grad, m[i], 0.05, 0.8, True, 0.02, None)
+            assert float((p.detach().double().cpu() - ref[i]).norm()) <= 1e-5 * float(ref[i].norm()) + 6e-4 * 0.05 * 3 * min(p.shape) ** 0.5
+            step = q.detach().double() - before[i].double()
+            assert float((step - (ref[i] - old)).norm()) <= 0.25 * float((ref[i] - old).norm())
