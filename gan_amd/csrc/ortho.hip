@@ -81,6 +81,7 @@ struct Mat {
 struct Source {
     float mu, eps;
     int nesterov;
+    float growth;  // what the steps can multiply X by at most (1 at least)
 };
 
 struct Mats {
@@ -90,8 +91,9 @@ struct Mats {
     Mat mat[NOPS];
 };
 
-// Byte offsets in one matrix's workspace: the partial sums, two X (m x n), five symmetric m x m, the slices' tiles of a product that is cut.  All multiples of 256.
+// Byte offsets in one matrix's workspace: the partial sums, 1 / lift (256 bytes), two X (m x n), five symmetric m x m, the slices' tiles of a product that is cut.  All multiples of 256.
 enum { A0, A1, P0, P1, Q0, SQUARES };
+constexpr int LIFT_AT = MAXPARTS * 8;
 struct Lay {
     int64_t mp, np, nparts, x[2], sq[SQUARES], join, bytes;
     int cut;
@@ -149,7 +151,7 @@ Lay lay_of(const gan_matrix& g) {
     l.mp = up64(rows < cols ? rows : cols);
     l.np = up64(rows < cols ? cols : rows);
     l.nparts = parts_of(rows * cols);
-    int64_t at = MAXPARTS * 8;
+    int64_t at = LIFT_AT + 256;
     const int64_t x = l.mp * l.np * 4, sq = l.mp * l.mp * 4;
     for (int k = 0; k < 2; ++k) {
         l.x[k] = at;
@@ -240,17 +242,33 @@ __global__ void __launch_bounds__(256) ortho_norm_k(const Mats s) {
     if (threadIdx.x == 0) ((double*)(q.ws + b * q.stride))[c] = red[0] + red[1] + red[2] + red[3];
 }
 
-// SX / max(|u|, eps) of a matrix, every workgroup for itself and all the same: the partial sums in their order.  Not finite:
-// NaN, so that the whole matrix says so.
-__device__ __forceinline__ float scale_of(const double* part, int nparts, float eps) {
+// SX / max(|u|, eps) times the lift.  A matrix of a norm far below eps stays small through all steps; its halves would fall into fp16's
+// subnormals (a norm of 1e-5 eps: four digits), so X is held a power of two higher, as far as `growth` leaves room: 1 for a norm of
+// eps and more.  (One for all steps: an entry of average size then is held to 2^-38 growth sqrt(m n) of it, 2.7e-6 for 512 x 4608 in
+// five.)  A is held as it is (as small as it then is, P is a I and little else).  Not finite: NaN, so that the whole matrix says so.
+__device__ __forceinline__ float scale_of(double norm, const Source& s, float& lift) {
+    lift = 1.f;
+    if (!(norm < 1e300)) return __builtin_nanf("");
+    double scale = (double)SX / (norm > (double)s.eps ? norm : (double)s.eps);
+    int up;
+    frexp(norm / (double)s.eps * (double)s.growth, &up);
+    if (norm > 0. && up < 0) {
+        for (up = up < -100 ? -100 : up; up < 0 && ldexp(scale, -up) > 1e37; ++up) {}  // (fp32)
+        lift = (float)ldexp(1., -up);
+        scale = ldexp(scale, -up);
+    }
+    return (float)scale;
+}
+
+// Of the partial sums in their order, every workgroup for itself and all the same
+__device__ __forceinline__ float scale_of(const double* part, int nparts, const Source& s, float& lift) {
     __shared__ double red[4];
     double sum = 0.;
     for (int i = threadIdx.x; i < nparts; i += 256) sum += part[i];
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
     __syncthreads();
-    const double n = sqrt(red[0] + red[1] + red[2] + red[3]);
-    return n < 1e300 ? (float)((double)SX / (n > (double)eps ? n : (double)eps)) : __builtin_nanf("");
+    return scale_of(sqrt(red[0] + red[1] + red[2] + red[3]), s, lift);
 }
 
 // ---- the scaled source as m x n, padded with zeros (a tall source transposed) --------------------------------------------
@@ -277,7 +295,9 @@ __global__ void __launch_bounds__(256) ortho_pack_k(const Mats s) {
         if (buf) m[k] = buf[at];
         if (!in) v[k] = m[k] = 0.f;
     }
-    const float scale = scale_of((const double*)ws, (int)parts_of(size), s.from.eps);
+    float lift;
+    const float scale = scale_of((const double*)ws, (int)parts_of(size), s.from, lift);
+    if (t == 0 && threadIdx.x == 0) *(float*)(ws + LIFT_AT) = 1.f / lift;
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
         const int r = k * 4 + (threadIdx.x >> 6), c = threadIdx.x & 63;
@@ -312,6 +332,7 @@ struct Op {
     int tiles;         // per matrix
     int cut, steps;    // slices of k, steps of 32 k in each but the last
     int kind;
+    int lifts;         // how often X is a factor of the product without being one of the result
     float gain;        // of the product; P and what CHAIN adds have the scale SP, POLY's A has SA
 };
 
@@ -382,7 +403,13 @@ __device__ __forceinline__ void store_result(const Rule& rule, T* to, float (&o)
     }
 }
 
-__device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int b, int i0, int j0, f32x16& acc, bool mirror, int dtype, float* t) {
+// 1 / lift where the product has it too often.  (A scalar load: the kernels' vector loads are counted, and none is waited for early.)
+__device__ __forceinline__ float unlift_of(const Op& q, const char* ws) {
+    return q.lifts ? *(const __attribute__((address_space(4))) float*)(uintptr_t)(ws + LIFT_AT) : 1.f;
+}
+
+__device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, float unlift, int b, int i0, int j0, f32x16& acc, bool mirror, int dtype,
+                                       float* t) {
     const int lane = threadIdx.x & 63;
     // the values first, where the accumulators hold them: no branch or load stands between the trips through LDS
     if (q.kind == POLY || q.kind == CHAIN) {  // (what is added is symmetric: its rows for the columns held here)
@@ -414,7 +441,7 @@ __device__ __forceinline__ void finish(const Ops& s, const Op& q, char* ws, int 
             for (int r = 0; r < 16; ++r) acc[r] += on == 8 * (r >> 2) + (r & 3) ? s.rule.a * SP : 0.f;
         }
     } else {
-        const float gain = q.kind == SCALED ? q.gain : 1.f / (SP * SX);
+        const float gain = (q.kind == SCALED ? q.gain : 1.f / (SP * SX)) * unlift * (q.lifts == 2 ? unlift : 1.f);
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] *= gain;
     }
@@ -562,6 +589,7 @@ __global__ void __launch_bounds__(T == 256 ? 512 : 256 * KG, T == 64 ? 4 : 2) or
     const int in_b = id - b * per;
     const int slice = __builtin_amdgcn_readfirstlane(in_b / q.tiles), tile = in_b - slice * q.tiles;
     char* ws = q.ws + b * q.stride;
+    const float unlift = unlift_of(q, ws);  // (here, so that nobody waits for it at the end)
     const char *u = ws + (int64_t)q.u * 256, *v = ws + (int64_t)q.v * 256;
     const int M = q.M, N = q.N, K = q.K;
     int ti, tj;
@@ -757,7 +785,7 @@ __global__ void __launch_bounds__(T == 256 ? 512 : 256 * KG, T == 64 ? 4 : 2) or
 #pragma unroll
             for (int r = 0; r < 4; ++r) out[(f * 4 + r) * 64] = make_float4(one[r * 4], one[r * 4 + 1], one[r * 4 + 2], one[r * 4 + 3]);
         } else if (i < M && j < N) {
-            finish(s, q, ws, b, i, j, one, !q.apply && ti != tj, dtype, t);
+            finish(s, q, ws, unlift, b, i, j, one, !q.apply && ti != tj, dtype, t);
         }
     }
 }
@@ -772,6 +800,7 @@ __global__ void __launch_bounds__(64) ortho_join_k(const Ops s, int dtype) {
     const int lane = threadIdx.x;
     const int local = (int)blockIdx.x - s.first[group], tile_b = local / BLK, b = tile_b / q.tiles, tile = tile_b - b * q.tiles;
     char* ws = q.ws + b * q.stride;
+    const float unlift = unlift_of(q, ws);
     const int blk = local % BLK, wave = blk / (BLK / WAVES), frag = blk % (BLK / WAVES);
     const float4* in = (const float4*)(ws + (int64_t)q.join * 256) + (int64_t)tile * (T * T / 4) + blk * 256 + lane;
     const int64_t next = (int64_t)q.tiles * (T * T / 4);
@@ -799,7 +828,7 @@ __global__ void __launch_bounds__(64) ortho_join_k(const Ops s, int dtype) {
     }
     const int2 t = tile_of(tile, (q.M + T - 1) / T);
     const int i = t.x * T + (wave / WN) * (T / 2) + frag / FN * 32, j = t.y * T + (wave % WN) * (T / WN) + frag % FN * 32;
-    if (i < q.M && j < q.N) finish(s, q, ws, b, i, j, acc, t.x != t.y, dtype, lds);
+    if (i < q.M && j < q.N) finish(s, q, ws, unlift, b, i, j, acc, t.x != t.y, dtype, lds);
 }
 
 template <int T, int NST, int KG>
@@ -859,6 +888,7 @@ struct Walk {
             o.apply = 0;
             o.gain = gain;
             o.kind = kind;
+            o.lifts = kind == RESULT ? 1 : 0;
             o.cut = 1;
             o.M = o.N = o.K = (int)l.mp;
         };
@@ -866,6 +896,7 @@ struct Walk {
         const int last = size == 1 ? 2 : beside ? 5 : 6;
         if (at == 0) {
             mul(0, 0, A0, SA / (SX * SX));
+            q->lifts = 2;
             q->u = q->v = (unsigned)(l.x[cur] / 256);
             q->K = (int)l.np;
             q->cut = l.cut;
@@ -1199,7 +1230,9 @@ __global__ void __launch_bounds__(1024) ortho_small_k(const Smalls s, const Sour
 #pragma unroll
     for (int w = 0; w < 16; ++w) sum += red[w];
     const double norm = sqrt(sum);
-    const float scale = norm < 1e300 ? (float)((double)SX / (norm > (double)h.eps ? norm : (double)h.eps)) : __builtin_nanf("");
+    float lift;
+    const float scale = scale_of(norm, h, lift);
+    const float unlift = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, 1.f / lift)));
     each([&](int k, int j, int i) __attribute__((always_inline)) {
         float v[4];
 #pragma unroll
@@ -1227,7 +1260,7 @@ __global__ void __launch_bounds__(1024) ortho_small_k(const Smalls s, const Sour
             if (si == sj) small_part<true, true, 0>(acc, X, si, X, sj, 0, bn);
             else small_part<true, true, 1>(acc, X, si, X, sj, 0, bn);
             acc[0] += acc[1];
-            Q.store(si, sj, acc[0], SA / (SX * SX));
+            Q.store(si, sj, acc[0], SA / (SX * SX) * unlift * unlift);
         }
         __syncthreads();
         if (square) {
@@ -1298,7 +1331,7 @@ __global__ void __launch_bounds__(1024) ortho_small_k(const Smalls s, const Sour
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int e = 8 * (r >> 2) + (r & 3);
-            const float x = acc[z][r] * (1.f / (SP * SX));
+            const float x = acc[z][r] * (1.f / (SP * SX) * unlift);
             if (e < in) element(out, at + e * di) = (T)(o.update ? fmaf(-shaped, x, o.decay * old[r]) : x);
         }
     }
@@ -1329,8 +1362,10 @@ int run_small(const gan_matrix* mats, int n, int steps, const Source& h, const R
 }
 
 // The largest factor that a singular value can have grown to after each step, from 1: extremes of x |a + b x^2 + c x^4| on [0, r].
-bool bounded(int steps, float a, float b, float c) {
-    double r = 1.0;
+// growth: of the steps' factors |a + b x^2 + c x^4|, the largest product of the first ones.
+bool bounded(int steps, float a, float b, float c, float& growth) {
+    double r = 1.0, grown = 1.0;
+    growth = 1.f;
     for (int k = 0; k < steps; ++k) {
         auto f = [&](double x) { return fabs(x * (a + b * x * x + c * x * x * x * x)); };
         auto p = [&](double x) { return fabs(a + b * x * x + c * x * x * x * x); };
@@ -1354,6 +1389,8 @@ bool bounded(int steps, float a, float b, float c) {
             }
         if (!(top <= 3.5) || !(poly <= 60.)) return false;  // (NaN too)
         r = top > 1e-3 ? top : 1e-3;
+        grown *= poly;
+        if (grown > growth) growth = grown < 1e30 ? (float)grown : 1e30f;
     }
     return true;
 }
@@ -1411,13 +1448,13 @@ bool all_small(const gan_matrix* mats, int count) {
     return true;
 }
 
-int run_all(const char* what, const gan_matrix* all, int count, int steps, const Source& source, const Rule& rule, int dtype, char* ws, int64_t bytes,
+int run_all(const char* what, const gan_matrix* all, int count, int steps, Source source, const Rule& rule, int dtype, char* ws, int64_t bytes,
             hipStream_t st) {
     GAN_CHECK_ARG(count >= 0 && (count == 0 || all), "%s: null list", what);
     GAN_CHECK_ARG(steps >= 1 && steps <= 100, "%s: 1 to 100 steps, got %d", what, steps);
     // (SX / eps has to be a finite fp32)
     GAN_CHECK_ARG(source.eps >= 1e-30f && source.eps <= 1e30f, "%s: eps must be positive, 1e-30 to 1e30, got %g", what, (double)source.eps);
-    GAN_CHECK_ARG(bounded(steps, rule.a, rule.b, rule.c), "%s: with coefficients %g %g %g a singular value can grow beyond 3.5", what, (double)rule.a,
+    GAN_CHECK_ARG(bounded(steps, rule.a, rule.b, rule.c, source.growth), "%s: with coefficients %g %g %g a singular value can grow beyond 3.5", what, (double)rule.a,
                   (double)rule.b, (double)rule.c);
     const int64_t need = total_bytes(all, count);
     GAN_CHECK_ARG(need >= 0, "%s: a matrix has a size that is not supported (1 to 2^20 either way, the smaller at most 32768, fewer than 2^30 elements when padded to 64s, fewer than 2^22 of them in a batch, in 2^23 blocks of 64 x 64)", what);
@@ -1482,7 +1519,7 @@ extern "C" int gan_orthogonalize(const gan_matrix* mats, int count, int steps, f
                                  int64_t ws_bytes, gan_stream_t stream) {
     GAN_CHECK_ARG(dtype == GAN_F32 || dtype == GAN_BF16, "orthogonalize: bad dtype %d", dtype);
     for (int k = 0; mats && k < count; ++k) GAN_CHECK_ARG(!mats[k].buf, "orthogonalize: matrix %d has a momentum buffer", k);
-    return run_all("orthogonalize", mats, count, steps, Source{0.f, eps, 0}, Rule{a, b, c, 1.f, 0.f, 0}, dtype, (char*)ws, ws_bytes, (hipStream_t)stream);
+    return run_all("orthogonalize", mats, count, steps, Source{0.f, eps, 0, 1.f}, Rule{a, b, c, 1.f, 0.f, 0}, dtype, (char*)ws, ws_bytes, (hipStream_t)stream);
 }
 
 extern "C" int gan_muon_step(const gan_matrix* mats, int count, float lr, float momentum, int nesterov, float weight_decay, int scaling, int steps,
@@ -1490,6 +1527,6 @@ extern "C" int gan_muon_step(const gan_matrix* mats, int count, float lr, float 
     GAN_CHECK_ARG(lr >= 0.f && momentum >= 0.f && momentum < 1.f && weight_decay >= 0.f,
                   "muon_step: bad hyper-parameters (lr %g, momentum %g, weight_decay %g)", (double)lr, (double)momentum, (double)weight_decay);
     GAN_CHECK_ARG(scaling >= 0 && scaling <= 2, "muon_step: bad scaling %d", scaling);
-    return run_all("muon_step", mats, count, steps, Source{momentum, eps, nesterov}, Rule{a, b, c, 1.f - lr * weight_decay, lr, 1 + scaling}, GAN_F32,
+    return run_all("muon_step", mats, count, steps, Source{momentum, eps, nesterov, 1.f}, Rule{a, b, c, 1.f - lr * weight_decay, lr, 1 + scaling}, GAN_F32,
                    (char*)ws, ws_bytes, (hipStream_t)stream);
 }

@@ -673,3 +673,35 @@ def test_modules_that_torch_muon_takes(dev):
             assert float((p.detach().double().cpu() - ref[i]).norm()) <= 1e-5 * float(ref[i].norm()) + 6e-4 * 0.05 * 3 * min(p.shape) ** 0.5
             step = q.detach().double() - before[i].double()
             assert float((step - (ref[i] - old)).norm()) <= 0.25 * float((ref[i] - old).norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(40, 150), (300, 1200), (200, 70), (1, 9), (512, 4608)])
+def test_norms_far_below_eps(dev, m, n):
+    """X = G / eps stays small through all steps, which then multiply by little more than a: three roundings of 2^-22 a step, 15 in
+    all, 3.6e-6; 1e-5 is asked, whatever the norm.  In LDS and not, with sums in slices, as a batch beside matrices of other norms."""
+    from gan_amd import functional as GF
+    from gan_amd.optim import muon_step
+
+    g = make(m, n, dev)
+    g = g / g.norm()
+    for norm, eps in ((1e-9, 1e-7), (1e-13, 1e-7), (1e-18, 1e-7), (1e-30, 1e-7), (1.0, 1e4), (1e-3, 1e30), (1e-33, 1e-30), (1e-36, 1e-30)):
+        x = g * norm
+        want = definition(x, eps=eps)
+        assert rel_err(GF.orthogonalize(x, eps=eps), want) < 1e-5, (norm, eps)
+        mixed = torch.stack([g, x, torch.zeros_like(g), 3 * g])
+        got = GF.orthogonalize(mixed, eps=eps)
+        assert rel_err(got[1], want) < 1e-5 and torch.equal(got[2], torch.zeros_like(g))
+    x = (g * 1e-13).bfloat16()
+    assert rel_err(GF.orthogonalize(x), definition(x)) < 1e-5 + 2.0**-8
+    for steps, coefficients in ((1, COEFFS), (8, COEFFS), (12, (1.5, -0.5, 0.0)), (3, (0.5, 0.1, 0.0))):
+        # X is held under one power of two through all steps, so that what it grows to, by up to a factor a^steps, has room: at first
+        # its norm then is as little as 1 / (2 a^steps), an entry of average size 1 / (2 a^steps sqrt(m n)), and an entry is held to
+        # half of fp16's least step under the scale 2^14, 2^-25 / 2^14: 2^-38 a^steps sqrt(m n) relative to it.  (Eight steps of 512 x
+        # 4608: 3.4445^8 = 19820, 1536 / 2^38 * 19820 = 1.1e-4, where 27 * 2^-22 alone is 6.4e-6.)
+        faint = 2.0**-38 * max(1.0, coefficients[0]) ** steps * math.sqrt(m * n)
+        want = definition(g * 1e-12, steps, coefficients)
+        assert rel_err(GF.orthogonalize(g * 1e-12, steps=steps, coefficients=coefficients), want) < 3 * (steps + 1) * 2.0**-22 + faint, steps
+    p, buf = torch.zeros_like(g), torch.zeros_like(g)
+    muon_step([p], [g * 1e-12], [buf], lr=1.0, momentum=0.5, adjust_lr_fn="none")
+    assert rel_err(-p, definition(g * 0.75e-12)) < 1e-5
