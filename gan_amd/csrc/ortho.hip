@@ -855,14 +855,15 @@ int launch_gemm(unsigned blocks, const Ops& s, int dtype, hipStream_t st) {
 // stage is a single iteration: the small values are smallest there.
 // Side by side is a product more and a launch less: taken where two products of each matrix leave no CU with more than one tile,
 // the launch then being as long as one (512 x 4608: 195 -> 184 us, 704 x 1500 187 -> 178; 1000 x 4000, which has more tiles, gains nothing).
-// Up to 128 rows they are not taken, alone or in a list (13 of 70 x 2589: 3.7e-6 in 143 us against 1.4e-6 in 163, where fp32 products
-// give 1.6e-6; 64 x 576 in a discriminator's list 3.6e-6 against 1.2e-6, fp32 products 2.0e-6, for 408 us of that list instead of
-// 393).  Beyond that they have to gain a launch's time by the cost rule: else step by step it is, the more accurate way (300 x 700: 0.7e-6
-// in 122 us against 1.8e-6 in 121; 512 x 4608: 1.2e-6 in 193 us, taken are 1.6e-6 in 175).  Where several sizes share the launches, all
-// of more than 128 rows go the same way as far as they can, whatever each would gain alone: a discriminator's step takes 408 us, 485
-// with some of its large matrices step by step, and their errors stay under 0.7 of those of fp32 products (0.4 to 0.6 step by step).
+// Up to 192 rows they are not taken, alone or in a list, where they leave more than fp32 products do (13 of 70 x 2589: 3.7e-6 in 143 us
+// against 1.4e-6 in 163, fp32 products 1.6e-6; in lists 64 x 576 3.6e-6 against 1.2e-6, fp32 products 2.0e-6, and 171 x 340 2.2e-6
+// against 1.0e-6, 1.6e-6; a discriminator's list takes 400 to 411 us instead of 393 for it).  Beyond that they have to gain a launch's time by
+// the cost rule: else step by step it is, the more accurate way (300 x 700: 0.7e-6 in 122 us against 1.8e-6 in 121; 512 x 4608: 1.2e-6 in
+// 193 us, taken are 1.6e-6 in 175).  Where several sizes share the launches, all of more than 192 rows go the same way as far as they
+// can, whatever each would gain alone: a discriminator's step would take 485 us with some of its large matrices step by step; their errors
+// are 0.4 to 1.2 times those of fp32 products, most at 193 to 256 rows (0.4 to 0.6 step by step).
 bool two_at_a_time(const Lay& l, int64_t batch, bool beside, bool shared) {
-    if (l.np < 2 * l.mp || l.mp <= 128) return false;
+    if (l.np < 2 * l.mp || l.mp <= 192) return false;
     if (shared) return true;
     const double gram = least_cost(l.mp, l.mp, l.np, true, batch, l.cut), apply = least_cost(l.mp, l.np, l.mp, false, batch, 1),
                  square = least_cost(l.mp, l.mp, l.mp, true, batch, 1);

@@ -523,27 +523,28 @@ def test_refusals():
 
 @pytest.mark.gpu
 def test_narrow_matrices_in_a_list(dev):
-    """Up to 128 rows a matrix goes step by step in a list too: no less accurate than the same iteration in fp32 products, on the
-    average of five that are wide enough for two iterations from one A (which leave 1.1 to 2.3 times that error, measured; step by
+    """Up to 192 rows a matrix goes step by step in a list too: no less accurate than the same iteration in fp32 products, on the
+    average of some that are wide enough for two iterations from one A (which leave 1.1 to 2.3 times that error, measured; step by
     step 0.6 to 0.8).  With no momentum, a step of 1 from zero is the orthogonalised gradient itself."""
     from gan_amd.optim import muon_step
 
-    shapes = [(32, 288), (64, 288), (64, 576), (128, 576), (128, 1152), (300, 1000)]
+    shapes = [(32, 288), (64, 288), (64, 576), (128, 576), (128, 1152), (340, 171), (150, 800), (300, 1000)]
     gen = torch.Generator(device="cpu").manual_seed(11)
-    ratios = []
+    ratios, late = [], []
     for _ in range(3):
         g = [(0.25 * torch.randn(m, 16, generator=gen) @ torch.randn(16, n, generator=gen) + 0.5 * torch.randn(m, n, generator=gen)).to(dev) for m, n in shapes]
         p, buf = ([torch.zeros_like(t) for t in g] for _ in range(2))
         muon_step(p, g, buf, lr=1.0, momentum=0.0, nesterov=False, adjust_lr_fn="none")
-        for got, t in list(zip(p, g))[:5]:
+        for got, t in list(zip(p, g))[:7]:
             want = definition(t)
             a, b, c = COEFFS
-            x = t / t.norm()
+            x = t / t.norm() if t.shape[0] <= t.shape[1] else (t / t.norm()).t().contiguous()
             for _ in range(5):
                 gram = x @ x.t().contiguous()
                 x = a * x + (b * gram + c * (gram @ gram)) @ x
-            ratios.append(rel_err(-got, want) / rel_err(x, want))
-    assert sum(ratios) / len(ratios) < 1.0, ratios
+            x = x if t.shape[0] <= t.shape[1] else x.t()
+            (ratios if t.shape[1] > 171 and t.shape[0] <= 128 else late).append(rel_err(-got, want) / rel_err(x, want))
+    assert sum(ratios) / len(ratios) < 1.0 and sum(late) / len(late) < 1.0, (ratios, late)
 
 
 def test_limits_of_a_batch():
