@@ -3,7 +3,10 @@
 //   A = X X',  P = a I + b A + c A A,  X <- P X
 // Every product is C = U V' on 16-bit matrix instructions with 32-bit accuracy: a value is held as two fp16 planes
 // (hi + lo, 22 bits, times a power of two that its bound allows: |X|, |A|, |P| have bounds that the coefficients set), and
-// hi hi + hi lo + lo hi are accumulated in fp32.  The dropped lo lo is 2^-24 of the product.  Three fp16 products cost a third
+// hi hi + hi lo + lo hi are accumulated in fp32.  The dropped lo lo is 2^-24 of the product.  (22 bits end where the lo half falls into
+// fp16's subnormals: entries of X below 1.5e-5 of the norm are held to 2e-12 of it, of A to 7e-12, of P to 2e-9.  Rows of 1e-4 of the
+// others' size come out to 8e-6 of their own, of 1e-6 to 8e-4; the whole of the matrix is within 2e-6 all the same, and a scale of
+// its own for every row would cost a pass over X a step.)  Three fp16 products cost a third
 // of the fp16 rate, and fp32 matrix instructions run at an eighth of it (1.18 PFLOP/s and 0.154 for large products).
 // Measured: P X of 2048 x 8192 in 166 us = 1.24 PFLOP/s of fp16 (0.41 of fp32 accuracy), A = X X' of it in 116 us (0.94; half
 // of A is computed), A A in 37 (0.74: 136 tiles for 256 CUs); five iterations 1290 to 1460 us by the clock that

@@ -447,9 +447,10 @@ int gan_adam_step_ranges(float* p, const float* g, float* m, float* v, const int
 /* ---- orthogonalised updates: X = G / max(|G|, eps) (Frobenius norm; m x n, m <= n, a tall G as its transpose), then `steps`
  * times X <- (a I + b A + c A A) X with A = X X' (Newton-Schulz).  A gan_matrix is `batch` (0: none) dense row-major
  * (rows, cols) matrices one behind the other; a call takes a list of them, of any sizes.
- * gan_orthogonalize: out = X of g, both of `dtype`; buf must be NULL.  Products carry 22 bits of every factor and are
- *                    accumulated in fp32, whatever the dtype.  A matrix of zeros gives zeros, one with a value that is not
- *                    finite NaN throughout; the others of the call are not touched by it.
+ * gan_orthogonalize: out = X of g, both of `dtype`; buf must be NULL.  Products carry 22 bits of every factor (of X down
+ *                    to 1.5e-5 of the norm, fainter entries 2e-12 of it) and are accumulated in fp32, whatever the dtype.  A
+ *                    matrix of zeros gives zeros, one with a value that is not finite NaN throughout; the others of the call
+ *                    are not touched by it.
  * gan_muon_step    : fp32; buf = momentum buf + (1 - momentum) g;  u = nesterov ? momentum buf + (1 - momentum) g : buf;
  *                    out = (1 - lr weight_decay) out - lr s X(u) with s = 1 (scaling 0), sqrt(max(1, rows / cols)) (1) or
  *                    0.2 sqrt(max(rows, cols)) (2).
