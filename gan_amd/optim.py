@@ -280,7 +280,10 @@ class FlatMuon(torch.optim.Optimizer):
         base = arena.grad.data_ptr()
         present = tuple(p.grad is not None and p.requires_grad for p in arena.params)
         if any(p.grad is not None and p.grad.data_ptr() != base + 4 * o for p, o in zip(arena.params, arena.offsets)):
+            absent = [p for p in arena.params if p.grad is None]
             arena.gather_grads()  # re-attaches every slice; `present` remembers who really had a gradient
+            for p in absent:  # (a slice of zeros would count as a gradient from the next step on)
+                p.grad = None
         mats, ranges = self._matrices(present)
         groups = {("momentum" in g): g for g in self.param_groups}
         if len(mats):

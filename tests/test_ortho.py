@@ -706,3 +706,39 @@ def test_norms_far_below_eps(dev, m, n):
     p, buf = torch.zeros_like(g), torch.zeros_like(g)
     muon_step([p], [g * 1e-12], [buf], lr=1.0, momentum=0.5, adjust_lr_fn="none")
     assert rel_err(-p, definition(g * 0.75e-12)) < 1e-5
+
+
+@pytest.mark.gpu
+def test_parameters_without_a_gradient_stay_out(dev):
+    """Whose .grad is None is skipped in every step, not in the first one only: no decay, no update by what its momentum still
+    holds (an orthogonalised momentum is full-sized however small it has become), the state as it was, .grad None as it was."""
+    from torch import nn
+
+    from gan_amd.optim import make_optimizer
+
+    torch.manual_seed(4)
+    net = nn.ModuleList([nn.Linear(12, 8), nn.Linear(8, 6), nn.Conv2d(2, 3, 3)]).to(dev)
+    opt = make_optimizer("Muon", net, 0.05, {"weight_decay": 0.1})
+    params = list(net.parameters())
+    for p in params:
+        p.grad = torch.randn_like(p)
+    opt.step()  # momentum for all of them
+    idle = params[2:4]
+    held = [p.detach().clone() for p in idle]
+    state = [{k: v.clone() for k, v in opt.state[p].items() if k != "step"} for p in idle]
+    for p in idle:
+        p.grad = None
+    for _ in range(3):
+        before = [p.detach().clone() for p in params]
+        for p in params[:2] + params[4:]:
+            p.grad = torch.randn_like(p)
+        opt.step()
+        for i, (p, q) in enumerate(zip(params, before)):
+            assert torch.equal(p, q) == (i in (2, 3)), i
+        assert all(p.grad is None for p in idle)
+    for p, h, s in zip(idle, held, state):
+        assert torch.equal(p, h) and all(torch.equal(opt.state[p][k], v) for k, v in s.items())
+    for p in params:  # and they come back
+        p.grad = torch.randn_like(p)
+    opt.step()
+    assert not any(torch.equal(p, h) for p, h in zip(idle, held))
