@@ -10,7 +10,7 @@
 // of the fp16 rate, and fp32 matrix instructions run at an eighth of it (1.18 PFLOP/s and 0.154 for large products).
 // Measured: P X of 2048 x 8192 in 166 us = 1.24 PFLOP/s of fp16 (0.41 of fp32 accuracy), A = X X' of it in 116 us (0.94; half
 // of A is computed), A A in 37 (0.74: 136 tiles for 256 CUs); five iterations 1290 to 1460 us by the clock that
-// the card holds, of 512 x 4608 181 to 190.  Large products are
+// the card holds, of 512 x 4608 170 to 190.  Large products are
 // bound by the matrix instructions, those of a few hundred rows by their latency: 8 to 10 us a launch, 3 of them matrix
 // instructions, the others the way of the first requests through the caches and the end of the workgroup.
 // All matrices of a call share the launches (one per product), their tiles side by side in the grid; A and P are symmetric,
@@ -173,7 +173,7 @@ Lay lay_of(const gan_matrix& g) {
 }
 
 // The most workgroups that one of these matrices takes in a launch: a product's tiles of 64, or, where sums are cut in slices, up to
-// 4096 tiles of slices and 1024 / T^2 of a tile's blocks for the launch that joins them.
+// 4096 tiles of slices, or every 32 x 32 block on and above the diagonal, in whole tiles, for the launch that joins them.
 int64_t blocks_of(const Lay& l) {
     const int64_t t = l.mp / 64, tiles = t * (l.np / 64);
     return (tiles > l.nparts ? tiles : l.nparts) + (l.cut > 1 ? 4096 + 2 * (t + 3) * (t + 7) : 0);

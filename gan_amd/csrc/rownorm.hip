@@ -17,7 +17,7 @@
 // Sums and statistics are fp32 throughout; bf16 results are rounded once, on the store.
 // Measured, launches alone, of 5.0 TB/s that a copy reaches (in brackets the bytes' time at that rate):
 //                          forward        backward, x only   and the column sums   second, all three
-//   65536 x 512 bf16       25 us (26.7)   35 (40)            41                    84 (67)
+//   65536 x 512 bf16       22-25 (26.7)   35 (40)            41                    84 (67)
 //   16384 x 512 bf16       7.7 (6.7)      11 (10)            17                    23 (17)
 //   131072 x 128 bf16      12.6 (13.4)    18 (20)            24                    34 (33)
 //   4099 x 1001 fp32       7.7 (6.5)      12 (10)            21                    23 (16)
